@@ -35,7 +35,7 @@ enum tbf16_status {
   TBF16_ERR_TIMEOUT = 7      /* a kernel gave up on a bounded wait (see tbf16_device_status) */
 };
 
-enum tbf16_dtype { TBF16_BF16 = 0, TBF16_F16 = 1 };
+enum tbf16_dtype { TBF16_BF16 = 0, TBF16_F16 = 1, TBF16_E4M3 = 2 };
 
 /* ------------------------------------------------------------------ library */
 
@@ -47,7 +47,9 @@ const char* tbf16_status_string(int status);
 int tbf16_device_check(int device);
 /* Bits set by kernels on the current device since the last reset (1 = a bounded wait timed out,
  * 2 = attention backward produced a non-finite value, 4 = a kernel found its dynamic shared memory
- * window not 1024-byte aligned and did nothing). Synchronises the device; reset != 0 clears. */
+ * window not 1024-byte aligned and did nothing, 8 = a paged-cache call met a page number, length or
+ * count outside its tables and left those rows out or read them as page 0). Synchronises the device;
+ * reset != 0 clears. */
 int tbf16_device_status(unsigned int* bits, int reset);
 /* Failure-path self-test (no counterpart in the reference): one warp waits on an mbarrier that nothing
  * arrives on, through the bounded-wait helper the pipelined kernels use, with the limit timeout_ns
@@ -397,6 +399,76 @@ int tbf16_attn_bwd_sharded(const void* q16, const void* k16, const void* v16, co
                            int64_t mask_sh, int64_t mask_sq, int t_do, void* dq, void* dk, void* dv, int32_t* G_out,
                            unsigned int* flag, void* ws, int64_t ws_bytes, float dropout_p, uint64_t seed,
                            const int32_t* e_global, void* stream);
+
+/* ------------------------------------------------------------------ paged key/value cache (serving)
+ *
+ * No counterpart in the reference, which leaves token-by-token decoding to torch (its
+ * MIN_QUERY_ROWS, tbf16/convert.py). A cache of one layer: pages of page_size token slots, each slot one
+ * row of D values per key/value head, bf16 or e4m3. An e4m3 row is its bf16 row times a power of two that
+ * takes the row's largest magnitude to [128, 256), and its inverse scale stands in k_scale / v_scale
+ * (a zero row has 1, a row that holds an infinity or NaN has NaN). Sequence b's token j sits in slot
+ * j % page_size of page table[b * table_ld + j / page_size]; lens[b] tokens are cached. table, lens and
+ * counts are read on the device, so a captured graph follows their contents.
+ *
+ * Limits: D 64, 128 or 256 (zero-pad others); page_size a power of two from 16 to 1024; batch up to 1024;
+ * pointers and strides multiples of 16 bytes (scales: 16-byte pointers, strides multiples of 4 floats,
+ * the page_size scales of a (page, head) contiguous). Page numbers outside [0, pages), lengths outside
+ * [0, max_pages * page_size] and counts outside [0, min(T, lens)] set bit 8 of the device status word. */
+typedef struct tbf16_paged_cache {
+  void* k;              /* [pages, heads, page_size, D], last dimension contiguous */
+  void* v;
+  float* k_scale;       /* TBF16_E4M3: [pages, heads, page_size] inverse scales; else NULL */
+  float* v_scale;
+  const int32_t* table; /* [batch, max_pages] */
+  const int32_t* lens;  /* [batch] */
+  int64_t k_sp, k_sh, k_ss, v_sp, v_sh, v_ss; /* element strides of page, head, slot */
+  int64_t ks_sp, ks_sh, vs_sp, vs_sh;         /* element strides of the scales' page, head */
+  int64_t table_ld;
+  int64_t batch, heads, D, page_size, pages, max_pages;
+  int64_t dtype; /* TBF16_BF16 or TBF16_E4M3 */
+} tbf16_paged_cache;
+
+/* Writes the newest rows of every sequence into its pages: k, v bf16 (batch, heads, T, d) with element
+ * strides of batch, head, token and contiguous last dimension, d <= D a multiple of 8 (the cache row's
+ * remaining columns are zeroed). lens counts the new tokens already: token t < counts[b] goes to position
+ * lens[b] - counts[b] + t (counts NULL: min(T, lens[b]) each). pos (nullable): int32 (batch, heads, capacity) with
+ * strides pos_sb, pos_sh; position j of every head receives seen[b] - counts[b] + t, the token's number
+ * in the whole sequence, where seen[b] counts all tokens ever appended. */
+int tbf16_paged_append(const tbf16_paged_cache* cache, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                       const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int64_t T, int64_t d,
+                       const int32_t* counts, int32_t* pos, int64_t pos_sb, int64_t pos_sh, const int32_t* seen,
+                       void* stream);
+
+/* Attention of the newest T tokens of every sequence over its cache. q bf16 (batch, Hq, T, D), out bf16
+ * of the same shape, element strides of batch, head, token, contiguous last dimension, 16-byte rows;
+ * Hq a multiple of heads (query head h reads key/value head h / (Hq / heads)). Token t < counts[b]
+ * (NULL: min(T, lens[b])) sits at position i = lens[b] - counts[b] + t and sees the cached positions j
+ * with i - window < j <= i (window 0: all j <= i). Rows that see nothing, and tokens t >= counts[b], give zeros.
+ * weights (nullable): fp32 (batch, heads, capacity) with strides w_sb, w_sh; the softmax weight of every
+ * visible position, summed over the head's query heads and the new tokens, is added to it.
+ * sync: tbf16_paged_attend_sync_size() bytes that are zero before the first call; every call leaves them
+ * zero. ws: tbf16_paged_attend_ws_size() bytes. Neither is shared with a concurrent call. */
+int64_t tbf16_paged_attend_ws_size(const tbf16_paged_cache* cache, int64_t Hq, int64_t T, int with_weights);
+int64_t tbf16_paged_attend_sync_size(const tbf16_paged_cache* cache, int64_t Hq, int64_t T);
+int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                       int64_t Hq, int64_t T, const int32_t* counts, float scale, int64_t window, void* out,
+                       int64_t out_sb, int64_t out_sh, int64_t out_st, float* weights, int64_t w_sb, int64_t w_sh,
+                       void* sync, void* ws, int64_t ws_bytes, void* stream);
+
+/* Cuts every sequence longer than `keep` to the `keep` positions of each head that carry the largest
+ * weights; the newest `recent` tokens (pos >= seen[b] - recent) rank above every weight, ties go to the
+ * lowest position, a NaN weight ranks highest. Kept positions below `keep` stay where they are; the i-th
+ * position below `keep` that is given up receives the i-th kept position at or beyond `keep`: its key and
+ * value rows (and scales) are copied within the pages. weights, pos: (batch, heads, cols) with strides
+ * *_sb, *_sh; weights_out, pos_out: contiguous (batch, heads, cols), the weights and token numbers in the
+ * new order, 0 and -1 from min(lens, keep) on; they may not overlap weights and pos. lens is not written:
+ * the caller takes min(lens, keep) once every layer is done. Pages may not be shared between sequences.
+ * ws: tbf16_paged_compact_ws_size() bytes, not shared with a concurrent call. */
+int64_t tbf16_paged_compact_ws_size(const tbf16_paged_cache* cache, int64_t cols, int64_t keep);
+int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* weights, int64_t w_sb, int64_t w_sh,
+                        const int32_t* pos, int64_t pos_sb, int64_t pos_sh, int64_t cols, const int32_t* seen,
+                        int64_t keep, int64_t recent, float* weights_out, int32_t* pos_out, void* ws,
+                        int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,7 @@ namespace tbf16 {
 constexpr unsigned int kErrWaitTimeout = 1u;
 constexpr unsigned int kErrOverflow = 2u;
 constexpr unsigned int kErrSmemAlign = 4u;  // dynamic shared window not 1024-byte aligned
+constexpr unsigned int kErrPage = 8u;       // paged cache: page number, length or count outside its tables
 
 // ------------------------------------------------------------------ scale rules
 // The scale is an exact power of two built from exponent bits, never exp2/log2.

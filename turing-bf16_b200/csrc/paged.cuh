@@ -1,0 +1,47 @@
+// The paged key/value cache as the kernels see it, and the lookups they share. Layout and limits:
+// tbf16_paged_cache in include/tbf16_sm100.h.
+#pragma once
+#include "common.cuh"
+
+namespace tbf16 {
+
+struct PagedView {
+  uint8_t* k;  // rows of D bf16 or e4m3 values; strides below in bytes
+  uint8_t* v;
+  float* k_scale;  // e4m3: inverse row scales; strides in floats
+  float* v_scale;
+  const int* table;
+  const int* lens;
+  int64_t k_sp, k_sh, k_ss, v_sp, v_sh, v_ss, ks_sp, ks_sh, vs_sp, vs_sh, table_ld;
+  int64_t pages;
+  int batch, heads, page_shift, max_pages, cap;  // cap = max_pages << page_shift, below 2^31
+  unsigned int* err;
+};
+
+// Cached tokens of sequence b, held inside [0, cap].
+__device__ __forceinline__ int paged_len(const PagedView& c, int b) {
+  const int n = c.lens[b];
+  if (n < 0 || n > c.cap) atomicOr(c.err, kErrPage);
+  return min(max(n, 0), c.cap);
+}
+// New tokens of sequence b, held inside [0, min(T, len)] (counts null: that many).
+__device__ __forceinline__ int paged_count(const PagedView& c, const int* counts, int b, int T, int len) {
+  const int n = counts ? counts[b] : min(T, len);
+  if (n < 0 || n > T || n > len) atomicOr(c.err, kErrPage);
+  return min(max(n, 0), min(T, len));
+}
+// Page that holds position j of sequence b, or -1 (with the error bit set) for a number outside the pool.
+__device__ __forceinline__ int paged_page(const PagedView& c, int b, int j) {
+  const int id = c.table[b * c.table_ld + (j >> c.page_shift)];
+  if (id >= 0 && id < c.pages) return id;
+  atomicOr(c.err, kErrPage);
+  return -1;
+}
+__device__ __forceinline__ int paged_slot(const PagedView& c, int j) { return j & ((1 << c.page_shift) - 1); }
+
+}  // namespace tbf16
+
+namespace tbf16_host {
+// Checks a tbf16_paged_cache and fills the device view; TBF16_OK or the status to return.
+int paged_view(const tbf16_paged_cache* cache, tbf16::PagedView* view);
+}  // namespace tbf16_host

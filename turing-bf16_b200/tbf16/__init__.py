@@ -10,7 +10,8 @@ from . import autograd, ops
 from .attention import sdpa
 from .convert import Linear, TrainLinear, convert, install_sdpa, is_supported_gpu, uninstall_sdpa
 from .ops import prepare_weight, quantize_rows, scaled_linear
+from .paged import PagedCache
 from .patch import TuringBF16Mode, patch
 
 __all__ = ["quantize_rows", "scaled_linear", "prepare_weight", "sdpa", "patch", "TuringBF16Mode", "convert",
-           "Linear", "TrainLinear", "autograd", "install_sdpa", "uninstall_sdpa", "is_supported_gpu"]
+           "Linear", "TrainLinear", "PagedCache", "autograd", "install_sdpa", "uninstall_sdpa", "is_supported_gpu"]

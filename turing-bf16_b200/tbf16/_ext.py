@@ -73,6 +73,10 @@ SIGNATURES = {
     "tbf16_attn_bwd_sharded": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                _i64, _i64, _i64, ctypes.c_float, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp,
                                _vp, _vp, _i64, ctypes.c_float, ctypes.c_uint64, _vp, _vp],
+    "tbf16_paged_append": [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp],
+    "tbf16_paged_attend": [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_float, _i64, _vp, _i64, _i64, _i64, _vp,
+                           _i64, _i64, _vp, _vp, _i64, _vp],
+    "tbf16_paged_compact": [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
     "tbf16_device_check": [_i32],
     "tbf16_device_status": [_vp, _i32],
     "tbf16_selftest_bounded_wait": [ctypes.c_uint64, _vp],
@@ -82,12 +86,22 @@ SIGNATURES = {
 SIGNATURES_I64 = {
     "tbf16_attn_bwd_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64],
     "tbf16_attn_fwd_ws_size": [_i64, _i64, _i64, _i64, _i64, _i64, _i32],
+    "tbf16_paged_attend_ws_size": [_vp, _i64, _i64, _i32],
+    "tbf16_paged_attend_sync_size": [_vp, _i64, _i64],
+    "tbf16_paged_compact_ws_size": [_vp, _i64, _i64],
 }
 
-BF16, F16 = 0, 1
+BF16, F16, E4M3 = 0, 1, 2
 STATUS = {1: "invalid argument", 2: "misaligned pointer or leading dimension", 3: "unsupported dtype",
           4: "CUDA launch error", 5: "not an sm_100 (B200) GPU", 6: "unsupported by this build",
           7: "kernel timed out on a bounded wait"}
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """tbf16_paged_cache of include/tbf16_sm100.h."""
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale", "table", "lens")]
+                + [(n, _i64) for n in ("k_sp", "k_sh", "k_ss", "v_sp", "v_sh", "v_ss", "ks_sp", "ks_sh", "vs_sp", "vs_sh",
+                                       "table_ld", "batch", "heads", "D", "page_size", "pages", "max_pages", "dtype")])
 
 
 def _build_module():
