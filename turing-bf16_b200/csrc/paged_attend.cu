@@ -1,10 +1,46 @@
-// Attention of the newest tokens over a paged key/value cache.
+// Attention of the newest tokens over a paged key/value cache (decoding): tbf16_paged_attend.
 #include <cuda_fp8.h>
+
+#include <algorithm>
 
 #include "paged.cuh"
 
 namespace {
 using namespace tbf16;
+
+// For a query row r of a key/value head (T new tokens x the head's group of query heads)
+//   s_j = (q_r . k_j) scale,  out_r = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  m = max_j s_j
+// over the visible positions j. Every cached byte is used by 2 T group flops per element, 2..64 in practice
+// against the ~260 per byte the tensor cores could do: the time is the cache's bytes over the HBM rate, as long
+// as enough bytes are in flight on every SM, however few or uneven the sequences.
+//
+// Work split. The keys of a (sequence, head, 16 query rows) item are cut into blocks of BK keys; the blocks of
+// all items, laid end to end, are shared out evenly over the CTAs (one per SM), from the lengths on the device:
+// ragged batches and one long sequence keep all SMs equally busy, and a captured graph follows the lengths. A
+// CTA's blocks go round-robin to its warps. Each warp is a pipeline of its own: it issues the TMA loads of its
+// blocks into its own ring of stages, waits for them, and keeps its own running maximum, sum and output in
+// registers (mma.sync m16n8k16: with 16 query rows a tile, tcgen05's 128-row tile would be seven eighths empty,
+// and the tensor work is far from the bound), so the warps never wait for one another inside an item. At its
+// end they are added up through shared memory. An item that spans CTAs leaves one partial (output, maximum,
+// sum) per CTA in the workspace; the CTA that arrives last adds them in a fixed order, so results do not depend
+// on which one that is.
+constexpr int kRows = 16;      // query rows of an item: one m16n8k16 tile
+constexpr int kMaxStages = 8;
+
+template <int D_, bool E4M3_>
+struct Tile {
+  static constexpr int D = D_;
+  static constexpr bool E4M3 = E4M3_;
+  static constexpr int RB = D * (E4M3 ? 1 : 2);              // bytes of a cached row
+  static constexpr int AW = RB < 128 ? RB : 128;             // swizzle span: 64 or 128 bytes
+  static constexpr int NA = RB / AW;                         // spans of a row
+  static constexpr int BK = RB <= 64 ? 64 : RB <= 128 ? 32 : 16;  // keys of a block
+  static constexpr int NG = BK / 16;                         // groups of 16 keys, one TMA box each
+  static constexpr int GB = 16 * RB;                         // bytes of a group: [NA][16 keys][AW]
+  static constexpr int KB = NG * GB;                         // bytes of a block's keys (or values)
+  static constexpr int W = RB == 512 ? 4 : 8;                // warps
+  static constexpr int SC = E4M3 ? 2 * BK * 4 : 0;           // bytes of a block's scales
+};
 
 struct AttendParams {
   PagedView c;
@@ -13,89 +49,713 @@ struct AttendParams {
   __nv_bfloat16* out;
   int64_t o_sb, o_sh, o_st;
   const int* counts;
-  float* weights;
-  int64_t w_sb, w_sh;
-  int T, group, window;
+  int T, group, rows, chunks, window;  // rows = T * group query rows of a head, in chunks of kRows
   float scale_log2;
+  int stages;
+  int nr;           // rows of an item that can be real: min(rows, kRows)
+  unsigned* sync;   // arrivals of each item, zero between calls
+  float* part;      // [2 * CTAs][nr * D + 3 * kRows]: partial outputs, maxima, sums
+  float* logits;    // weights wanted: [batch * heads][rows][cap], base-2 logits
+  float* lse;       // and [batch * heads][rows]: log2 of each row's sum
 };
 
+// What a CTA knows of a sequence: first of its blocks among all, blocks of one item, cached and new tokens.
+struct SeqInfo {
+  int cum, blocks, len, count;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two e4m3 values (the low or high half of v) as packed fp16, exactly.
+__device__ __forceinline__ uint32_t e4m3_f16(uint32_t v, bool high) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(high ? v >> 16 : v & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+// Packed e4m3 or bf16 values with infinities and NaNs replaced by zeros.
 template <bool E4M3>
-__device__ __forceinline__ float cached(const uint8_t* row, int i) {
-  if (E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw(row[i], __NV_E4M3)));
-  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[i]);
+__device__ __forceinline__ void finite_only(uint32_t (&r)[4]) {
+#pragma unroll
+  for (uint32_t& w : r) {
+    if (E4M3) w &= ~__vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+    else w &= ~__vcmpeq2(w & 0x7f807f80u, 0x7f807f80u);
+  }
+}
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2, int c3,
+                                            int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// One block per (sequence, key/value head); its query rows one after another, 128 keys at a time with the
-// running maximum and sum of an online softmax.
-template <int D, bool E4M3>
-__global__ void __launch_bounds__(128) attend_kernel(const AttendParams p) {
-  __shared__ float q[D], prob[128], red[4];
-  const int b = blockIdx.x / p.c.heads, h = blockIdx.x % p.c.heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int len = paged_len(p.c, b), n = paged_count(p.c, p.counts, b, p.T, len);
-  for (int r = 0; r < p.T * p.group; ++r) {
-    const int t = r / p.group, head = h * p.group + r % p.group;
+// Byte offset of 16-byte chunk `chunk` of key `row` inside a group, as TMA's swizzle places it.
+template <class C>
+__device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
+  if (C::AW == 128) return (chunk >> 3) * 2048 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+  return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+// Where a warp's next block lies: position t in the order of all blocks, and the item it belongs to.
+struct Cursor {
+  int t, b, h, j0, len;  // first key of the block; cached tokens (0 past the end of the warp's blocks)
+  int page;              // this lane's page of the block, loaded ahead
+};
+
+template <class C>
+struct Kernel {
+  static constexpr bool E4M3 = C::E4M3;
+
+  // Moves the cursor to the warp's next block with anything to load, from position t on, and starts loading
+  // the page numbers that block needs (lane = group + NG * {keys, values, key scales, value scales}).
+  static __device__ void seek(Cursor& u, int t, int end, const SeqInfo* info, const AttendParams& p, int lane) {
+    for (;; t += C::W) {
+      u.t = t;
+      u.len = 0;
+      if (t >= end) return;
+      while (t >= info[u.b + 1].cum) ++u.b;
+      const SeqInfo s = info[u.b];
+      if (s.count == 0) continue;
+      const unsigned rem = t - s.cum, item = rem / (unsigned)s.blocks;
+      u.h = (int)(item / (unsigned)p.chunks);
+      const int lo = p.window ? max(0, s.len - s.count + 1 - p.window) / C::BK : 0;
+      u.j0 = (lo + (int)(rem - item * s.blocks)) * C::BK;
+      u.len = s.len;
+      break;
+    }
+    const int j = u.j0 + (lane % C::NG) * 16;
+    u.page = lane < (E4M3 ? 4 : 2) * C::NG && j < u.len ? p.c.table[u.b * p.c.table_ld + (j >> p.c.page_shift)] : 0;
+  }
+
+  static __device__ void load(const Cursor& u, uint8_t* stage, float* scales, uint64_t* bar, const CUtensorMap* km,
+                              const CUtensorMap* vm, const AttendParams& p, int lane) {
+    const int groups = min(C::NG, (u.len - u.j0 + 15) >> 4);
+    if (lane == 0) mbar_arrive_expect_tx(bar, groups * (2 * C::GB + (E4M3 ? 128 : 0)));
+    __syncwarp();
+    const int g = lane % C::NG, kind = lane / C::NG, slot = paged_slot(p.c, u.j0 + g * 16);
+    if (g >= groups) return;
+    int page = u.page;
+    if (page < 0 || page >= p.c.pages) {
+      atomicOr(p.c.err, kErrPage);
+      page = 0;
+    }
+    if (kind == 0) tma_load_5d(stage + g * C::GB, km, bar, 0, slot, 0, u.h, page);
+    if (kind == 1) tma_load_5d(stage + C::KB + g * C::GB, vm, bar, 0, slot, 0, u.h, page);
+    if (E4M3 && kind == 2) bulk_load(scales + g * 16, p.c.k_scale + page * p.c.ks_sp + u.h * p.c.ks_sh + slot, 64, bar);
+    if (E4M3 && kind == 3)
+      bulk_load(scales + C::BK + g * 16, p.c.v_scale + page * p.c.vs_sp + u.h * p.c.vs_sh + slot, 64, bar);
+  }
+};
+
+// Shared memory: [rings][scales][merge outputs][info][factors ...]; sizes in attend_smem().
+template <class C>
+__global__ void __launch_bounds__(C::W * 32, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm, const AttendParams p) {
+  constexpr int D = C::D, NT = D / 8, W = C::W, NG = C::NG, KS = D / 16;
+  constexpr bool E4M3 = C::E4M3;
+  using K = Kernel<C>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* ring = smem;
+  float* scale_ring = reinterpret_cast<float*>(ring + (size_t)W * p.stages * 2 * C::KB);
+  float* merge = scale_ring + (size_t)W * p.stages * (C::SC / 4);
+  SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + W * p.nr * D);
+  __shared__ uint64_t bars[W * kMaxStages];
+  __shared__ float s_m[W][kRows], s_l[W][kRows], s_mv[W][kRows];  // each warp's maxima and sums, then factors
+  __shared__ float s_top[kRows], s_sum[kRows];
+  __shared__ int s_scan[W], s_abort, s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (tid == 0) atomicOr(p.c.err, kErrSmemAlign);
+    return;
+  }
+  pdl_launch_dependents();
+
+  // every sequence's blocks, and their running total
+  int carry = 0;
+  for (int b0 = 0; b0 < p.c.batch; b0 += W * 32) {
+    const int b = b0 + tid;
+    SeqInfo s{0, 0, 0, 0};
+    int mine = 0;
+    if (b < p.c.batch) {
+      s.len = paged_len(p.c, b);
+      s.count = paged_count(p.c, p.counts, b, p.T, s.len);
+      const int lo = p.window ? max(0, s.len - s.count + 1 - p.window) / C::BK : 0;
+      s.blocks = s.count ? (s.len + C::BK - 1) / C::BK - lo : 1;  // one empty block writes an idle sequence's zeros
+      mine = s.blocks * p.c.heads * p.chunks;
+    }
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_scan[warp] = x;
     __syncthreads();
-    for (int i = tid; i < D; i += 128)
-      q[i] = __bfloat162float(p.q[b * p.q_sb + head * p.q_sh + t * p.q_st + i]) * p.scale_log2;
-    const int last = t < n ? len - n + t : -1, first = p.window ? max(0, last - p.window + 1) : 0;
-    float m = -INFINITY, l = 0.f, acc[(D + 127) / 128] = {};
-    for (int pass = 0; pass < (p.weights ? 2 : 1); ++pass) {
-      for (int j0 = first; j0 <= last; j0 += 128) {
-        const int j = j0 + tid;
-        float s = -INFINITY;
-        __syncthreads();
-        const int page = j <= last ? paged_page(p.c, b, j) : -1;
-        const int slot = paged_slot(p.c, j);
-        if (page >= 0) {
-          const uint8_t* row = p.c.k + page * p.c.k_sp + h * p.c.k_sh + slot * p.c.k_ss;
-          s = 0.f;
-          for (int i = 0; i < D; ++i) s += q[i] * cached<E4M3>(row, i);
-          if (E4M3) s *= p.c.k_scale[page * p.c.ks_sp + h * p.c.ks_sh + slot];
+    int before = carry, total = carry;
+    for (int i = 0; i < W; ++i) {
+      before += i < warp ? s_scan[i] : 0;
+      total += s_scan[i];
+    }
+    s.cum = before + x - mine;
+    if (b < p.c.batch) info[b] = s;
+    if (b == p.c.batch - 1) info[b + 1] = SeqInfo{before + x, 1, 0, 0};
+    carry = total;
+    __syncthreads();
+  }
+  const int total = carry;
+  // no more CTAs than give every warp a block
+  const int ctas = min((int)gridDim.x, (total + W - 1) / W);
+  if ((int)blockIdx.x >= ctas) return;
+  const int c0 = (int)((int64_t)total * blockIdx.x / ctas), c1 = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
+
+  if (tid == 0) {
+    for (int i = 0; i < W * p.stages; ++i) mbar_init(&bars[i], 1);
+    s_abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&km);
+    tma_prefetch_desc(&vm);
+  }
+  __syncthreads();
+  uint8_t* my_ring = ring + (size_t)warp * p.stages * 2 * C::KB;
+  float* my_scales = scale_ring + (size_t)warp * p.stages * (C::SC / 4);
+  uint64_t* my_bars = bars + warp * p.stages;
+  Cursor u;
+  u.b = 0;
+  int issued = 0, waiting = 0;  // blocks issued and not consumed yet
+  auto issue = [&]() {
+    K::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p, lane);
+    issued = issued + 1 == p.stages ? 0 : issued + 1;
+    ++waiting;
+    K::seek(u, u.t + W, c1, info, p, lane);
+  };
+  K::seek(u, c0 + warp, c1, info, p, lane);
+  while (waiting < p.stages && u.len) issue();
+  int stage = 0, phase = 0;
+  bool dead = false;  // a wait gave up: nothing more is loaded or computed, every barrier is still reached
+
+  const int g4 = lane >> 2, c4 = lane & 3;
+  // this lane's row and chunk offset in the ldmatrix of keys and of values
+  const int k_row = E4M3 ? lane & 15 : ((lane >> 4) & 1) * 8 + (lane & 7), k_ch = E4M3 ? lane >> 4 : (lane >> 3) & 1;
+  const int v_row = lane & 15, v_ch = lane >> 4;
+
+  int b = 0;
+  for (int t = c0; t < c1;) {
+    while (t >= info[b + 1].cum) ++b;
+    const SeqInfo s = info[b];
+    const int item = (t - s.cum) / s.blocks, start = s.cum + item * s.blocks, end = min(c1, start + s.blocks);
+    const int h = item / p.chunks, row0 = (item % p.chunks) * kRows;
+    const int nrow = min(kRows, p.rows - row0);
+    const int lo = p.window ? max(0, s.len - s.count + 1 - p.window) / C::BK : 0;
+    // query rows g4 and g4 + 8 of the item: their A fragments and positions
+    uint32_t qf[KS][4];
+    float mul[2];
+    int at[2];  // position of the row's token; -1: the row is not there
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = row0 + g4 + i * 8, tok = r / p.group;
+      const bool there = r < p.rows && tok < s.count;
+      at[i] = there ? s.len - s.count + tok : -1;
+      const __nv_bfloat16* q = p.q + b * p.q_sb + (int64_t)(h * p.group + r % p.group) * p.q_sh + tok * p.q_st;
+      mul[i] = p.scale_log2;
+      if (E4M3) {
+        // fp16 rows: the largest magnitude to [2^14, 2^15) by a power of two, undone in the logits' factor. In
+        // column 16 k + 4 c of a k16 step sit the two pairs the byte order of a cached row puts there.
+        uint2 x[KS];
+        unsigned m = 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          x[k] = there ? *reinterpret_cast<const uint2*>(q + k * 16 + c4 * 4) : make_uint2(0, 0);
+          m = max(m, max(max((x[k].x << 16) & 0x7fffffffu, x[k].x & 0x7fff0000u),
+                         max((x[k].y << 16) & 0x7fffffffu, x[k].y & 0x7fff0000u)));
         }
-        if (pass == 1) {
-          if (page >= 0) p.weights[b * p.w_sb + h * p.w_sh + j] += exp2f(s - m) / l;
-          continue;
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = m == 0 || m >= 0x7f800000u ? 15 : max(frexp_exp(__uint_as_float(m)), -110);
+        const float f = exp2i(15 - e);
+        mul[i] *= exp2i(e - 15);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          qf[k][i] = pack_f16(bf16lo(x[k].x) * f, bf16hi(x[k].x) * f);
+          qf[k][2 + i] = pack_f16(bf16lo(x[k].y) * f, bf16hi(x[k].y) * f);
         }
-        float mx = warp_max(s);
-        if (lane == 0) red[warp] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-        const float base = mx == -INFINITY ? 0.f : mx, fac = exp2f(m - base), pr = page >= 0 ? exp2f(s - base) : 0.f;
-        m = mx;
-        prob[tid] = pr;
-        __syncthreads();
-        l *= fac;
-        for (int i = 0; i < 128; ++i) l += prob[i];
-        for (int e = 0; e * 128 + tid < D; ++e) acc[e] *= fac;
-        for (int i = 0; i < 128 && j0 + i <= last; ++i) {
-          const int pg = paged_page(p.c, b, j0 + i);
-          if (pg < 0) continue;
-          const int sl = paged_slot(p.c, j0 + i);
-          const float sv = E4M3 ? p.c.v_scale[pg * p.c.vs_sp + h * p.c.vs_sh + sl] : 1.f;
-          const uint8_t* row = p.c.v + pg * p.c.v_sp + h * p.c.v_sh + sl * p.c.v_ss;
-          for (int e = 0; e * 128 + tid < D; ++e) acc[e] += prob[i] * (cached<E4M3>(row, e * 128 + tid) * sv);
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          qf[k][i] = there ? *reinterpret_cast<const uint32_t*>(q + k * 16 + c4 * 2) : 0u;
+          qf[k][2 + i] = there ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + c4 * 2) : 0u;
         }
       }
     }
-    for (int e = 0; e * 128 + tid < D; ++e)
-      p.out[b * p.o_sb + head * p.o_sh + t * p.o_st + e * 128 + tid] = __float2bfloat16(l == 0.f ? 0.f : acc[e] / l);
+    float o[NT][4] = {};
+    float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int pos_min = s.len - s.count, pos_max = s.len - 1;
+
+    const int first = t + (warp - (t - c0) % W + W) % W;
+    for (int x = first; x < end && s.count; x += W) {
+      if (dead || !mbar_wait_warp(&my_bars[stage], phase, &s_abort, p.c.err)) {
+        dead = true;
+        break;
+      }
+      const uint32_t kb = smem_u32(my_ring + (size_t)stage * 2 * C::KB), vb = kb + C::KB;
+      const float* ksc = my_scales + stage * (C::SC / 4);
+      const int j0 = (lo + x - start) * C::BK;
+      const int groups = min(NG, (s.len - j0 + 15) >> 4);
+      float sc[NG][2][4];
+      // logits of 16 query rows x BK keys, in units of log 2
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[g][n][e] = 0.f;
+        if (g >= groups) continue;
+        const uint32_t base = kb + g * C::GB;
+        if (E4M3) {
+#pragma unroll
+          for (int k = 0; k < KS; k += 2) {
+            uint32_t r[4];
+            ldsm4(r, base + chunk_at<C>(k_row, k + k_ch));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // r[0], r[1]: keys 0-7 and 8-15 of chunk k; r[2], r[3]: of chunk k + 1
+              mma16<true>(sc[g][i & 1], qf[k + (i >> 1)], e4m3_f16(r[i], false), e4m3_f16(r[i], true));
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            uint32_t r[4];
+            ldsm4(r, base + chunk_at<C>(k_row, 2 * k + k_ch));
+            mma16<false>(sc[g][0], qf[k], r[0], r[1]);
+            mma16<false>(sc[g][1], qf[k], r[2], r[3]);
+          }
+        }
+      }
+      float top[2] = {m[0], m[1]}, topv[2] = {mv[0], mv[1]};
+      float ev[NG][2][2];  // e4m3: log2 of the value rows' scales (NaN for a row that reads as NaN)
+      unsigned masked = 0;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int jg = j0 + g * 16;
+        const bool whole = g < groups && jg + 15 <= pos_min && (!p.window || jg > pos_max - p.window);
+        if (!whole) masked |= 1u << g;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float2 ks = make_float2(1.f, 1.f);
+          if (E4M3) {
+            ks = *reinterpret_cast<const float2*>(ksc + g * 16 + n * 8 + c4 * 2);
+            const float2 vs = *reinterpret_cast<const float2*>(ksc + C::BK + g * 16 + n * 8 + c4 * 2);
+            ev[g][n][0] = (float)(int)((__float_as_uint(vs.x) >> 23) & 255u) - 127.f + vs.x * 0.f;
+            ev[g][n][1] = (float)(int)((__float_as_uint(vs.y) >> 23) & 255u) - 127.f + vs.y * 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = sc[g][n][e] * mul[e >> 1];
+            if (E4M3) v *= (e & 1) ? ks.y : ks.x;
+            if (!whole) {
+              const int j = jg + n * 8 + c4 * 2 + (e & 1), i = at[e >> 1];
+              const bool see = j <= i && (!p.window || j > i - p.window);
+              v = see ? v : -INFINITY;
+            }
+            sc[g][n][e] = v;
+            top[e >> 1] = fmaxf(top[e >> 1], v);
+            if (E4M3) topv[e >> 1] = fmaxf(topv[e >> 1], v == -INFINITY ? v : v + ev[g][n][e & 1]);
+          }
+          if (p.logits && g < groups) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (at[i] >= 0)
+                *reinterpret_cast<float2*>(p.logits + ((int64_t)(b * p.c.heads + h) * p.rows + row0 + g4 + i * 8) * p.c.cap +
+                                           jg + n * 8 + c4 * 2) = make_float2(sc[g][n][2 * i], sc[g][n][2 * i + 1]);
+          }
+        }
+      }
+      // running maxima: m for the sum; e4m3 also keeps mv, of logit + log2(value scale), for the output, so that
+      // fp16 weights times e4m3 values cannot overflow whatever the rows' scales are
+      float fac[2];
+      bool grew = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = quad_max(top[i]);
+        if (E4M3) topv[i] = quad_max(topv[i]);
+        const float base = top[i] == -INFINITY ? 0.f : top[i];
+        l[i] *= ex2(m[i] - base);
+        const float was = E4M3 ? mv[i] : m[i], now = E4M3 ? topv[i] : top[i];
+        fac[i] = ex2(was - (now == -INFINITY ? 0.f : now));
+        grew |= now != was;
+        m[i] = top[i];
+        mv[i] = topv[i];
+        top[i] = base;
+        topv[i] = topv[i] == -INFINITY ? 0.f : topv[i];
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][e] *= fac[e >> 1];
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        if (g >= groups) continue;
+        float pw[2][4];  // weights for the output
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = sc[g][n][e], w = ex2(v - top[e >> 1]);
+            l[e >> 1] += w;
+            pw[n][e] = !E4M3 ? w : v == -INFINITY ? 0.f : ex2(v + ev[g][n][e & 1] - topv[e >> 1]);
+          }
+        const uint32_t base = vb + g * C::GB;
+        bool odd = false;
+        if ((masked >> g) & 1) {
+          // A masked weight is 0, but 0 x NaN is not: if the values of a partly masked group hold infinities or
+          // NaNs (stale slots, a later token's), those are added here, to the rows that see them, and are zeros in
+          // the products below; all other bits of the result stay what they are without them.
+          for (int i = lane; i < C::GB / 16; i += 32) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(base + i * 16));
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              odd |= E4M3 ? __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0
+                          : (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
+          }
+          odd = __any_sync(0xffffffffu, odd);
+          if (odd) {
+            for (int k = 0; k < 16; ++k) {
+              const int from = (lane & ~3) | ((k & 7) >> 1), j = j0 + g * 16 + k;
+              float w[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float a = __shfl_sync(0xffffffffu, pw[0][2 * i + 0], from), c = __shfl_sync(0xffffffffu, pw[0][2 * i + 1], from);
+                const float d = __shfl_sync(0xffffffffu, pw[1][2 * i + 0], from), f = __shfl_sync(0xffffffffu, pw[1][2 * i + 1], from);
+                w[i] = k < 8 ? (k & 1 ? c : a) : (k & 1 ? f : d);
+              }
+              const bool see0 = j <= at[0] && (!p.window || j > at[0] - p.window);
+              const bool see1 = j <= at[1] && (!p.window || j > at[1] - p.window);
+#pragma unroll
+              for (int n = 0; n < NT; n += E4M3 ? 2 : 1) {
+                uint32_t v;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(base + chunk_at<C>(k, E4M3 ? n / 2 : n) + c4 * 4));
+                if (E4M3) {
+                  const uint32_t lo2 = e4m3_f16(v, false), hi2 = e4m3_f16(v, true);
+                  const float x4[4] = {f16lo(lo2), f16hi(lo2), f16lo(hi2), f16hi(hi2)};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    float(&t4)[4] = o[n + (e & 1)];
+                    if (see0 && !isfinite(x4[e])) t4[e >> 1] += w[0] * x4[e];
+                    if (see1 && !isfinite(x4[e])) t4[2 + (e >> 1)] += w[1] * x4[e];
+                  }
+                } else {
+                  const float x2[2] = {bf16lo(v), bf16hi(v)};
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    if (see0 && !isfinite(x2[e])) o[n][e] += w[0] * x2[e];
+                    if (see1 && !isfinite(x2[e])) o[n][2 + e] += w[1] * x2[e];
+                  }
+                }
+              }
+            }
+          }
+        }
+        if (E4M3) {
+          // fp16 weights: 11 bits, on values that are exact in fp16
+          const uint32_t a[4] = {pack_f16(pw[0][0], pw[0][1]), pack_f16(pw[0][2], pw[0][3]), pack_f16(pw[1][0], pw[1][1]),
+                                 pack_f16(pw[1][2], pw[1][3])};
+#pragma unroll
+          for (int k = 0; k < KS; k += 2) {
+            uint32_t r[4];
+            ldsm4t(r, base + chunk_at<C>(v_row, k + v_ch));
+            if (odd) finite_only<E4M3>(r);
+            // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: pair the keys, one tile for the even
+            // columns of the chunk, one for the odd ones
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x0 = __byte_perm(r[2 * i], 0, 0x3120), x1 = __byte_perm(r[2 * i + 1], 0, 0x3120);
+              mma16<true>(o[2 * (k + i)], a, e4m3_f16(x0, false), e4m3_f16(x1, false));
+              mma16<true>(o[2 * (k + i) + 1], a, e4m3_f16(x0, true), e4m3_f16(x1, true));
+            }
+          }
+        } else {
+          // bf16 weights in two parts (16 bits of them): one part would add its 2^-9 to the output's own rounding
+          uint32_t hi[4], lw[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = pw[i >> 1][2 * (i & 1)], y = pw[i >> 1][2 * (i & 1) + 1];
+            hi[i] = pack_bf16(x, y);
+            lw[i] = pack_bf16(x - bf16lo(hi[i]), y - bf16hi(hi[i]));
+          }
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {
+            uint32_t r[4];
+            ldsm4t(r, base + chunk_at<C>(v_row, n + v_ch));
+            if (odd) finite_only<E4M3>(r);
+            mma16<false>(o[n], hi, r[0], r[1]);
+            mma16<false>(o[n + 1], hi, r[2], r[3]);
+            mma16<false>(o[n], lw, r[0], r[1]);
+            mma16<false>(o[n + 1], lw, r[2], r[3]);
+          }
+        }
+      }
+      __syncwarp();  // the stage is free
+      --waiting;
+      if (u.len) issue();
+      stage = stage + 1 == p.stages ? 0 : stage + 1;
+      phase ^= stage == 0;
+    }
+
+    // the warps' parts of the item
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] = quad_sum(l[i]);
+      if (c4 == 0) {
+        s_m[warp][g4 + i * 8] = m[i];
+        s_mv[warp][g4 + i * 8] = E4M3 ? mv[i] : m[i];
+        s_l[warp][g4 + i * 8] = l[i];
+      }
+      if (g4 + i * 8 < p.nr) {
+        float* dst = merge + ((size_t)warp * p.nr + g4 + i * 8) * D;
+        if (E4M3) {
+#pragma unroll
+          for (int n = 0; n < NT; n += 2)
+            *reinterpret_cast<float4*>(dst + n * 8 + c4 * 4) =
+                make_float4(o[n][2 * i], o[n + 1][2 * i], o[n][2 * i + 1], o[n + 1][2 * i + 1]);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<float2*>(dst + n * 8 + c4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        }
+      }
+    }
+    __syncthreads();
+    // Factors that bring `parts` outputs (maxima m, mv, sums l in columns of kRows) to their common maximum.
+    // s_sum: the total sum; s_top: log2 of what the total output still has to be multiplied with before the sum divides it
+    const bool split = end - t != s.blocks;
+    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * (p.nr * D + 3 * kRows);
+    if (tid < kRows) {
+      float a = -INFINITY, av = -INFINITY, sum = 0.f;
+      for (int i = 0; i < W; ++i) {
+        a = fmaxf(a, s_m[i][tid]);
+        av = fmaxf(av, s_mv[i][tid]);
+      }
+      for (int i = 0; i < W; ++i) {
+        sum += s_l[i][tid] * ex2(s_m[i][tid] - (a == -INFINITY ? 0.f : a));
+        s_mv[i][tid] = ex2(s_mv[i][tid] - (av == -INFINITY ? 0.f : av));
+      }
+      s_top[tid] = E4M3 ? av - a : 0.f;
+      s_sum[tid] = sum;
+      if (split) {
+        part[p.nr * D + tid] = a;
+        part[p.nr * D + kRows + tid] = av;
+        part[p.nr * D + 2 * kRows + tid] = sum;
+      } else if (p.lse && tid < nrow) {
+        p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + tid] = a + log2f(sum);
+      }
+    }
+    __syncthreads();
+    auto store = [&](int r, int d, float4 v) {  // v / sum as bf16; zeros for rows that see nothing
+      const int row = row0 + r, tok = row / p.group;
+      const float sum = s_sum[r], f = sum == 0.f || tok >= s.count ? 0.f : E4M3 ? ex2(s_top[r]) / sum : 1.f / sum;
+      if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * p.group + row % p.group) * p.o_sh + tok * p.o_st + d) =
+          make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+    };
+    for (int i = tid; i < nrow * (D / 4); i += W * 32) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(merge + ((size_t)w * p.nr + r) * D + d);
+        const float f = s_mv[w][r];
+        v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
+      }
+      if (split) *reinterpret_cast<float4*>(part + r * D + d) = v;
+      else store(r, d, v);
+    }
+    if (split) {
+      // CTAs whose blocks the item's first and last one are: theirs and all between hold a partial
+      auto owner = [&](int x) {
+        int i = (int)((int64_t)x * ctas / total);
+        while ((int)((int64_t)total * (i + 1) / ctas) <= x) ++i;
+        while ((int)((int64_t)total * i / ctas) > x) --i;
+        return i;
+      };
+      const int i0 = owner(start), parts = owner(start + s.blocks - 1) - i0 + 1;
+      const bool skip0 = (int)((int64_t)total * i0 / ctas) < start;  // CTA i0 has another item before this one
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        unsigned* word = p.sync + ((size_t)b * p.c.heads + h) * p.chunks + row0 / kRows;
+        const bool last = atomicAdd(word, 1u) == (unsigned)parts - 1;
+        if (last) *word = 0;
+        s_last = last;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        const size_t ld = p.nr * D + 3 * kRows;
+        const float* p0 = p.part + (2 * (size_t)i0) * ld;
+        auto at_part = [&](int i) { return p0 + (2 * (size_t)i + (i == 0 && skip0 ? 1 : 0)) * ld; };
+        float* fac = merge;  // [parts][nr]: fits, a part for each CTA of the grid at most (checked on the host)
+        if (tid < p.nr) {
+          float a = -INFINITY, av = -INFINITY, sum = 0.f;
+          for (int i = 0; i < parts; ++i) {
+            const float* x = at_part(i) + p.nr * D + tid;
+            a = fmaxf(a, __ldcg(x));
+            av = fmaxf(av, __ldcg(x + kRows));
+          }
+          for (int i = 0; i < parts; ++i) {
+            const float* x = at_part(i) + p.nr * D + tid;
+            sum += __ldcg(x + 2 * kRows) * ex2(__ldcg(x) - (a == -INFINITY ? 0.f : a));
+            fac[i * p.nr + tid] = ex2(__ldcg(x + kRows) - (av == -INFINITY ? 0.f : av));
+          }
+          s_top[tid] = E4M3 ? av - a : 0.f;
+          s_sum[tid] = sum;
+          if (p.lse && tid < nrow) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + tid] = a + log2f(sum);
+        }
+        __syncthreads();
+        for (int i = tid; i < nrow * (D / 4); i += W * 32) {
+          const int r = i / (D / 4), d = i % (D / 4) * 4;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int k = 0; k < parts; ++k) {
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(at_part(k) + r * D + d));
+            const float f = fac[k * p.nr + r];
+            v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
+          }
+          store(r, d, v);
+        }
+      }
+    }
+    __syncthreads();  // merge and the factors are free
+    t = end;
+  }
+  if (dead) {  // see this warp's copies in flight through, again with a limit, before leaving
+    for (int i = 0; lane == 0 && i < waiting; ++i) {
+      volatile int never = 0;
+      mbar_wait(&my_bars[stage], phase, &never, p.c.err);
+      stage = stage + 1 == p.stages ? 0 : stage + 1;
+      phase ^= stage == 0;
+    }
+    __syncwarp();
   }
 }
 
-template <int D>
-void launch_attend(const AttendParams& p, bool e4m3, cudaStream_t st) {
-  const unsigned grid = (unsigned)(p.c.batch * p.c.heads);
-  if (e4m3) attend_kernel<D, true><<<grid, 128, 0, st>>>(p);
-  else attend_kernel<D, false><<<grid, 128, 0, st>>>(p);
+// weights[b, h, j] += sum_r e^(s_rj - log-sum_r) over the head's query rows, from the logits the attention left
+// (fp32, 4 rows bytes a position: a few per cent of the cache's own bytes) and its row sums. Four positions a thread.
+__global__ void __launch_bounds__(256) weights_kernel(const AttendParams p, float* weights, int64_t w_sb, int64_t w_sh,
+                                                      int block_keys) {
+  pdl_wait();
+  const int per = (p.c.cap + 1023) / 1024;
+  for (int x = blockIdx.x; x < p.c.batch * p.c.heads * per; x += gridDim.x) {
+    const int bh = x / per, b = bh / p.c.heads, h = bh % p.c.heads;
+    const int len = paged_len(p.c, b), n = paged_count(p.c, p.counts, b, p.T, len);
+    const int lo = p.window ? max(0, len - n + 1 - p.window) / block_keys * block_keys : 0;
+    const int j = (x % per) * 1024 + threadIdx.x * 4;
+    if (n == 0 || j + 3 < lo || j >= len) continue;
+    const float* logits = p.logits + (int64_t)bh * p.rows * p.c.cap + j;
+    const float* lse = p.lse + (int64_t)bh * p.rows;
+    float a[4] = {};
+    for (int r = 0; r < n * p.group; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(logits + (int64_t)r * p.c.cap);
+      const float z = lse[r], vs[4] = {v.x, v.y, v.z, v.w};
+      if (z == -INFINITY) continue;  // a row that sees nothing
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] += j + i < len ? ex2(vs[i] - z) : 0.f;
+    }
+    float* w = weights + b * w_sb + h * w_sh + j;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j + i >= lo && j + i < len) w[i] += a[i];
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+int tile_map(CUtensorMap* map, void* base, const tbf16_paged_cache* c, int64_t sp, int64_t sh, int64_t ss) {
+  const int item = c->dtype == TBF16_E4M3 ? 1 : 2, span = (int)std::min<int64_t>(c->D * item, 128);
+  return tbf16_host::make_tmap_pages(map, base, item, c->D, span, c->page_size, c->heads, c->pages, ss, sh, sp);
+}
+
+constexpr int kSmemMax = 227 * 1024;
+
+template <class C>
+int attend_smem(int batch, int nr, int stages) {
+  return C::W * stages * (2 * C::KB + C::SC) + C::W * nr * C::D * 4 + (batch + 1) * (int)sizeof(SeqInfo);
+}
+// Static shared memory of the kernel, rounded up.
+constexpr int kSmemStatic = 3 * 1024;
+
+template <class C>
+int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
+  CUtensorMap km, vm;
+  if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss)) return s;
+  if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss)) return s;
+  p.stages = kMaxStages;
+  while (p.stages > 1 && attend_smem<C>(p.c.batch, p.nr, p.stages) + kSmemStatic > kSmemMax) --p.stages;
+  const int smem = attend_smem<C>(p.c.batch, p.nr, p.stages);
+  if (smem + kSmemStatic > kSmemMax || sms > C::W * C::D) return TBF16_ERR_UNSUPPORTED;
+  static const cudaError_t attr =
+      cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic);
+  if (attr != cudaSuccess) return TBF16_ERR_LAUNCH;
+  attend_kernel<C><<<sms, C::W * 32, smem, st>>>(km, vm, p);
+  return tbf16_host::check_launch();
+}
+
+struct Workspace {
+  int64_t rows, chunks, nr, part, lse, logits;  // sizes in floats, in this order
+  Workspace(const tbf16_paged_cache* c, int64_t Hq, int64_t T, bool weights, int sms) {
+    rows = T * (Hq / c->heads);
+    chunks = (rows + kRows - 1) / kRows;
+    nr = std::min<int64_t>(rows, kRows);
+    part = 2 * (int64_t)sms * (nr * c->D + 3 * kRows);
+    lse = weights ? (c->batch * c->heads * rows + 3) / 4 * 4 : 0;
+    logits = weights ? c->batch * c->heads * rows * c->max_pages * c->page_size : 0;
+  }
+  int64_t bytes() const { return (part + lse + logits) * 4; }
+};
+
+bool attend_sizes_ok(const tbf16_paged_cache* c, int64_t Hq, int64_t T) {
+  return c && c->batch >= 0 && c->heads >= 1 && Hq >= 1 && Hq <= 65536 && Hq % c->heads == 0 && T >= 0 && T <= 4096 &&
+         T * (Hq / c->heads) <= 65536;
 }
 
 }  // namespace
 
 extern "C" int64_t tbf16_paged_attend_ws_size(const tbf16_paged_cache* cache, int64_t Hq, int64_t T, int with_weights) {
-  return 0;
+  const tbf16_host::DeviceInfo* dev = tbf16_host::device_info();
+  if (!dev || !attend_sizes_ok(cache, Hq, T)) return 0;
+  return Workspace(cache, Hq, T, with_weights != 0, dev->sms).bytes();
 }
 
-extern "C" int64_t tbf16_paged_attend_sync_size(const tbf16_paged_cache* cache, int64_t Hq, int64_t T) { return 0; }
+extern "C" int64_t tbf16_paged_attend_sync_size(const tbf16_paged_cache* cache, int64_t Hq, int64_t T) {
+  if (!attend_sizes_ok(cache, Hq, T)) return 0;
+  return cache->batch * cache->heads * ((T * (Hq / cache->heads) + kRows - 1) / kRows) * 4;
+}
 
 extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh,
                                   int64_t q_st, int64_t Hq, int64_t T, const int32_t* counts, float scale,
@@ -106,28 +766,55 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   AttendParams p;
   if (int st = tbf16_host::paged_view(cache, &p.c)) return st;
   if (T == 0 || cache->batch == 0) return TBF16_OK;
-  if (!q || !out || T < 0 || Hq < 1 || Hq % cache->heads || window < 0 || !(scale == scale)) return TBF16_ERR_INVALID;
-  if (T > 4096 || Hq > 65536 || T * (Hq / cache->heads) > 65536) return TBF16_ERR_INVALID;
+  if (!q || !out || !attend_sizes_ok(cache, Hq, T) || window < 0 || !(scale == scale)) return TBF16_ERR_INVALID;
   for (int64_t s : {q_sb, q_sh, q_st, out_sb, out_sh, out_st}) {
     if (s < 0) return TBF16_ERR_INVALID;
     if (s % 8) return TBF16_ERR_ALIGN;
   }
-  if (!tbf16_host::aligned16(q) || !tbf16_host::aligned16(out)) return TBF16_ERR_ALIGN;
+  if (!tbf16_host::aligned16(q) || !tbf16_host::aligned16(out) || !tbf16_host::aligned16(ws)) return TBF16_ERR_ALIGN;
+  const tbf16_host::DeviceInfo* dev = tbf16_host::device_info();
+  const Workspace need(cache, Hq, T, weights != nullptr, dev->sms);
+  if (!sync || !ws || ws_bytes < need.bytes()) return TBF16_ERR_INVALID;
+  // blocks are counted in 32 bits, 16 keys at the least in each
+  if (cache->batch * cache->heads * need.chunks > INT32_MAX / (p.c.cap / 16 + 1)) return TBF16_ERR_INVALID;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_sb = q_sb; p.q_sh = q_sh; p.q_st = q_st;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.o_sb = out_sb; p.o_sh = out_sh; p.o_st = out_st;
   p.counts = counts;
-  p.weights = weights;
-  p.w_sb = w_sb; p.w_sh = w_sh;
   p.T = (int)T;
   p.group = (int)(Hq / cache->heads);
+  p.rows = (int)need.rows;
+  p.chunks = (int)need.chunks;
+  p.nr = (int)need.nr;
   p.window = (int)(window > p.c.cap ? 0 : window);
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.sync = static_cast<unsigned*>(sync);
+  p.part = static_cast<float*>(ws);
+  p.lse = weights ? p.part + need.part : nullptr;
+  p.logits = weights ? p.lse + need.lse : nullptr;
   const bool e4m3 = cache->dtype == TBF16_E4M3;
   auto st = static_cast<cudaStream_t>(stream);
-  if (cache->D == 64) launch_attend<64>(p, e4m3, st);
-  else if (cache->D == 128) launch_attend<128>(p, e4m3, st);
-  else launch_attend<256>(p, e4m3, st);
+  int rc;
+  if (cache->D == 64)
+    rc = e4m3 ? launch_attend<Tile<64, true>>(cache, p, dev->sms, st) : launch_attend<Tile<64, false>>(cache, p, dev->sms, st);
+  else if (cache->D == 128)
+    rc = e4m3 ? launch_attend<Tile<128, true>>(cache, p, dev->sms, st) : launch_attend<Tile<128, false>>(cache, p, dev->sms, st);
+  else
+    rc = e4m3 ? launch_attend<Tile<256, true>>(cache, p, dev->sms, st) : launch_attend<Tile<256, false>>(cache, p, dev->sms, st);
+  if (rc != TBF16_OK || !weights) return rc;
+  const int block_keys = cache->D * (e4m3 ? 1 : 2) <= 64 ? 64 : cache->D * (e4m3 ? 1 : 2) <= 128 ? 32 : 16;
+  const int64_t blocks = cache->batch * cache->heads * ((p.c.cap + 1023) / 1024);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, weights_kernel, p, weights, w_sb, w_sh, block_keys) != cudaSuccess)
+    return TBF16_ERR_LAUNCH;
   return tbf16_host::check_launch();
 }

@@ -145,6 +145,25 @@ int make_tmap_3d_f32(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d
   return r == CUDA_SUCCESS ? TBF16_OK : TBF16_ERR_INVALID;
 }
 
+int make_tmap_pages(CUtensorMap* map, const void* base, int item, int64_t D, int span, int64_t slots, int64_t heads,
+                    int64_t pages, int64_t slot_stride, int64_t head_stride, int64_t page_stride) {
+  if (!encode_fn()) return TBF16_ERR_LAUNCH;
+  if ((span != 64 && span != 128) || D * item % span) return TBF16_ERR_INVALID;
+  const cuuint64_t spans = (cuuint64_t)(D * item / span);
+  // A dimension of one element still needs a stride that the encoder accepts.
+  const auto stride = [&](int64_t n, int64_t s) { return n > 1 ? (cuuint64_t)(s * item) : (cuuint64_t)(D * item); };
+  cuuint64_t gdim[5] = {(cuuint64_t)(span / item), (cuuint64_t)slots, spans, (cuuint64_t)heads, (cuuint64_t)pages};
+  cuuint64_t gstride[4] = {stride(slots, slot_stride), (cuuint64_t)span, stride(heads, head_stride),
+                           stride(pages, page_stride)};
+  cuuint32_t box[5] = {(cuuint32_t)(span / item), 16, (cuuint32_t)spans, 1, 1};
+  cuuint32_t estride[5] = {1, 1, 1, 1, 1};
+  CUresult r = g_encode(map, item == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+                        const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TBF16_OK : TBF16_ERR_INVALID;
+}
+
 }  // namespace tbf16_host
 
 namespace {
