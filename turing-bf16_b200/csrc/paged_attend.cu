@@ -50,11 +50,13 @@ struct AttendParams {
   int64_t o_sb, o_sh, o_st;
   const int* counts;
   int T, group, rows, chunks, window;  // rows = T * group query rows of a head, in chunks of kRows
+  unsigned group_inv;                  // ceil(2^32 / group): row / group = umulhi(row, group_inv) below 2^16
   float scale_log2;
   int stages;
   int nr;           // rows of an item that can be real: min(rows, kRows)
+  int merge;        // floats of the merge area
   unsigned* sync;   // arrivals of each item, zero between calls
-  float* part;      // [2 * CTAs][nr * D + 3 * kRows]: partial outputs, maxima, sums
+  float* part;      // [2 * CTAs][nr * D + 2 * kRows]: partial outputs, maxima, sums
   float* logits;    // weights wanted: [batch * heads][rows][cap], base-2 logits
   float* lse;       // and [batch * heads][rows]: log2 of each row's sum
 };
@@ -63,6 +65,15 @@ struct AttendParams {
 struct SeqInfo {
   int cum, blocks, len, count;
 };
+
+// First block that a sequence's window reaches.
+template <class C>
+__device__ __forceinline__ int first_block(const AttendParams& p, int len, int count) {
+  return p.window ? max(0, len - count + 1 - p.window) / C::BK : 0;
+}
+__device__ __forceinline__ int token_of(const AttendParams& p, int row) {
+  return p.group == 1 ? row : (int)__umulhi((unsigned)row, p.group_inv);
+}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -120,20 +131,32 @@ __device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
   if (C::AW == 128) return (chunk >> 3) * 2048 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
   return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
+// The address of chunk `even + odd` from that of chunk `odd` (odd = 0 or 1, even a constant): the swizzle is an
+// exclusive or, and a group starts on a multiple of its span.
+template <class C>
+__device__ __forceinline__ uint32_t chunk_from(uint32_t at_odd, int even) {
+  return C::AW == 128 ? (at_odd ^ ((even & 7) << 4)) + (even >> 3) * 2048 : at_odd ^ (even << 4);
+}
 
-// Where a warp's next block lies: position t in the order of all blocks, and the item it belongs to.
+// Where a warp's next block lies: t in the order of all blocks, the item it belongs to, block of that item.
 struct Cursor {
-  int t, b, h, j0, len;  // first key of the block; cached tokens (0 past the end of the warp's blocks)
-  int page;              // this lane's page of the block, loaded ahead
+  int t, b, h, blk, blocks, j0, len;  // j0: its first key; len: cached tokens, 0 past the end of the warp's blocks
+  int page;                           // this lane's page of the block, loaded ahead
 };
 
 template <class C>
-struct Kernel {
+struct Loader {
   static constexpr bool E4M3 = C::E4M3;
 
-  // Moves the cursor to the warp's next block with anything to load, from position t on, and starts loading
-  // the page numbers that block needs (lane = group + NG * {keys, values, key scales, value scales}).
-  static __device__ void seek(Cursor& u, int t, int end, const SeqInfo* info, const AttendParams& p, int lane) {
+  // Starts loading the page numbers that the cursor's block needs (lane = group + NG * {keys, values, key
+  // scales, value scales}).
+  static __device__ __forceinline__ void fetch_pages(Cursor& u, const AttendParams& p, int lane) {
+    const int j = u.j0 + (lane % C::NG) * 16;
+    u.page = lane < (E4M3 ? 4 : 2) * C::NG && j < u.len ? p.c.table[u.b * p.c.table_ld + (j >> p.c.page_shift)] : 0;
+  }
+
+  // Moves the cursor to the warp's first block at or after position t with anything to load.
+  static __device__ __forceinline__ void seek(Cursor& u, int t, int end, const SeqInfo* info, const AttendParams& p, int lane) {
     for (;; t += C::W) {
       u.t = t;
       u.len = 0;
@@ -142,145 +165,167 @@ struct Kernel {
       const SeqInfo s = info[u.b];
       if (s.count == 0) continue;
       const unsigned rem = t - s.cum, item = rem / (unsigned)s.blocks;
-      u.h = (int)(item / (unsigned)p.chunks);
-      const int lo = p.window ? max(0, s.len - s.count + 1 - p.window) / C::BK : 0;
-      u.j0 = (lo + (int)(rem - item * s.blocks)) * C::BK;
+      u.h = p.chunks == 1 ? (int)item : (int)(item / (unsigned)p.chunks);
+      u.blk = (int)(rem - item * s.blocks);
+      u.blocks = s.blocks;
+      u.j0 = (first_block<C>(p, s.len, s.count) + u.blk) * C::BK;
       u.len = s.len;
       break;
     }
-    const int j = u.j0 + (lane % C::NG) * 16;
-    u.page = lane < (E4M3 ? 4 : 2) * C::NG && j < u.len ? p.c.table[u.b * p.c.table_ld + (j >> p.c.page_shift)] : 0;
+    fetch_pages(u, p, lane);
+  }
+  static __device__ __forceinline__ void next(Cursor& u, int end, const SeqInfo* info, const AttendParams& p, int lane) {
+    if (u.blk + C::W < u.blocks && u.t + C::W < end) {
+      u.t += C::W;
+      u.blk += C::W;
+      u.j0 += C::W * C::BK;
+      fetch_pages(u, p, lane);
+    } else {
+      seek(u, u.t + C::W, end, info, p, lane);
+    }
   }
 
-  static __device__ void load(const Cursor& u, uint8_t* stage, float* scales, uint64_t* bar, const CUtensorMap* km,
-                              const CUtensorMap* vm, const AttendParams& p, int lane) {
+  static __device__ __forceinline__ void load(const Cursor& u, uint8_t* stage, float* scales, uint64_t* bar,
+                                              const CUtensorMap* km, const CUtensorMap* vm, const AttendParams& p, int lane) {
     const int groups = min(C::NG, (u.len - u.j0 + 15) >> 4);
     if (lane == 0) mbar_arrive_expect_tx(bar, groups * (2 * C::GB + (E4M3 ? 128 : 0)));
     __syncwarp();
     const int g = lane % C::NG, kind = lane / C::NG, slot = paged_slot(p.c, u.j0 + g * 16);
     if (g >= groups) return;
     int page = u.page;
-    if (page < 0 || page >= p.c.pages) {
+    if (page < 0 || page >= p.c.pages) {  // read as page 0
       atomicOr(p.c.err, kErrPage);
       page = 0;
     }
-    if (kind == 0) tma_load_5d(stage + g * C::GB, km, bar, 0, slot, 0, u.h, page);
-    if (kind == 1) tma_load_5d(stage + C::KB + g * C::GB, vm, bar, 0, slot, 0, u.h, page);
+    if (kind < 2) tma_load_5d(stage + (kind * C::NG + g) * C::GB, kind ? vm : km, bar, 0, slot, 0, u.h, page);
     if (E4M3 && kind == 2) bulk_load(scales + g * 16, p.c.k_scale + page * p.c.ks_sp + u.h * p.c.ks_sh + slot, 64, bar);
     if (E4M3 && kind == 3)
       bulk_load(scales + C::BK + g * 16, p.c.v_scale + page * p.c.vs_sp + u.h * p.c.vs_sh + slot, 64, bar);
   }
 };
 
-// Shared memory: [rings][scales][merge outputs][info][factors ...]; sizes in attend_smem().
+// A weight grows to at most 2^kSlack before a new maximum is taken: the running maximum then changes, and the
+// output is rescaled, a few times per item and not with every block, and no lane has to ask the others for it.
+constexpr float kSlack = 8.f;
+constexpr float kNoMax = -3.4028234e38f;  // of a row that has seen nothing: every logit is far above it
+// e4m3: the weights that multiply the values carry the value row's scale over a power of two that is at least
+// the largest scale met so far, times 2^7: at most 2^15 in fp16 (2^kSlack 2^7), with 29 bits below that.
+constexpr int kWeightShift = 7;
+
+// Shared memory: [rings][scales][merge][info].
 template <class C>
 __global__ void __launch_bounds__(C::W * 32, 1)
     attend_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm, const AttendParams p) {
-  constexpr int D = C::D, NT = D / 8, W = C::W, NG = C::NG, KS = D / 16;
+  constexpr int D = C::D, NT = D / 8, W = C::W, NG = C::NG, KS = D / 16, NTHREADS = W * 32;
   constexpr bool E4M3 = C::E4M3;
-  using K = Kernel<C>;
+  using L = Loader<C>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem;
   float* scale_ring = reinterpret_cast<float*>(ring + (size_t)W * p.stages * 2 * C::KB);
   float* merge = scale_ring + (size_t)W * p.stages * (C::SC / 4);
-  SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + W * p.nr * D);
+  SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + p.merge);
   __shared__ uint64_t bars[W * kMaxStages];
-  __shared__ float s_m[W][kRows], s_l[W][kRows], s_mv[W][kRows];  // each warp's maxima and sums, then factors
-  __shared__ float s_top[kRows], s_sum[kRows];
-  __shared__ int s_scan[W], s_abort, s_last;
+  __shared__ float s_m[W][kRows], s_l[W][kRows];  // each warp's maxima and sums
+  __shared__ float s_sum[kRows];
+  __shared__ int s_scan[W], s_work[W], s_abort, s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((smem_u32(smem) & 1023u) != 0) {
     if (tid == 0) atomicOr(p.c.err, kErrSmemAlign);
     return;
   }
   pdl_launch_dependents();
+  if (lane < p.stages) mbar_init(&bars[warp * p.stages + lane], 1);
+  if (tid == 0) s_abort = 0;
+  fence_barrier_init();
 
-  // every sequence's blocks, and their running total
-  int carry = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += W * 32) {
+  // every sequence's blocks and their running total; `work`: CTAs that would give each warp at most one block
+  int total = 0, work = 0;
+  for (int b0 = 0; b0 < p.c.batch; b0 += NTHREADS) {
     const int b = b0 + tid;
     SeqInfo s{0, 0, 0, 0};
-    int mine = 0;
+    int x = 0, ctas_wanted = 0;
     if (b < p.c.batch) {
       s.len = paged_len(p.c, b);
       s.count = paged_count(p.c, p.counts, b, p.T, s.len);
-      const int lo = p.window ? max(0, s.len - s.count + 1 - p.window) / C::BK : 0;
-      s.blocks = s.count ? (s.len + C::BK - 1) / C::BK - lo : 1;  // one empty block writes an idle sequence's zeros
-      mine = s.blocks * p.c.heads * p.chunks;
+      // one empty block writes an idle sequence's zeros
+      s.blocks = s.count ? (s.len + C::BK - 1) / C::BK - first_block<C>(p, s.len, s.count) : 1;
+      x = s.blocks * p.c.heads * p.chunks;
+      ctas_wanted = (s.blocks + W - 1) / W * p.c.heads * p.chunks;
     }
-    int x = mine;
+    const int mine = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (lane == 31) s_scan[warp] = x;
+    ctas_wanted = __reduce_add_sync(0xffffffffu, ctas_wanted);
+    if (lane == 31) {
+      s_scan[warp] = x;
+      s_work[warp] = ctas_wanted;
+    }
     __syncthreads();
-    int before = carry, total = carry;
+    int before = total;
+#pragma unroll
     for (int i = 0; i < W; ++i) {
       before += i < warp ? s_scan[i] : 0;
       total += s_scan[i];
+      work += s_work[i];
     }
     s.cum = before + x - mine;
     if (b < p.c.batch) info[b] = s;
     if (b == p.c.batch - 1) info[b + 1] = SeqInfo{before + x, 1, 0, 0};
-    carry = total;
     __syncthreads();
   }
-  const int total = carry;
-  // no more CTAs than give every warp a block
-  const int ctas = min((int)gridDim.x, (total + W - 1) / W);
+  const int ctas = min((int)gridDim.x, work);
   if ((int)blockIdx.x >= ctas) return;
-  const int c0 = (int)((int64_t)total * blockIdx.x / ctas), c1 = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
+  // CTA i takes blocks [share(i), share(i + 1)): `each` of them, the first `more` CTAs one more
+  const int each = total / ctas, more = total - each * ctas;
+  auto share = [&](int i) { return each * i + min(i, more); };
+  const int c0 = share(blockIdx.x), c1 = share(blockIdx.x + 1);
 
-  if (tid == 0) {
-    for (int i = 0; i < W * p.stages; ++i) mbar_init(&bars[i], 1);
-    s_abort = 0;
-    fence_barrier_init();
-    tma_prefetch_desc(&km);
-    tma_prefetch_desc(&vm);
-  }
-  __syncthreads();
   uint8_t* my_ring = ring + (size_t)warp * p.stages * 2 * C::KB;
   float* my_scales = scale_ring + (size_t)warp * p.stages * (C::SC / 4);
   uint64_t* my_bars = bars + warp * p.stages;
   Cursor u;
   u.b = 0;
-  int issued = 0, waiting = 0;  // blocks issued and not consumed yet
+  int issued = 0, waiting = 0;  // stage of the next load; blocks issued and not consumed yet
   auto issue = [&]() {
-    K::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p, lane);
+    L::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p, lane);
     issued = issued + 1 == p.stages ? 0 : issued + 1;
     ++waiting;
-    K::seek(u, u.t + W, c1, info, p, lane);
+    L::next(u, c1, info, p, lane);
   };
-  K::seek(u, c0 + warp, c1, info, p, lane);
+  L::seek(u, c0 + warp, c1, info, p, lane);
+#pragma unroll 1
   while (waiting < p.stages && u.len) issue();
   int stage = 0, phase = 0;
   bool dead = false;  // a wait gave up: nothing more is loaded or computed, every barrier is still reached
 
   const int g4 = lane >> 2, c4 = lane & 3;
-  // this lane's row and chunk offset in the ldmatrix of keys and of values
-  const int k_row = E4M3 ? lane & 15 : ((lane >> 4) & 1) * 8 + (lane & 7), k_ch = E4M3 ? lane >> 4 : (lane >> 3) & 1;
-  const int v_row = lane & 15, v_ch = lane >> 4;
+  // this lane's addresses in the ldmatrix of keys and of values, for chunk pair 0 of a group
+  const uint32_t k_lane = E4M3 ? chunk_at<C>(lane & 15, lane >> 4) : chunk_at<C>(((lane >> 4) & 1) * 8 + (lane & 7), (lane >> 3) & 1);
+  const uint32_t v_lane = chunk_at<C>(lane & 15, lane >> 4);
 
   int b = 0;
+#pragma unroll 1
   for (int t = c0; t < c1;) {
     while (t >= info[b + 1].cum) ++b;
     const SeqInfo s = info[b];
-    const int item = (t - s.cum) / s.blocks, start = s.cum + item * s.blocks, end = min(c1, start + s.blocks);
-    const int h = item / p.chunks, row0 = (item % p.chunks) * kRows;
+    const int item = (int)((unsigned)(t - s.cum) / (unsigned)s.blocks), start = s.cum + item * s.blocks;
+    const int end = min(c1, start + s.blocks);
+    const int h = p.chunks == 1 ? item : item / p.chunks, row0 = (item - h * p.chunks) * kRows;
     const int nrow = min(kRows, p.rows - row0);
-    const int lo = p.window ? max(0, s.len - s.count + 1 - p.window) / C::BK : 0;
+    const int lo = first_block<C>(p, s.len, s.count);
     // query rows g4 and g4 + 8 of the item: their A fragments and positions
     uint32_t qf[KS][4];
     float mul[2];
     int at[2];  // position of the row's token; -1: the row is not there
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = row0 + g4 + i * 8, tok = r / p.group;
+      const int r = row0 + g4 + i * 8, tok = token_of(p, r);
       const bool there = r < p.rows && tok < s.count;
       at[i] = there ? s.len - s.count + tok : -1;
-      const __nv_bfloat16* q = p.q + b * p.q_sb + (int64_t)(h * p.group + r % p.group) * p.q_sh + tok * p.q_st;
+      const __nv_bfloat16* q = p.q + b * p.q_sb + (int64_t)(h * p.group + r - tok * p.group) * p.q_sh + tok * p.q_st;
       mul[i] = p.scale_log2;
       if (E4M3) {
         // fp16 rows: the largest magnitude to [2^14, 2^15) by a power of two, undone in the logits' factor. In
@@ -288,11 +333,11 @@ __global__ void __launch_bounds__(C::W * 32, 1)
         uint2 x[KS];
         unsigned m = 0;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          x[k] = there ? *reinterpret_cast<const uint2*>(q + k * 16 + c4 * 4) : make_uint2(0, 0);
+        for (int k = 0; k < KS; ++k) x[k] = there ? *reinterpret_cast<const uint2*>(q + k * 16 + c4 * 4) : make_uint2(0, 0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
           m = max(m, max(max((x[k].x << 16) & 0x7fffffffu, x[k].x & 0x7fff0000u),
                          max((x[k].y << 16) & 0x7fffffffu, x[k].y & 0x7fff0000u)));
-        }
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const int e = m == 0 || m >= 0x7f800000u ? 15 : max(frexp_exp(__uint_as_float(m)), -110);
@@ -312,155 +357,165 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       }
     }
     float o[NT][4] = {};
-    float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+    float vtop = 0.f, vmul = 0.f;  // e4m3: bound of the value scales met so far, and 2^kWeightShift over it
     const int pos_min = s.len - s.count, pos_max = s.len - 1;
 
     const int first = t + (warp - (t - c0) % W + W) % W;
+#pragma unroll 1
     for (int x = first; x < end && s.count; x += W) {
       if (dead || !mbar_wait_warp(&my_bars[stage], phase, &s_abort, p.c.err)) {
         dead = true;
         break;
       }
-      const uint32_t kb = smem_u32(my_ring + (size_t)stage * 2 * C::KB), vb = kb + C::KB;
-      const float* ksc = my_scales + stage * (C::SC / 4);
+      const uint32_t kb = smem_u32(my_ring) + stage * (2 * C::KB);
+      const float* ksc = my_scales + stage * (C::SC / 4) + c4 * 2;
       const int j0 = (lo + x - start) * C::BK;
       const int groups = min(NG, (s.len - j0 + 15) >> 4);
-      float sc[NG][2][4];
-      // logits of 16 query rows x BK keys, in units of log 2
+#pragma unroll 1
+      for (int g = 0; g < groups; ++g) {
+        // products of 16 query rows x 16 keys; two accumulators a tile shorten the chain of dependent products
+        const uint32_t ka = kb + g * C::GB + k_lane;
+        float sc[2][4] = {}, sd[2][4] = {};
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[g][n][e] = 0.f;
-        if (g >= groups) continue;
-        const uint32_t base = kb + g * C::GB;
-        if (E4M3) {
-#pragma unroll
-          for (int k = 0; k < KS; k += 2) {
-            uint32_t r[4];
-            ldsm4(r, base + chunk_at<C>(k_row, k + k_ch));
+        for (int k = 0; k < KS; k += E4M3 ? 2 : 1) {
+          uint32_t r[4];
+          if (E4M3) {
+            ldsm4(r, chunk_from<C>(ka, k));
 #pragma unroll
             for (int i = 0; i < 4; ++i)  // r[0], r[1]: keys 0-7 and 8-15 of chunk k; r[2], r[3]: of chunk k + 1
-              mma16<true>(sc[g][i & 1], qf[k + (i >> 1)], e4m3_f16(r[i], false), e4m3_f16(r[i], true));
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            uint32_t r[4];
-            ldsm4(r, base + chunk_at<C>(k_row, 2 * k + k_ch));
-            mma16<false>(sc[g][0], qf[k], r[0], r[1]);
-            mma16<false>(sc[g][1], qf[k], r[2], r[3]);
+              mma16<true>(i < 2 ? sc[i] : sd[i - 2], qf[k + (i >> 1)], e4m3_f16(r[i], false), e4m3_f16(r[i], true));
+          } else {
+            ldsm4(r, chunk_from<C>(ka, 2 * k));
+            mma16<false>(k & 1 ? sd[0] : sc[0], qf[k], r[0], r[1]);
+            mma16<false>(k & 1 ? sd[1] : sc[1], qf[k], r[2], r[3]);
           }
         }
-      }
-      float top[2] = {m[0], m[1]}, topv[2] = {mv[0], mv[1]};
-      float ev[NG][2][2];  // e4m3: log2 of the value rows' scales (NaN for a row that reads as NaN)
-      unsigned masked = 0;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
         const int jg = j0 + g * 16;
-        const bool whole = g < groups && jg + 15 <= pos_min && (!p.window || jg > pos_max - p.window);
-        if (!whole) masked |= 1u << g;
+        const bool whole = jg + 15 <= pos_min && (!p.window || jg > pos_max - p.window);
+        float vs[2][2];  // e4m3: scales of this lane's value rows
+        // logits in units of log 2
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           float2 ks = make_float2(1.f, 1.f);
           if (E4M3) {
-            ks = *reinterpret_cast<const float2*>(ksc + g * 16 + n * 8 + c4 * 2);
-            const float2 vs = *reinterpret_cast<const float2*>(ksc + C::BK + g * 16 + n * 8 + c4 * 2);
-            ev[g][n][0] = (float)(int)((__float_as_uint(vs.x) >> 23) & 255u) - 127.f + vs.x * 0.f;
-            ev[g][n][1] = (float)(int)((__float_as_uint(vs.y) >> 23) & 255u) - 127.f + vs.y * 0.f;
+            ks = *reinterpret_cast<const float2*>(ksc + g * 16 + n * 8);
+            const float2 y = *reinterpret_cast<const float2*>(ksc + C::BK + g * 16 + n * 8);
+            vs[n][0] = y.x;
+            vs[n][1] = y.y;
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = sc[g][n][e] * mul[e >> 1];
-            if (E4M3) v *= (e & 1) ? ks.y : ks.x;
-            if (!whole) {
+          for (int e = 0; e < 4; ++e)
+            sc[n][e] = (sc[n][e] + sd[n][e]) * (E4M3 ? mul[e >> 1] * ((e & 1) ? ks.y : ks.x) : mul[e >> 1]);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
               const int j = jg + n * 8 + c4 * 2 + (e & 1), i = at[e >> 1];
               const bool see = j <= i && (!p.window || j > i - p.window);
-              v = see ? v : -INFINITY;
+              if (!see) sc[n][e] = -INFINITY;
+              // the scale of a row that nobody sees may be anything
+              if (E4M3 && e < 2 && (j > pos_max || (p.window && j <= pos_min - p.window))) vs[n][e] = 0.f;
             }
-            sc[g][n][e] = v;
-            top[e >> 1] = fmaxf(top[e >> 1], v);
-            if (E4M3) topv[e >> 1] = fmaxf(topv[e >> 1], v == -INFINITY ? v : v + ev[g][n][e & 1]);
-          }
-          if (p.logits && g < groups) {
+        }
+        if (p.logits) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
               if (at[i] >= 0)
                 *reinterpret_cast<float2*>(p.logits + ((int64_t)(b * p.c.heads + h) * p.rows + row0 + g4 + i * 8) * p.c.cap +
-                                           jg + n * 8 + c4 * 2) = make_float2(sc[g][n][2 * i], sc[g][n][2 * i + 1]);
-          }
+                                           jg + n * 8 + c4 * 2) = make_float2(sc[n][2 * i], sc[n][2 * i + 1]);
         }
-      }
-      // running maxima: m for the sum; e4m3 also keeps mv, of logit + log2(value scale), for the output, so that
-      // fp16 weights times e4m3 values cannot overflow whatever the rows' scales are
-      float fac[2];
-      bool grew = false;
+        float top[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = quad_max(top[i]);
-        if (E4M3) topv[i] = quad_max(topv[i]);
-        const float base = top[i] == -INFINITY ? 0.f : top[i];
-        l[i] *= ex2(m[i] - base);
-        const float was = E4M3 ? mv[i] : m[i], now = E4M3 ? topv[i] : top[i];
-        fac[i] = ex2(was - (now == -INFINITY ? 0.f : now));
-        grew |= now != was;
-        m[i] = top[i];
-        mv[i] = topv[i];
-        top[i] = base;
-        topv[i] = topv[i] == -INFINITY ? 0.f : topv[i];
-      }
-      if (__any_sync(0xffffffffu, grew)) {
+        for (int i = 0; i < 2; ++i)
+          top[i] = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
+        bool grew = top[0] - m[0] > kSlack || top[1] - m[1] > kSlack;
+        if (E4M3) {
+          const float y = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+          grew |= y > vtop && y < INFINITY;
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+          float fac[2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int i = 0; i < 2; ++i) {
+            const float was = m[i];
+            m[i] = fmaxf(was, quad_max(top[i]));
+            fac[i] = ex2(was - m[i]);
+            l[i] *= fac[i];
+          }
+          if (E4M3) {
+            float y = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][e] *= fac[e >> 1];
-      }
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        if (g >= groups) continue;
+              for (int e = 0; e < 2; ++e) y = fmaxf(y, vs[n][e] < INFINITY ? vs[n][e] : 0.f);
+            y = quad_max(y);
+            if (y > vtop) {  // a power of two: two bits of room, so that the next ones rarely come here
+              const float now = fmaxf(y * 4.f, 0x1p-110f), f = vtop / now;
+              fac[0] *= f;
+              fac[1] *= f;
+              vtop = now;
+              vmul = (float)(1 << kWeightShift) / now;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] *= fac[e >> 1];
+        }
         float pw[2][4];  // weights for the output
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float v = sc[g][n][e], w = ex2(v - top[e >> 1]);
+            const float w = ex2(sc[n][e] - m[e >> 1]);
             l[e >> 1] += w;
-            pw[n][e] = !E4M3 ? w : v == -INFINITY ? 0.f : ex2(v + ev[g][n][e & 1] - topv[e >> 1]);
+            pw[n][e] = E4M3 ? w * (vs[n][e & 1] * vmul) : w;
           }
-        const uint32_t base = vb + g * C::GB;
+        const uint32_t vg = kb + C::KB + g * C::GB, va = vg + v_lane;
         bool odd = false;
-        if ((masked >> g) & 1) {
+        if (!whole) {
           // A masked weight is 0, but 0 x NaN is not: if the values of a partly masked group hold infinities or
           // NaNs (stale slots, a later token's), those are added here, to the rows that see them, and are zeros in
           // the products below; all other bits of the result stay what they are without them.
+#pragma unroll 1
           for (int i = lane; i < C::GB / 16; i += 32) {
             uint32_t w[4];
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(base + i * 16));
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vg + i * 16));
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              odd |= E4M3 ? __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0
-                          : (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
+              odd |= (E4M3 ? __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpeq2(w[k] & 0x7f807f80u, 0x7f807f80u)) != 0;
           }
           odd = __any_sync(0xffffffffu, odd);
+          if (E4M3) {  // a scale may be NaN too
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (sc[n][e] == -INFINITY) pw[n][e] = 0.f;
+          }
           if (odd) {
+#pragma unroll 1
             for (int k = 0; k < 16; ++k) {
-              const int from = (lane & ~3) | ((k & 7) >> 1), j = j0 + g * 16 + k;
+              const int from = (lane & ~3) | ((k & 7) >> 1), j = jg + k;
               float w[2];
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const float a = __shfl_sync(0xffffffffu, pw[0][2 * i + 0], from), c = __shfl_sync(0xffffffffu, pw[0][2 * i + 1], from);
-                const float d = __shfl_sync(0xffffffffu, pw[1][2 * i + 0], from), f = __shfl_sync(0xffffffffu, pw[1][2 * i + 1], from);
-                w[i] = k < 8 ? (k & 1 ? c : a) : (k & 1 ? f : d);
+                const float a = __shfl_sync(0xffffffffu, pw[0][2 * i], from), d = __shfl_sync(0xffffffffu, pw[0][2 * i + 1], from);
+                const float e = __shfl_sync(0xffffffffu, pw[1][2 * i], from), f = __shfl_sync(0xffffffffu, pw[1][2 * i + 1], from);
+                w[i] = k < 8 ? (k & 1 ? d : a) : (k & 1 ? f : e);
               }
               const bool see0 = j <= at[0] && (!p.window || j > at[0] - p.window);
               const bool see1 = j <= at[1] && (!p.window || j > at[1] - p.window);
 #pragma unroll
               for (int n = 0; n < NT; n += E4M3 ? 2 : 1) {
                 uint32_t v;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(base + chunk_at<C>(k, E4M3 ? n / 2 : n) + c4 * 4));
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(vg + chunk_at<C>(k, E4M3 ? n / 2 : n) + c4 * 4));
                 if (E4M3) {
                   const uint32_t lo2 = e4m3_f16(v, false), hi2 = e4m3_f16(v, true);
                   const float x4[4] = {f16lo(lo2), f16hi(lo2), f16lo(hi2), f16hi(hi2)};
@@ -489,7 +544,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
 #pragma unroll
           for (int k = 0; k < KS; k += 2) {
             uint32_t r[4];
-            ldsm4t(r, base + chunk_at<C>(v_row, k + v_ch));
+            ldsm4t(r, chunk_from<C>(va, k));
             if (odd) finite_only<E4M3>(r);
             // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: pair the keys, one tile for the even
             // columns of the chunk, one for the odd ones
@@ -505,14 +560,14 @@ __global__ void __launch_bounds__(C::W * 32, 1)
           uint32_t hi[4], lw[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float x = pw[i >> 1][2 * (i & 1)], y = pw[i >> 1][2 * (i & 1) + 1];
-            hi[i] = pack_bf16(x, y);
-            lw[i] = pack_bf16(x - bf16lo(hi[i]), y - bf16hi(hi[i]));
+            const float y = pw[i >> 1][2 * (i & 1)], z = pw[i >> 1][2 * (i & 1) + 1];
+            hi[i] = pack_bf16(y, z);
+            lw[i] = pack_bf16(y - bf16lo(hi[i]), z - bf16hi(hi[i]));
           }
 #pragma unroll
           for (int n = 0; n < NT; n += 2) {
             uint32_t r[4];
-            ldsm4t(r, base + chunk_at<C>(v_row, n + v_ch));
+            ldsm4t(r, chunk_from<C>(va, n));
             if (odd) finite_only<E4M3>(r);
             mma16<false>(o[n], hi, r[0], r[1]);
             mma16<false>(o[n + 1], hi, r[2], r[3]);
@@ -534,16 +589,16 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       l[i] = quad_sum(l[i]);
       if (c4 == 0) {
         s_m[warp][g4 + i * 8] = m[i];
-        s_mv[warp][g4 + i * 8] = E4M3 ? mv[i] : m[i];
         s_l[warp][g4 + i * 8] = l[i];
       }
       if (g4 + i * 8 < p.nr) {
         float* dst = merge + ((size_t)warp * p.nr + g4 + i * 8) * D;
         if (E4M3) {
+          const float f = vtop * (1.f / (1 << kWeightShift));
 #pragma unroll
           for (int n = 0; n < NT; n += 2)
             *reinterpret_cast<float4*>(dst + n * 8 + c4 * 4) =
-                make_float4(o[n][2 * i], o[n + 1][2 * i], o[n][2 * i + 1], o[n + 1][2 * i + 1]);
+                make_float4(o[n][2 * i] * f, o[n + 1][2 * i] * f, o[n][2 * i + 1] * f, o[n + 1][2 * i + 1] * f);
         } else {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -552,60 +607,49 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       }
     }
     __syncthreads();
-    // Factors that bring `parts` outputs (maxima m, mv, sums l in columns of kRows) to their common maximum.
-    // s_sum: the total sum; s_top: log2 of what the total output still has to be multiplied with before the sum divides it
     const bool split = end - t != s.blocks;
-    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * (p.nr * D + 3 * kRows);
-    if (tid < kRows) {
-      float a = -INFINITY, av = -INFINITY, sum = 0.f;
-      for (int i = 0; i < W; ++i) {
-        a = fmaxf(a, s_m[i][tid]);
-        av = fmaxf(av, s_mv[i][tid]);
-      }
-      for (int i = 0; i < W; ++i) {
-        sum += s_l[i][tid] * ex2(s_m[i][tid] - (a == -INFINITY ? 0.f : a));
-        s_mv[i][tid] = ex2(s_mv[i][tid] - (av == -INFINITY ? 0.f : av));
-      }
-      s_top[tid] = E4M3 ? av - a : 0.f;
-      s_sum[tid] = sum;
-      if (split) {
-        part[p.nr * D + tid] = a;
-        part[p.nr * D + kRows + tid] = av;
-        part[p.nr * D + 2 * kRows + tid] = sum;
-      } else if (p.lse && tid < nrow) {
-        p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + tid] = a + log2f(sum);
-      }
-    }
-    __syncthreads();
-    auto store = [&](int r, int d, float4 v) {  // v / sum as bf16; zeros for rows that see nothing
-      const int row = row0 + r, tok = row / p.group;
-      const float sum = s_sum[r], f = sum == 0.f || tok >= s.count ? 0.f : E4M3 ? ex2(s_top[r]) / sum : 1.f / sum;
+    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * (p.nr * D + 2 * kRows);
+    // v / sum as bf16; zeros for rows that see nothing
+    auto store = [&](int r, int d, float4 v, float sum) {
+      const int row = row0 + r, tok = token_of(p, row);
+      const float f = sum == 0.f || tok >= s.count ? 0.f : 1.f / sum;
       if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * p.group + row % p.group) * p.o_sh + tok * p.o_st + d) =
+      *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * p.group + row - tok * p.group) * p.o_sh + tok * p.o_st + d) =
           make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
     };
-    for (int i = tid; i < nrow * (D / 4); i += W * 32) {
+#pragma unroll 1
+    for (int i = tid; i < nrow * (D / 4); i += NTHREADS) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float a = kNoMax, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) a = fmaxf(a, s_m[w][r]);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const float4 y = *reinterpret_cast<const float4*>(merge + ((size_t)w * p.nr + r) * D + d);
-        const float f = s_mv[w][r];
+        const float f = ex2(s_m[w][r] - a);
+        sum += s_l[w][r] * f;
         v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
       }
-      if (split) *reinterpret_cast<float4*>(part + r * D + d) = v;
-      else store(r, d, v);
+      if (split) {
+        *reinterpret_cast<float4*>(part + r * D + d) = v;
+        if (d == 0) {
+          part[p.nr * D + r] = a;
+          part[p.nr * D + kRows + r] = sum;
+        }
+      } else {
+        store(r, d, v, sum);
+        if (p.lse && d == 0) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + r] = a + log2f(sum);
+      }
     }
     if (split) {
-      // CTAs whose blocks the item's first and last one are: theirs and all between hold a partial
+      // the CTAs whose blocks the item's first and last one are: theirs and all between hold a partial
       auto owner = [&](int x) {
-        int i = (int)((int64_t)x * ctas / total);
-        while ((int)((int64_t)total * (i + 1) / ctas) <= x) ++i;
-        while ((int)((int64_t)total * i / ctas) > x) --i;
-        return i;
+        const int big = more * (each + 1);
+        return x < big ? x / (each + 1) : more + (x - big) / each;
       };
       const int i0 = owner(start), parts = owner(start + s.blocks - 1) - i0 + 1;
-      const bool skip0 = (int)((int64_t)total * i0 / ctas) < start;  // CTA i0 has another item before this one
+      const bool skip0 = share(i0) < start;  // CTA i0 has another item before this one
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -617,41 +661,59 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       __syncthreads();
       if (s_last) {
         __threadfence();
-        const size_t ld = p.nr * D + 3 * kRows;
-        const float* p0 = p.part + (2 * (size_t)i0) * ld;
+        const size_t ld = p.nr * D + 2 * kRows;
+        const float* p0 = p.part + 2 * (size_t)i0 * ld;
         auto at_part = [&](int i) { return p0 + (2 * (size_t)i + (i == 0 && skip0 ? 1 : 0)) * ld; };
-        float* fac = merge;  // [parts][nr]: fits, a part for each CTA of the grid at most (checked on the host)
-        if (tid < p.nr) {
-          float a = -INFINITY, av = -INFINITY, sum = 0.f;
-          for (int i = 0; i < parts; ++i) {
-            const float* x = at_part(i) + p.nr * D + tid;
-            a = fmaxf(a, __ldcg(x));
-            av = fmaxf(av, __ldcg(x + kRows));
+        float* fac = merge;  // [parts][nr], then the thread groups' sums
+        float* sums = merge + (parts * p.nr + 3) / 4 * 4;
+        for (int r = warp; r < nrow; r += W) {
+          float a = kNoMax, sum = 0.f;
+          for (int i = lane; i < parts; i += 32) a = fmaxf(a, __ldcg(at_part(i) + p.nr * D + r));
+          a = warp_max(a);
+          for (int i = lane; i < parts; i += 32) {
+            const float* x = at_part(i) + p.nr * D + r;
+            const float f = ex2(__ldcg(x) - a);
+            fac[i * p.nr + r] = f;
+            sum += __ldcg(x + kRows) * f;
           }
-          for (int i = 0; i < parts; ++i) {
-            const float* x = at_part(i) + p.nr * D + tid;
-            sum += __ldcg(x + 2 * kRows) * ex2(__ldcg(x) - (a == -INFINITY ? 0.f : a));
-            fac[i * p.nr + tid] = ex2(__ldcg(x + kRows) - (av == -INFINITY ? 0.f : av));
+#pragma unroll
+          for (int o2 = 16; o2 > 0; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+          if (lane == 0) {
+            s_sum[r] = sum;
+            if (p.lse) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + r] = a + log2f(sum);
           }
-          s_top[tid] = E4M3 ? av - a : 0.f;
-          s_sum[tid] = sum;
-          if (p.lse && tid < nrow) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + tid] = a + log2f(sum);
         }
         __syncthreads();
-        for (int i = tid; i < nrow * (D / 4); i += W * 32) {
+        // `teams` groups of threads take every teams-th part each
+        const int n4 = nrow * (D / 4), teams = max(1, min(parts, NTHREADS / n4));
+        const int team = teams == 1 ? 0 : tid / n4;
+#pragma unroll 1
+        for (int i = teams == 1 ? tid : tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
           const int r = i / (D / 4), d = i % (D / 4) * 4;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-          for (int k = 0; k < parts; ++k) {
+          for (int k = team; k < parts; k += teams) {
             const float4 y = __ldcg(reinterpret_cast<const float4*>(at_part(k) + r * D + d));
             const float f = fac[k * p.nr + r];
             v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
           }
-          store(r, d, v);
+          if (teams == 1) store(r, d, v, s_sum[r]);
+          else *reinterpret_cast<float4*>(sums + ((size_t)team * n4 + i) * 4) = v;
+        }
+        if (teams > 1) {
+          __syncthreads();
+          if (tid < n4) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < teams; ++k) {
+              const float4 y = *reinterpret_cast<const float4*>(sums + ((size_t)k * n4 + tid) * 4);
+              v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+            }
+            store(tid / (D / 4), tid % (D / 4) * 4, v, s_sum[tid / (D / 4)]);
+          }
         }
       }
     }
-    __syncthreads();  // merge and the factors are free
+    __syncthreads();  // merge and the sums are free
     t = end;
   }
   if (dead) {  // see this warp's copies in flight through, again with a limit, before leaving
@@ -704,8 +766,8 @@ int tile_map(CUtensorMap* map, void* base, const tbf16_paged_cache* c, int64_t s
 constexpr int kSmemMax = 227 * 1024;
 
 template <class C>
-int attend_smem(int batch, int nr, int stages) {
-  return C::W * stages * (2 * C::KB + C::SC) + C::W * nr * C::D * 4 + (batch + 1) * (int)sizeof(SeqInfo);
+int attend_smem(const AttendParams& p, int stages) {
+  return C::W * stages * (2 * C::KB + C::SC) + p.merge * 4 + (p.c.batch + 1) * (int)sizeof(SeqInfo);
 }
 // Static shared memory of the kernel, rounded up.
 constexpr int kSmemStatic = 3 * 1024;
@@ -715,10 +777,12 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   CUtensorMap km, vm;
   if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss)) return s;
   if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss)) return s;
+  // the warps' outputs, or a join's factors (a part for each CTA at the most) and its thread groups' sums
+  p.merge = std::max(C::W * p.nr * C::D, sms * p.nr + 4 + C::W * 32 * 4);
   p.stages = kMaxStages;
-  while (p.stages > 1 && attend_smem<C>(p.c.batch, p.nr, p.stages) + kSmemStatic > kSmemMax) --p.stages;
-  const int smem = attend_smem<C>(p.c.batch, p.nr, p.stages);
-  if (smem + kSmemStatic > kSmemMax || sms > C::W * C::D) return TBF16_ERR_UNSUPPORTED;
+  while (p.stages > 1 && attend_smem<C>(p, p.stages) + kSmemStatic > kSmemMax) --p.stages;
+  const int smem = attend_smem<C>(p, p.stages);
+  if (smem + kSmemStatic > kSmemMax) return TBF16_ERR_UNSUPPORTED;
   static const cudaError_t attr =
       cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic);
   if (attr != cudaSuccess) return TBF16_ERR_LAUNCH;
@@ -732,7 +796,7 @@ struct Workspace {
     rows = T * (Hq / c->heads);
     chunks = (rows + kRows - 1) / kRows;
     nr = std::min<int64_t>(rows, kRows);
-    part = 2 * (int64_t)sms * (nr * c->D + 3 * kRows);
+    part = 2 * (int64_t)sms * (nr * c->D + 2 * kRows);
     lse = weights ? (c->batch * c->heads * rows + 3) / 4 * 4 : 0;
     logits = weights ? c->batch * c->heads * rows * c->max_pages * c->page_size : 0;
   }
@@ -784,6 +848,7 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   p.counts = counts;
   p.T = (int)T;
   p.group = (int)(Hq / cache->heads);
+  p.group_inv = (unsigned)(((UINT64_C(1) << 32) + p.group - 1) / p.group);
   p.rows = (int)need.rows;
   p.chunks = (int)need.chunks;
   p.nr = (int)need.nr;
