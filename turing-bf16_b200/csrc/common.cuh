@@ -625,9 +625,9 @@ int make_tmap_3d_f32(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d
                      uint64_t stride2, uint32_t box0, uint32_t box1, int swizzle_bytes = 128);
 // Tiled map of a cache pool: rows of `span` bytes' worth of D elements of `item` bytes (16-bit or 8-bit), as a
 // 5-D tensor {element in span, slot, span, head, page} with element strides of slot, head and page; the box is
-// one span x 16 slots x all spans of a row, swizzled over the span (64 or 128 bytes).
+// one span x box_slots slots x all spans of a row, swizzled over the span (64 or 128 bytes).
 int make_tmap_pages(CUtensorMap* map, const void* base, int item, int64_t D, int span, int64_t slots, int64_t heads,
-                    int64_t pages, int64_t slot_stride, int64_t head_stride, int64_t page_stride);
+                    int64_t pages, int64_t slot_stride, int64_t head_stride, int64_t page_stride, int box_slots);
 // Attention dropout: threshold (a key is kept when its 16 hash bits are >= thr) and 1 / keep probability
 // for dropout_p in [0, 1); false outside that range.
 inline bool dropout_params(float dropout_p, uint32_t* thr, float* inv_keep) {

@@ -33,10 +33,9 @@ struct Tile {
   static constexpr bool E4M3 = E4M3_;
   static constexpr int RB = D * (E4M3 ? 1 : 2);              // bytes of a cached row
   static constexpr int AW = RB < 128 ? RB : 128;             // swizzle span: 64 or 128 bytes
-  static constexpr int NA = RB / AW;                         // spans of a row
   static constexpr int BK = RB <= 64 ? 64 : RB <= 128 ? 32 : 16;  // keys of a block
-  static constexpr int NG = BK / 16;                         // groups of 16 keys, one TMA box each
-  static constexpr int GB = 16 * RB;                         // bytes of a group: [NA][16 keys][AW]
+  static constexpr int NG = BK / 16;                         // groups of 16 keys, worked on one after another
+  static constexpr int GB = 16 * RB;                         // bytes of a group: [RB / AW][16 keys][AW]
   static constexpr int KB = NG * GB;                         // bytes of a block's keys (or values)
   static constexpr int W = RB == 512 ? 4 : 8;                // warps
   static constexpr int SC = E4M3 ? 2 * BK * 4 : 0;           // bytes of a block's scales
@@ -53,6 +52,7 @@ struct AttendParams {
   unsigned group_inv;                  // ceil(2^32 / group): row / group = umulhi(row, group_inv) below 2^16
   float scale_log2;
   int stages;
+  int box;          // keys that one TMA load brings: min(BK, page size); rows of one span when over 16
   int nr;           // rows of an item that can be real: min(rows, kRows)
   int merge;        // floats of the merge area
   unsigned* sync;   // arrivals of each item, zero between calls
@@ -94,10 +94,23 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two e4m3 values (the low or high half of v) as packed fp16, exactly.
-__device__ __forceinline__ uint32_t e4m3_f16(uint32_t v, bool high) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(high ? v >> 16 : v & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// The same from a zero accumulator.
+template <bool F16>
+__device__ __forceinline__ void mma16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Four e4m3 values as two packed fp16 pairs, exactly.
+__device__ __forceinline__ void e4m3_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(v));
 }
 // Packed e4m3 or bf16 values with infinities and NaNs replaced by zeros.
 template <bool E4M3>
@@ -148,11 +161,10 @@ template <class C>
 struct Loader {
   static constexpr bool E4M3 = C::E4M3;
 
-  // Starts loading the page numbers that the cursor's block needs (lane = group + NG * {keys, values, key
-  // scales, value scales}).
+  // Starts loading the page numbers that the cursor's block needs, lane i that of its i-th box.
   static __device__ __forceinline__ void fetch_pages(Cursor& u, const AttendParams& p, int lane) {
-    const int j = u.j0 + (lane % C::NG) * 16;
-    u.page = lane < (E4M3 ? 4 : 2) * C::NG && j < u.len ? p.c.table[u.b * p.c.table_ld + (j >> p.c.page_shift)] : 0;
+    const int j = u.j0 + lane * p.box;
+    u.page = j < min(u.len, u.j0 + C::BK) ? p.c.table[u.b * p.c.table_ld + (j >> p.c.page_shift)] : 0;
   }
 
   // Moves the cursor to the warp's first block at or after position t with anything to load.
@@ -185,22 +197,26 @@ struct Loader {
     }
   }
 
+  // Loads the cursor's block into a stage: up to NG boxes of keys and of values, and their scales.
   static __device__ __forceinline__ void load(const Cursor& u, uint8_t* stage, float* scales, uint64_t* bar,
-                                              const CUtensorMap* km, const CUtensorMap* vm, const AttendParams& p, int lane) {
-    const int groups = min(C::NG, (u.len - u.j0 + 15) >> 4);
-    if (lane == 0) mbar_arrive_expect_tx(bar, groups * (2 * C::GB + (E4M3 ? 128 : 0)));
-    __syncwarp();
-    const int g = lane % C::NG, kind = lane / C::NG, slot = paged_slot(p.c, u.j0 + g * 16);
-    if (g >= groups) return;
-    int page = u.page;
-    if (page < 0 || page >= p.c.pages) {  // read as page 0
-      atomicOr(p.c.err, kErrPage);
-      page = 0;
+                                              const CUtensorMap* km, const CUtensorMap* vm, const AttendParams& p) {
+    const int boxes = min(C::NG, (min(C::BK, u.len - u.j0) + p.box - 1) / p.box);
+    if (u.page < 0 || u.page >= p.c.pages) atomicOr(p.c.err, kErrPage);
+    const int mine = u.page < 0 || u.page >= p.c.pages ? 0 : u.page;  // a bad number is read as page 0
+    const bool one = elect_one();
+    if (one) mbar_arrive_expect_tx(bar, boxes * p.box * (2 * C::RB + (E4M3 ? 8 : 0)));
+#pragma unroll 1
+    for (int i = 0; i < boxes; ++i) {
+      const int page = __shfl_sync(0xffffffffu, mine, i), slot = paged_slot(p.c, u.j0 + i * p.box);
+      if (one) {
+        tma_load_5d(stage + i * p.box * C::RB, km, bar, 0, slot, 0, u.h, page);
+        tma_load_5d(stage + C::KB + i * p.box * C::RB, vm, bar, 0, slot, 0, u.h, page);
+        if (E4M3) {
+          bulk_load(scales + i * p.box, p.c.k_scale + page * p.c.ks_sp + u.h * p.c.ks_sh + slot, p.box * 4, bar);
+          bulk_load(scales + C::BK + i * p.box, p.c.v_scale + page * p.c.vs_sp + u.h * p.c.vs_sh + slot, p.box * 4, bar);
+        }
+      }
     }
-    if (kind < 2) tma_load_5d(stage + (kind * C::NG + g) * C::GB, kind ? vm : km, bar, 0, slot, 0, u.h, page);
-    if (E4M3 && kind == 2) bulk_load(scales + g * 16, p.c.k_scale + page * p.c.ks_sp + u.h * p.c.ks_sh + slot, 64, bar);
-    if (E4M3 && kind == 3)
-      bulk_load(scales + C::BK + g * 16, p.c.v_scale + page * p.c.vs_sp + u.h * p.c.vs_sh + slot, 64, bar);
   }
 };
 
@@ -290,7 +306,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   u.b = 0;
   int issued = 0, waiting = 0;  // stage of the next load; blocks issued and not consumed yet
   auto issue = [&]() {
-    L::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p, lane);
+    L::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p);
     issued = issued + 1 == p.stages ? 0 : issued + 1;
     ++waiting;
     L::next(u, c1, info, p, lane);
@@ -364,7 +380,9 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     const int first = t + (warp - (t - c0) % W + W) % W;
 #pragma unroll 1
     for (int x = first; x < end && s.count; x += W) {
-      if (dead || !mbar_wait_warp(&my_bars[stage], phase, &s_abort, p.c.err)) {
+      // every lane looks once; only a wait in earnest is left to one lane and its limit
+      if (!__all_sync(0xffffffffu, !dead && mbar_try_wait(&my_bars[stage], phase)) &&
+          (dead || !mbar_wait_warp(&my_bars[stage], phase, &s_abort, p.c.err))) {
         dead = true;
         break;
       }
@@ -376,19 +394,31 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       for (int g = 0; g < groups; ++g) {
         // products of 16 query rows x 16 keys; two accumulators a tile shorten the chain of dependent products
         const uint32_t ka = kb + g * C::GB + k_lane;
-        float sc[2][4] = {}, sd[2][4] = {};
+        float sc[2][4], sd[2][4];
 #pragma unroll
         for (int k = 0; k < KS; k += E4M3 ? 2 : 1) {
           uint32_t r[4];
           if (E4M3) {
             ldsm4(r, chunk_from<C>(ka, k));
 #pragma unroll
-            for (int i = 0; i < 4; ++i)  // r[0], r[1]: keys 0-7 and 8-15 of chunk k; r[2], r[3]: of chunk k + 1
-              mma16<true>(i < 2 ? sc[i] : sd[i - 2], qf[k + (i >> 1)], e4m3_f16(r[i], false), e4m3_f16(r[i], true));
+            for (int i = 0; i < 4; ++i) {  // r[0], r[1]: keys 0-7 and 8-15 of chunk k; r[2], r[3]: of chunk k + 1
+              float(&d)[4] = i < 2 ? sc[i] : sd[i - 2];
+              uint32_t b0, b1;
+              e4m3_f16(r[i], b0, b1);
+              if (k == 0) mma16_first<true>(d, qf[i >> 1], b0, b1);
+              else mma16<true>(d, qf[k + (i >> 1)], b0, b1);
+            }
           } else {
             ldsm4(r, chunk_from<C>(ka, 2 * k));
-            mma16<false>(k & 1 ? sd[0] : sc[0], qf[k], r[0], r[1]);
-            mma16<false>(k & 1 ? sd[1] : sc[1], qf[k], r[2], r[3]);
+            float(&d0)[4] = k & 1 ? sd[0] : sc[0];
+            float(&d1)[4] = k & 1 ? sd[1] : sc[1];
+            if (k < 2) {
+              mma16_first<false>(d0, qf[k], r[0], r[1]);
+              mma16_first<false>(d1, qf[k], r[2], r[3]);
+            } else {
+              mma16<false>(d0, qf[k], r[0], r[1]);
+              mma16<false>(d1, qf[k], r[2], r[3]);
+            }
           }
         }
         const int jg = j0 + g * 16;
@@ -517,7 +547,8 @@ __global__ void __launch_bounds__(C::W * 32, 1)
                 uint32_t v;
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(vg + chunk_at<C>(k, E4M3 ? n / 2 : n) + c4 * 4));
                 if (E4M3) {
-                  const uint32_t lo2 = e4m3_f16(v, false), hi2 = e4m3_f16(v, true);
+                  uint32_t lo2, hi2;
+                  e4m3_f16(v, lo2, hi2);
                   const float x4[4] = {f16lo(lo2), f16hi(lo2), f16lo(hi2), f16hi(hi2)};
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
@@ -550,9 +581,11 @@ __global__ void __launch_bounds__(C::W * 32, 1)
             // columns of the chunk, one for the odd ones
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint32_t x0 = __byte_perm(r[2 * i], 0, 0x3120), x1 = __byte_perm(r[2 * i + 1], 0, 0x3120);
-              mma16<true>(o[2 * (k + i)], a, e4m3_f16(x0, false), e4m3_f16(x1, false));
-              mma16<true>(o[2 * (k + i) + 1], a, e4m3_f16(x0, true), e4m3_f16(x1, true));
+              uint32_t even0, odd0, even1, odd1;
+              e4m3_f16(__byte_perm(r[2 * i], 0, 0x3120), even0, odd0);
+              e4m3_f16(__byte_perm(r[2 * i + 1], 0, 0x3120), even1, odd1);
+              mma16<true>(o[2 * (k + i)], a, even0, even1);
+              mma16<true>(o[2 * (k + i) + 1], a, odd0, odd1);
             }
           }
         } else {
@@ -758,9 +791,9 @@ __global__ void __launch_bounds__(256) weights_kernel(const AttendParams p, floa
 
 // ------------------------------------------------------------------ host
 
-int tile_map(CUtensorMap* map, void* base, const tbf16_paged_cache* c, int64_t sp, int64_t sh, int64_t ss) {
+int tile_map(CUtensorMap* map, void* base, const tbf16_paged_cache* c, int64_t sp, int64_t sh, int64_t ss, int box) {
   const int item = c->dtype == TBF16_E4M3 ? 1 : 2, span = (int)std::min<int64_t>(c->D * item, 128);
-  return tbf16_host::make_tmap_pages(map, base, item, c->D, span, c->page_size, c->heads, c->pages, ss, sh, sp);
+  return tbf16_host::make_tmap_pages(map, base, item, c->D, span, c->page_size, c->heads, c->pages, ss, sh, sp, box);
 }
 
 constexpr int kSmemMax = 227 * 1024;
@@ -775,8 +808,9 @@ constexpr int kSmemStatic = 3 * 1024;
 template <class C>
 int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
   CUtensorMap km, vm;
-  if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss)) return s;
-  if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss)) return s;
+  p.box = (int)std::min<int64_t>(C::BK, cache->page_size);
+  if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss, p.box)) return s;
+  if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss, p.box)) return s;
   // the warps' outputs, or a join's factors (a part for each CTA at the most) and its thread groups' sums
   p.merge = std::max(C::W * p.nr * C::D, sms * p.nr + 4 + C::W * 32 * 4);
   p.stages = kMaxStages;

@@ -146,7 +146,7 @@ int make_tmap_3d_f32(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d
 }
 
 int make_tmap_pages(CUtensorMap* map, const void* base, int item, int64_t D, int span, int64_t slots, int64_t heads,
-                    int64_t pages, int64_t slot_stride, int64_t head_stride, int64_t page_stride) {
+                    int64_t pages, int64_t slot_stride, int64_t head_stride, int64_t page_stride, int box_slots) {
   if (!encode_fn()) return TBF16_ERR_LAUNCH;
   if ((span != 64 && span != 128) || D * item % span) return TBF16_ERR_INVALID;
   const cuuint64_t spans = (cuuint64_t)(D * item / span);
@@ -155,7 +155,7 @@ int make_tmap_pages(CUtensorMap* map, const void* base, int item, int64_t D, int
   cuuint64_t gdim[5] = {(cuuint64_t)(span / item), (cuuint64_t)slots, spans, (cuuint64_t)heads, (cuuint64_t)pages};
   cuuint64_t gstride[4] = {stride(slots, slot_stride), (cuuint64_t)span, stride(heads, head_stride),
                            stride(pages, page_stride)};
-  cuuint32_t box[5] = {(cuuint32_t)(span / item), 16, (cuuint32_t)spans, 1, 1};
+  cuuint32_t box[5] = {(cuuint32_t)(span / item), (cuuint32_t)box_slots, (cuuint32_t)spans, 1, 1};
   cuuint32_t estride[5] = {1, 1, 1, 1, 1};
   CUresult r = g_encode(map, item == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                         const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
