@@ -52,24 +52,29 @@ struct AttendParams {
   unsigned group_inv;                  // ceil(2^32 / group): row / group = umulhi(row, group_inv) below 2^16
   float scale_log2;
   int stages;
-  int box;          // keys that one TMA load brings: min(BK, page size); rows of one span when over 16
+  int box_shift;    // log2 of the keys that one TMA load brings: min(BK, page size); rows of one span when over 16
   int nr;           // rows of an item that can be real: min(rows, kRows)
   int merge;        // floats of the merge area
   unsigned* sync;   // arrivals of each item, zero between calls
-  float* part;      // [2 * CTAs][nr * D + 2 * kRows]: partial outputs, maxima, sums
+  float* part;      // [2 * CTAs][nr * D + 2 * kRows]: partial outputs, (maximum, sum) pairs
   float* logits;    // weights wanted: [batch * heads][rows][cap], base-2 logits
   float* lse;       // and [batch * heads][rows]: log2 of each row's sum
 };
 
-// What a CTA knows of a sequence: first of its blocks among all, blocks of one item, cached and new tokens.
+// What a CTA knows of a sequence: the first of its blocks, and of its rounds, among all; cached and new tokens.
 struct SeqInfo {
-  int cum, blocks, len, count;
+  int cum, rounds, len, count;
 };
 
-// First block that a sequence's window reaches.
+// First block that a sequence's window reaches, and the blocks of one of its items (one empty block writes an
+// idle sequence's zeros).
 template <class C>
 __device__ __forceinline__ int first_block(const AttendParams& p, int len, int count) {
   return p.window ? max(0, len - count + 1 - p.window) / C::BK : 0;
+}
+template <class C>
+__device__ __forceinline__ int item_blocks(const AttendParams& p, int len, int count) {
+  return count ? (len + C::BK - 1) / C::BK - first_block<C>(p, len, count) : 1;
 }
 __device__ __forceinline__ int token_of(const AttendParams& p, int row) {
   return p.group == 1 ? row : (int)__umulhi((unsigned)row, p.group_inv);
@@ -86,11 +91,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 template <bool F16>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -98,11 +103,11 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
 template <bool F16>
 __device__ __forceinline__ void mma16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
@@ -163,7 +168,7 @@ struct Loader {
 
   // Starts loading the page numbers that the cursor's block needs, lane i that of its i-th box.
   static __device__ __forceinline__ void fetch_pages(Cursor& u, const AttendParams& p, int lane) {
-    const int j = u.j0 + lane * p.box;
+    const int j = u.j0 + (lane << p.box_shift);
     u.page = j < min(u.len, u.j0 + C::BK) ? p.c.table[u.b * p.c.table_ld + (j >> p.c.page_shift)] : 0;
   }
 
@@ -176,10 +181,10 @@ struct Loader {
       while (t >= info[u.b + 1].cum) ++u.b;
       const SeqInfo s = info[u.b];
       if (s.count == 0) continue;
-      const unsigned rem = t - s.cum, item = rem / (unsigned)s.blocks;
+      u.blocks = item_blocks<C>(p, s.len, s.count);
+      const unsigned rem = t - s.cum, item = rem / (unsigned)u.blocks;
       u.h = p.chunks == 1 ? (int)item : (int)(item / (unsigned)p.chunks);
-      u.blk = (int)(rem - item * s.blocks);
-      u.blocks = s.blocks;
+      u.blk = (int)(rem - item * u.blocks);
       u.j0 = (first_block<C>(p, s.len, s.count) + u.blk) * C::BK;
       u.len = s.len;
       break;
@@ -200,20 +205,20 @@ struct Loader {
   // Loads the cursor's block into a stage: up to NG boxes of keys and of values, and their scales.
   static __device__ __forceinline__ void load(const Cursor& u, uint8_t* stage, float* scales, uint64_t* bar,
                                               const CUtensorMap* km, const CUtensorMap* vm, const AttendParams& p) {
-    const int boxes = min(C::NG, (min(C::BK, u.len - u.j0) + p.box - 1) / p.box);
+    const int box = 1 << p.box_shift, boxes = (min(C::BK, u.len - u.j0) + box - 1) >> p.box_shift;
     if (u.page < 0 || u.page >= p.c.pages) atomicOr(p.c.err, kErrPage);
     const int mine = u.page < 0 || u.page >= p.c.pages ? 0 : u.page;  // a bad number is read as page 0
     const bool one = elect_one();
-    if (one) mbar_arrive_expect_tx(bar, boxes * p.box * (2 * C::RB + (E4M3 ? 8 : 0)));
+    if (one) mbar_arrive_expect_tx(bar, boxes * box * (2 * C::RB + (E4M3 ? 8 : 0)));
 #pragma unroll 1
     for (int i = 0; i < boxes; ++i) {
-      const int page = __shfl_sync(0xffffffffu, mine, i), slot = paged_slot(p.c, u.j0 + i * p.box);
+      const int page = __shfl_sync(0xffffffffu, mine, i), slot = paged_slot(p.c, u.j0 + i * box);
       if (one) {
-        tma_load_5d(stage + i * p.box * C::RB, km, bar, 0, slot, 0, u.h, page);
-        tma_load_5d(stage + C::KB + i * p.box * C::RB, vm, bar, 0, slot, 0, u.h, page);
+        tma_load_5d(stage + i * box * C::RB, km, bar, 0, slot, 0, u.h, page);
+        tma_load_5d(stage + C::KB + i * box * C::RB, vm, bar, 0, slot, 0, u.h, page);
         if (E4M3) {
-          bulk_load(scales + i * p.box, p.c.k_scale + page * p.c.ks_sp + u.h * p.c.ks_sh + slot, p.box * 4, bar);
-          bulk_load(scales + C::BK + i * p.box, p.c.v_scale + page * p.c.vs_sp + u.h * p.c.vs_sh + slot, p.box * 4, bar);
+          bulk_load(scales + i * box, p.c.k_scale + page * p.c.ks_sp + u.h * p.c.ks_sh + slot, box * 4, bar);
+          bulk_load(scales + C::BK + i * box, p.c.v_scale + page * p.c.vs_sp + u.h * p.c.vs_sh + slot, box * 4, bar);
         }
       }
     }
@@ -242,8 +247,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + p.merge);
   __shared__ uint64_t bars[W * kMaxStages];
   __shared__ float s_m[W][kRows], s_l[W][kRows];  // each warp's maxima and sums
-  __shared__ float s_sum[kRows];
-  __shared__ int s_scan[W], s_work[W], s_abort, s_last;
+  __shared__ int s_scan[W], s_work[W], s_abort, s_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((smem_u32(smem) & 1023u) != 0) {
     if (tid == 0) atomicOr(p.c.err, kErrSmemAlign);
@@ -254,56 +258,70 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   if (tid == 0) s_abort = 0;
   fence_barrier_init();
 
-  // every sequence's blocks and their running total; `work`: CTAs that would give each warp at most one block
+  // Every sequence's blocks and rounds (a round: a block for each warp) and their running totals.
   int total = 0, work = 0;
   for (int b0 = 0; b0 < p.c.batch; b0 += NTHREADS) {
     const int b = b0 + tid;
     SeqInfo s{0, 0, 0, 0};
-    int x = 0, ctas_wanted = 0;
+    int x = 0, y = 0;
     if (b < p.c.batch) {
       s.len = paged_len(p.c, b);
       s.count = paged_count(p.c, p.counts, b, p.T, s.len);
-      // one empty block writes an idle sequence's zeros
-      s.blocks = s.count ? (s.len + C::BK - 1) / C::BK - first_block<C>(p, s.len, s.count) : 1;
-      x = s.blocks * p.c.heads * p.chunks;
-      ctas_wanted = (s.blocks + W - 1) / W * p.c.heads * p.chunks;
+      const int blocks = item_blocks<C>(p, s.len, s.count);
+      x = blocks * p.c.heads * p.chunks;
+      y = (blocks + W - 1) / W * p.c.heads * p.chunks;
     }
-    const int mine = x;
+    const int my_x = x, my_y = y;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      const int dx = __shfl_up_sync(0xffffffffu, x, o), dy = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) x += dx, y += dy;
     }
-    ctas_wanted = __reduce_add_sync(0xffffffffu, ctas_wanted);
     if (lane == 31) {
       s_scan[warp] = x;
-      s_work[warp] = ctas_wanted;
+      s_work[warp] = y;
     }
     __syncthreads();
-    int before = total;
+    x += total - my_x;
+    y += work - my_y;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      before += i < warp ? s_scan[i] : 0;
+      if (i < warp) x += s_scan[i], y += s_work[i];
       total += s_scan[i];
       work += s_work[i];
     }
-    s.cum = before + x - mine;
+    s.cum = x;
+    s.rounds = y;
     if (b < p.c.batch) info[b] = s;
-    if (b == p.c.batch - 1) info[b + 1] = SeqInfo{before + x, 1, 0, 0};
+    if (b == p.c.batch - 1) info[b + 1] = SeqInfo{x + my_x, y + my_y, 0, 0};
     __syncthreads();
   }
-  const int ctas = min((int)gridDim.x, work);
+  // Few rounds: a CTA takes one, so no item waits for another. Else CTA i takes blocks [share(i), share(i + 1)):
+  // `each` of them, the first `more` CTAs one more.
+  const bool by_round = work <= (int)gridDim.x;
+  const int ctas = by_round ? work : (int)gridDim.x;
   if ((int)blockIdx.x >= ctas) return;
-  // CTA i takes blocks [share(i), share(i + 1)): `each` of them, the first `more` CTAs one more
   const int each = total / ctas, more = total - each * ctas;
   auto share = [&](int i) { return each * i + min(i, more); };
-  const int c0 = share(blockIdx.x), c1 = share(blockIdx.x + 1);
+  int c0 = share(blockIdx.x), c1 = share(blockIdx.x + 1), b = 0;
+  for (int hi = p.c.batch; hi - b > 1;) {
+    const int mid = (b + hi) >> 1;
+    if (by_round ? info[mid].rounds <= (int)blockIdx.x : info[mid].cum <= c0) b = mid;
+    else hi = mid;
+  }
+  if (by_round) {
+    const SeqInfo s = info[b];
+    const int blocks = item_blocks<C>(p, s.len, s.count), rounds = (blocks + W - 1) / W, x = blockIdx.x - s.rounds;
+    const int item = x / rounds, r = x - item * rounds;
+    c0 = s.cum + item * blocks + r * W;
+    c1 = s.cum + item * blocks + min(blocks, (r + 1) * W);
+  }
 
   uint8_t* my_ring = ring + (size_t)warp * p.stages * 2 * C::KB;
   float* my_scales = scale_ring + (size_t)warp * p.stages * (C::SC / 4);
   uint64_t* my_bars = bars + warp * p.stages;
   Cursor u;
-  u.b = 0;
+  u.b = b;
   int issued = 0, waiting = 0;  // stage of the next load; blocks issued and not consumed yet
   auto issue = [&]() {
     L::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p);
@@ -322,15 +340,46 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   const uint32_t k_lane = E4M3 ? chunk_at<C>(lane & 15, lane >> 4) : chunk_at<C>(((lane >> 4) & 1) * 8 + (lane & 7), (lane >> 3) & 1);
   const uint32_t v_lane = chunk_at<C>(lane & 15, lane >> 4);
 
-  int b = 0;
+  // The item that holds block t.
+  struct Item {
+    SeqInfo s;
+    int start, blocks, b, h, row0, nrow;
+  };
+  auto item_at = [&](int t, int from) {
+    Item it;
+    it.b = from;
+    while (t >= info[it.b + 1].cum) ++it.b;
+    it.s = info[it.b];
+    it.blocks = item_blocks<C>(p, it.s.len, it.s.count);
+    const int i = (int)((unsigned)(t - it.s.cum) / (unsigned)it.blocks);
+    it.start = it.s.cum + i * it.blocks;
+    it.h = p.chunks == 1 ? i : i / p.chunks;
+    it.row0 = (i - it.h * p.chunks) * kRows;
+    it.nrow = min(kRows, p.rows - it.row0);
+    return it;
+  };
+  // v / sum as bf16; zeros for rows that see nothing
+  auto store = [&](const Item& it, int r, int d, float4 v, float sum) {
+    const int row = it.row0 + r, tok = token_of(p, row);
+    const float f = sum == 0.f || tok >= it.s.count ? 0.f : 1.f / sum;
+    if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<uint2*>(p.out + it.b * p.o_sb + (int64_t)(it.h * p.group + row - tok * p.group) * p.o_sh + tok * p.o_st +
+                              d) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+  };
+  auto store_lse = [&](const Item& it, int r, float m, float sum) {
+    if (p.lse) p.lse[(int64_t)(it.b * p.c.heads + it.h) * p.rows + it.row0 + r] = m + log2f(sum);
+  };
+  const size_t part_ld = p.nr * D + 2 * kRows;
+  int open[2] = {-1, -1};  // a block of the item whose partial stands in slot 0 (the CTA's first item) and 1 (its last)
+
+  const int first_b = b;
 #pragma unroll 1
   for (int t = c0; t < c1;) {
-    while (t >= info[b + 1].cum) ++b;
-    const SeqInfo s = info[b];
-    const int item = (int)((unsigned)(t - s.cum) / (unsigned)s.blocks), start = s.cum + item * s.blocks;
-    const int end = min(c1, start + s.blocks);
-    const int h = p.chunks == 1 ? item : item / p.chunks, row0 = (item - h * p.chunks) * kRows;
-    const int nrow = min(kRows, p.rows - row0);
+    const Item it = item_at(t, b);
+    const SeqInfo s = it.s;
+    const int start = it.start, h = it.h, row0 = it.row0, nrow = it.nrow;
+    const int end = min(c1, start + it.blocks);
+    b = it.b;
     const int lo = first_block<C>(p, s.len, s.count);
     // query rows g4 and g4 + 8 of the item: their A fragments and positions
     uint32_t qf[KS][4];
@@ -395,29 +444,35 @@ __global__ void __launch_bounds__(C::W * 32, 1)
         // products of 16 query rows x 16 keys; two accumulators a tile shorten the chain of dependent products
         const uint32_t ka = kb + g * C::GB + k_lane;
         float sc[2][4], sd[2][4];
+        // fragments come in batches of four loads, so that one load's latency is met per batch
+        constexpr int KI = E4M3 ? KS / 2 : KS, KB4 = KI < 4 ? KI : 4;
 #pragma unroll
-        for (int k = 0; k < KS; k += E4M3 ? 2 : 1) {
-          uint32_t r[4];
-          if (E4M3) {
-            ldsm4(r, chunk_from<C>(ka, k));
+        for (int k0 = 0; k0 < KI; k0 += KB4) {
+          uint32_t r[KB4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // r[0], r[1]: keys 0-7 and 8-15 of chunk k; r[2], r[3]: of chunk k + 1
-              float(&d)[4] = i < 2 ? sc[i] : sd[i - 2];
-              uint32_t b0, b1;
-              e4m3_f16(r[i], b0, b1);
-              if (k == 0) mma16_first<true>(d, qf[i >> 1], b0, b1);
-              else mma16<true>(d, qf[k + (i >> 1)], b0, b1);
-            }
-          } else {
-            ldsm4(r, chunk_from<C>(ka, 2 * k));
-            float(&d0)[4] = k & 1 ? sd[0] : sc[0];
-            float(&d1)[4] = k & 1 ? sd[1] : sc[1];
-            if (k < 2) {
-              mma16_first<false>(d0, qf[k], r[0], r[1]);
-              mma16_first<false>(d1, qf[k], r[2], r[3]);
+          for (int k = 0; k < KB4; ++k) ldsm4(r[k], chunk_from<C>(ka, 2 * (k0 + k)));
+#pragma unroll
+          for (int kk = 0; kk < KB4; ++kk) {
+            const int k = k0 + kk;
+            if (E4M3) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {  // 0, 1: keys 0-7 and 8-15 of chunk 2 k; 2, 3: of chunk 2 k + 1
+                float(&d)[4] = i < 2 ? sc[i] : sd[i - 2];
+                uint32_t b0, b1;
+                e4m3_f16(r[kk][i], b0, b1);
+                if (k == 0) mma16_first<true>(d, qf[i >> 1], b0, b1);
+                else mma16<true>(d, qf[2 * k + (i >> 1)], b0, b1);
+              }
             } else {
-              mma16<false>(d0, qf[k], r[0], r[1]);
-              mma16<false>(d1, qf[k], r[2], r[3]);
+              float(&d0)[4] = k & 1 ? sd[0] : sc[0];
+              float(&d1)[4] = k & 1 ? sd[1] : sc[1];
+              if (k < 2) {
+                mma16_first<false>(d0, qf[k], r[kk][0], r[kk][1]);
+                mma16_first<false>(d1, qf[k], r[kk][2], r[kk][3]);
+              } else {
+                mma16<false>(d0, qf[k], r[kk][0], r[kk][1]);
+                mma16<false>(d1, qf[k], r[kk][2], r[kk][3]);
+              }
             }
           }
         }
@@ -568,44 +623,44 @@ __global__ void __launch_bounds__(C::W * 32, 1)
             }
           }
         }
-        if (E4M3) {
-          // fp16 weights: 11 bits, on values that are exact in fp16
-          const uint32_t a[4] = {pack_f16(pw[0][0], pw[0][1]), pack_f16(pw[0][2], pw[0][3]), pack_f16(pw[1][0], pw[1][1]),
-                                 pack_f16(pw[1][2], pw[1][3])};
+        // weights as the products' A operand. e4m3: fp16, 11 bits, on values that are exact in fp16. bf16: in two parts
+        // (16 bits of them): one part would add its 2^-9 to the output's own rounding
+        uint32_t hi[4], lw[4];
 #pragma unroll
-          for (int k = 0; k < KS; k += 2) {
-            uint32_t r[4];
-            ldsm4t(r, chunk_from<C>(va, k));
-            if (odd) finite_only<E4M3>(r);
-            // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: pair the keys, one tile for the even
-            // columns of the chunk, one for the odd ones
+        for (int i = 0; i < 4; ++i) {
+          const float y = pw[i >> 1][2 * (i & 1)], z = pw[i >> 1][2 * (i & 1) + 1];
+          hi[i] = E4M3 ? pack_f16(y, z) : pack_bf16(y, z);
+          if (!E4M3) lw[i] = pack_bf16(y - bf16lo(hi[i]), z - bf16hi(hi[i]));
+        }
+        constexpr int VI = E4M3 ? KS / 2 : NT / 2, VB4 = VI < 4 ? VI : 4;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t even0, odd0, even1, odd1;
-              e4m3_f16(__byte_perm(r[2 * i], 0, 0x3120), even0, odd0);
-              e4m3_f16(__byte_perm(r[2 * i + 1], 0, 0x3120), even1, odd1);
-              mma16<true>(o[2 * (k + i)], a, even0, even1);
-              mma16<true>(o[2 * (k + i) + 1], a, odd0, odd1);
+        for (int k0 = 0; k0 < VI; k0 += VB4) {
+          uint32_t r[VB4][4];
+#pragma unroll
+          for (int k = 0; k < VB4; ++k) {
+            ldsm4t(r[k], chunk_from<C>(va, 2 * (k0 + k)));
+            if (odd) finite_only<E4M3>(r[k]);
+          }
+#pragma unroll
+          for (int kk = 0; kk < VB4; ++kk) {
+            const int k = 2 * (k0 + kk);
+            if (E4M3) {
+              // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: pair the keys, one tile for the even
+              // columns of the chunk, one for the odd ones
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint32_t even0, odd0, even1, odd1;
+                e4m3_f16(__byte_perm(r[kk][2 * i], 0, 0x3120), even0, odd0);
+                e4m3_f16(__byte_perm(r[kk][2 * i + 1], 0, 0x3120), even1, odd1);
+                mma16<true>(o[2 * (k + i)], hi, even0, even1);
+                mma16<true>(o[2 * (k + i) + 1], hi, odd0, odd1);
+              }
+            } else {
+              mma16<false>(o[k], hi, r[kk][0], r[kk][1]);
+              mma16<false>(o[k + 1], hi, r[kk][2], r[kk][3]);
+              mma16<false>(o[k], lw, r[kk][0], r[kk][1]);
+              mma16<false>(o[k + 1], lw, r[kk][2], r[kk][3]);
             }
-          }
-        } else {
-          // bf16 weights in two parts (16 bits of them): one part would add its 2^-9 to the output's own rounding
-          uint32_t hi[4], lw[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float y = pw[i >> 1][2 * (i & 1)], z = pw[i >> 1][2 * (i & 1) + 1];
-            hi[i] = pack_bf16(y, z);
-            lw[i] = pack_bf16(y - bf16lo(hi[i]), z - bf16hi(hi[i]));
-          }
-#pragma unroll
-          for (int n = 0; n < NT; n += 2) {
-            uint32_t r[4];
-            ldsm4t(r, chunk_from<C>(va, n));
-            if (odd) finite_only<E4M3>(r);
-            mma16<false>(o[n], hi, r[0], r[1]);
-            mma16<false>(o[n + 1], hi, r[2], r[3]);
-            mma16<false>(o[n], lw, r[0], r[1]);
-            mma16<false>(o[n + 1], lw, r[2], r[3]);
           }
         }
       }
@@ -640,16 +695,11 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       }
     }
     __syncthreads();
-    const bool split = end - t != s.blocks;
-    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * (p.nr * D + 2 * kRows);
-    // v / sum as bf16; zeros for rows that see nothing
-    auto store = [&](int r, int d, float4 v, float sum) {
-      const int row = row0 + r, tok = token_of(p, row);
-      const float f = sum == 0.f || tok >= s.count ? 0.f : 1.f / sum;
-      if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * p.group + row - tok * p.group) * p.o_sh + tok * p.o_st + d) =
-          make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
-    };
+    const bool split = end - t != it.blocks;
+    const int slot = t == c0 ? 0 : 1;
+    float* part = p.part + (2 * (size_t)blockIdx.x + slot) * part_ld;
+    if (split && slot == 0) open[0] = t;
+    if (split && slot == 1) open[1] = t;
 #pragma unroll 1
     for (int i = tid; i < nrow * (D / 4); i += NTHREADS) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
@@ -666,88 +716,120 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       }
       if (split) {
         *reinterpret_cast<float4*>(part + r * D + d) = v;
-        if (d == 0) {
-          part[p.nr * D + r] = a;
-          part[p.nr * D + kRows + r] = sum;
-        }
+        if (d == 0) *reinterpret_cast<float2*>(part + p.nr * D + 2 * r) = make_float2(a, sum);
       } else {
-        store(r, d, v, sum);
-        if (p.lse && d == 0) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + r] = a + log2f(sum);
-      }
-    }
-    if (split) {
-      // the CTAs whose blocks the item's first and last one are: theirs and all between hold a partial
-      auto owner = [&](int x) {
-        const int big = more * (each + 1);
-        return x < big ? x / (each + 1) : more + (x - big) / each;
-      };
-      const int i0 = owner(start), parts = owner(start + s.blocks - 1) - i0 + 1;
-      const bool skip0 = share(i0) < start;  // CTA i0 has another item before this one
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        unsigned* word = p.sync + ((size_t)b * p.c.heads + h) * p.chunks + row0 / kRows;
-        const bool last = atomicAdd(word, 1u) == (unsigned)parts - 1;
-        if (last) *word = 0;
-        s_last = last;
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        const size_t ld = p.nr * D + 2 * kRows;
-        const float* p0 = p.part + 2 * (size_t)i0 * ld;
-        auto at_part = [&](int i) { return p0 + (2 * (size_t)i + (i == 0 && skip0 ? 1 : 0)) * ld; };
-        float* fac = merge;  // [parts][nr], then the thread groups' sums
-        float* sums = merge + (parts * p.nr + 3) / 4 * 4;
-        for (int r = warp; r < nrow; r += W) {
-          float a = kNoMax, sum = 0.f;
-          for (int i = lane; i < parts; i += 32) a = fmaxf(a, __ldcg(at_part(i) + p.nr * D + r));
-          a = warp_max(a);
-          for (int i = lane; i < parts; i += 32) {
-            const float* x = at_part(i) + p.nr * D + r;
-            const float f = ex2(__ldcg(x) - a);
-            fac[i * p.nr + r] = f;
-            sum += __ldcg(x + kRows) * f;
-          }
-#pragma unroll
-          for (int o2 = 16; o2 > 0; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
-          if (lane == 0) {
-            s_sum[r] = sum;
-            if (p.lse) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row0 + r] = a + log2f(sum);
-          }
-        }
-        __syncthreads();
-        // `teams` groups of threads take every teams-th part each
-        const int n4 = nrow * (D / 4), teams = max(1, min(parts, NTHREADS / n4));
-        const int team = teams == 1 ? 0 : tid / n4;
-#pragma unroll 1
-        for (int i = teams == 1 ? tid : tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
-          const int r = i / (D / 4), d = i % (D / 4) * 4;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int k = team; k < parts; k += teams) {
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(at_part(k) + r * D + d));
-            const float f = fac[k * p.nr + r];
-            v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
-          }
-          if (teams == 1) store(r, d, v, s_sum[r]);
-          else *reinterpret_cast<float4*>(sums + ((size_t)team * n4 + i) * 4) = v;
-        }
-        if (teams > 1) {
-          __syncthreads();
-          if (tid < n4) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = 0; k < teams; ++k) {
-              const float4 y = *reinterpret_cast<const float4*>(sums + ((size_t)k * n4 + tid) * 4);
-              v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-            }
-            store(tid / (D / 4), tid % (D / 4) * 4, v, s_sum[tid / (D / 4)]);
-          }
-        }
+        store(it, r, d, v, sum);
+        if (d == 0) store_lse(it, r, a, sum);
       }
     }
     __syncthreads();  // merge and the sums are free
     t = end;
+  }
+
+  // The CTA's partials are out (at most that of its first and that of its last item). Only now it says so, so that
+  // no item of its own waited for a join: the last of an item's CTAs to say so adds the partials up.
+  if (open[0] >= 0 || open[1] >= 0) {
+    auto owner = [&](int x) {  // the CTA that has block x
+      const int big = more * (each + 1);
+      return x < big ? x / (each + 1) : more + (x - big) / each;
+    };
+    auto cover = [&](const Item& it, int& i0) {  // the CTAs that hold a partial: i0 and the parts - 1 after it
+      if (by_round) {
+        const int rounds = (it.blocks + W - 1) / W;
+        i0 = it.s.rounds + (it.h * p.chunks + it.row0 / kRows) * rounds;
+        return rounds;
+      }
+      i0 = owner(it.start);
+      return owner(it.start + it.blocks - 1) - i0 + 1;
+    };
+    if (tid == 0) {
+      __threadfence();  // with the barrier above: every thread's partials, before the counts
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        s_last[k] = 0;
+        if (open[k] < 0) continue;
+        const Item it = item_at(open[k], first_b);
+        int i0;
+        const int parts = cover(it, i0);
+        unsigned* word = p.sync + ((size_t)it.b * p.c.heads + it.h) * p.chunks + it.row0 / kRows;
+        if (atomicAdd(word, 1u) == (unsigned)parts - 1) {
+          *word = 0;
+          s_last[k] = 1;
+        }
+      }
+      __threadfence();
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+      if (!s_last[k]) continue;
+      const Item it = item_at(open[k], first_b);
+      int i0;
+      const int parts = cover(it, i0);
+      // CTA i0's partial is its slot 1 where it had another item before this one
+      const size_t skip0 = !by_round && share(i0) < it.start ? part_ld : 0;
+      const float* p0 = p.part + 2 * (size_t)i0 * part_ld;
+      // `teams` groups of threads take every teams-th part each, eight loads in flight
+      const int n4 = it.nrow * (D / 4), teams = max(1, min((parts + 3) / 4, NTHREADS / n4));
+      const int team = teams == 1 ? 0 : tid / n4;
+      float2* team_ms = reinterpret_cast<float2*>(merge + NTHREADS * 4);
+#pragma unroll 1
+      for (int i = teams == 1 ? tid : tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float a = kNoMax, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int k0 = team; k0 < parts; k0 += 8 * teams) {
+          float2 ms[8];
+          float4 y[8];
+          float top = a;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int x = k0 + j * teams;
+            const float* at = p0 + 2 * (size_t)x * part_ld + (x == 0 ? skip0 : 0);
+            ms[j] = x < parts ? __ldcg(reinterpret_cast<const float2*>(at + p.nr * D + 2 * r)) : make_float2(kNoMax, 0.f);
+            y[j] = x < parts ? __ldcg(reinterpret_cast<const float4*>(at + r * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = fmaxf(top, ms[j].x);
+          float f = ex2(a - top);
+          a = top;
+          sum *= f;
+          v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            f = ex2(ms[j].x - top);
+            sum += ms[j].y * f;
+            v.x += y[j].x * f; v.y += y[j].y * f; v.z += y[j].z * f; v.w += y[j].w * f;
+          }
+        }
+        if (teams == 1) {
+          store(it, r, d, v, sum);
+          if (d == 0) store_lse(it, r, a, sum);
+        } else {
+          *reinterpret_cast<float4*>(merge + tid * 4) = v;
+          team_ms[tid] = make_float2(a, sum);
+        }
+      }
+      if (teams > 1) {
+        __syncthreads();
+        if (tid < n4) {
+          float a = kNoMax, sum = 0.f;
+          for (int x = 0; x < teams; ++x) a = fmaxf(a, team_ms[x * n4 + tid].x);
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int x = 0; x < teams; ++x) {
+            const float4 y = *reinterpret_cast<const float4*>(merge + (x * n4 + tid) * 4);
+            const float2 ms = team_ms[x * n4 + tid];
+            const float f = ex2(ms.x - a);
+            sum += ms.y * f;
+            v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
+          }
+          store(it, tid / (D / 4), tid % (D / 4) * 4, v, sum);
+          if (tid % (D / 4) == 0) store_lse(it, tid / (D / 4), a, sum);
+        }
+        __syncthreads();
+      }
+    }
   }
   if (dead) {  // see this warp's copies in flight through, again with a limit, before leaving
     for (int i = 0; lane == 0 && i < waiting; ++i) {
@@ -808,11 +890,12 @@ constexpr int kSmemStatic = 3 * 1024;
 template <class C>
 int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
   CUtensorMap km, vm;
-  p.box = (int)std::min<int64_t>(C::BK, cache->page_size);
-  if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss, p.box)) return s;
-  if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss, p.box)) return s;
-  // the warps' outputs, or a join's factors (a part for each CTA at the most) and its thread groups' sums
-  p.merge = std::max(C::W * p.nr * C::D, sms * p.nr + 4 + C::W * 32 * 4);
+  const int box = (int)std::min<int64_t>(C::BK, cache->page_size);
+  p.box_shift = 0;
+  while ((1 << p.box_shift) < box) ++p.box_shift;
+  if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss, box)) return s;
+  if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss, box)) return s;
+  p.merge = std::max(C::W * p.nr * C::D, C::W * 32 * 6);  // the warps' outputs, or a join's thread groups' sums
   p.stages = kMaxStages;
   while (p.stages > 1 && attend_smem<C>(p, p.stages) + kSmemStatic > kSmemMax) --p.stages;
   const int smem = attend_smem<C>(p, p.stages);
