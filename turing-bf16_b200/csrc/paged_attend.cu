@@ -246,17 +246,23 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   float* merge = scale_ring + (size_t)W * p.stages * (C::SC / 4);
   SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + p.merge);
   __shared__ uint64_t bars[W * kMaxStages];
-  __shared__ float s_m[W][kRows], s_l[W][kRows];  // each warp's maxima and sums
-  __shared__ int s_scan[W], s_work[W], s_abort, s_last[2];
+  __shared__ float2 s_ms[W * kRows];   // each warp's (maximum, sum) of a row
+  __shared__ float2 s_team[NTHREADS];  // that of a row in each thread group of a join
+  __shared__ int s_scan[W], s_work[W], s_abort, s_todo;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((smem_u32(smem) & 1023u) != 0) {
     if (tid == 0) atomicOr(p.c.err, kErrSmemAlign);
     return;
   }
-  pdl_launch_dependents();
+  if (tid == 0) {
+    tma_prefetch_desc(&km);
+    tma_prefetch_desc(&vm);
+  }
   if (lane < p.stages) mbar_init(&bars[warp * p.stages + lane], 1);
   if (tid == 0) s_abort = 0;
   fence_barrier_init();
+  pdl_launch_dependents();
+  pdl_wait();
 
   // Every sequence's blocks and rounds (a round: a block for each warp) and their running totals.
   int total = 0, work = 0;
@@ -303,14 +309,14 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   if ((int)blockIdx.x >= ctas) return;
   const int each = total / ctas, more = total - each * ctas;
   auto share = [&](int i) { return each * i + min(i, more); };
-  int c0 = share(blockIdx.x), c1 = share(blockIdx.x + 1), b = 0;
-  for (int hi = p.c.batch; hi - b > 1;) {
-    const int mid = (b + hi) >> 1;
-    if (by_round ? info[mid].rounds <= (int)blockIdx.x : info[mid].cum <= c0) b = mid;
+  int c0 = share(blockIdx.x), c1 = share(blockIdx.x + 1), first_b = 0;
+  for (int hi = p.c.batch; hi - first_b > 1;) {
+    const int mid = (first_b + hi) >> 1;
+    if (by_round ? info[mid].rounds <= (int)blockIdx.x : info[mid].cum <= c0) first_b = mid;
     else hi = mid;
   }
   if (by_round) {
-    const SeqInfo s = info[b];
+    const SeqInfo s = info[first_b];
     const int blocks = item_blocks<C>(p, s.len, s.count), rounds = (blocks + W - 1) / W, x = blockIdx.x - s.rounds;
     const int item = x / rounds, r = x - item * rounds;
     c0 = s.cum + item * blocks + r * W;
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   float* my_scales = scale_ring + (size_t)warp * p.stages * (C::SC / 4);
   uint64_t* my_bars = bars + warp * p.stages;
   Cursor u;
-  u.b = b;
+  u.b = first_b;
   int issued = 0, waiting = 0;  // stage of the next load; blocks issued and not consumed yet
   auto issue = [&]() {
     L::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p);
@@ -358,28 +364,76 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     it.nrow = min(kRows, p.rows - it.row0);
     return it;
   };
-  // v / sum as bf16; zeros for rows that see nothing
-  auto store = [&](const Item& it, int r, int d, float4 v, float sum) {
-    const int row = it.row0 + r, tok = token_of(p, row);
-    const float f = sum == 0.f || tok >= it.s.count ? 0.f : 1.f / sum;
-    if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-    *reinterpret_cast<uint2*>(p.out + it.b * p.o_sb + (int64_t)(it.h * p.group + row - tok * p.group) * p.o_sh + tok * p.o_st +
-                              d) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
-  };
-  auto store_lse = [&](const Item& it, int r, float m, float sum) {
-    if (p.lse) p.lse[(int64_t)(it.b * p.c.heads + it.h) * p.rows + it.row0 + r] = m + log2f(sum);
-  };
   const size_t part_ld = p.nr * D + 2 * kRows;
-  int open[2] = {-1, -1};  // a block of the item whose partial stands in slot 0 (the CTA's first item) and 1 (its last)
+  auto owner = [&](int x) {  // the CTA that has block x
+    const int big = more * (each + 1);
+    return x < big ? x / (each + 1) : more + (x - big) / each;
+  };
+  // The partials the CTA leaves, of its first item (slot 0) and its last (1): a block of the item, the first of
+  // the CTAs that hold a partial of it and their number, and the word where they are counted.
+  int open0 = -1, open1 = -1, at0 = 0, at1 = 0, parts0 = 0, parts1 = 0, word0 = 0, word1 = 0;
+  int todo = -1;  // joins that are this CTA's (bit 0, 1), once its own items are done
 
-  const int first_b = b;
+  // One pass for each item of the CTA, then one for each join. Both share the code that adds up partials: the
+  // instructions of a short call run once, and fetching them is a good part of its time.
 #pragma unroll 1
-  for (int t = c0; t < c1;) {
-    const Item it = item_at(t, b);
+  for (int t = c0;;) {
+    const bool join = t >= c1;
+    if (join) {
+      if (todo < 0) {
+        if (open0 < 0 && open1 < 0) break;
+        // Only now the CTA says that its partials are out, so that no item of its own waited for a join. The last
+        // of an item's CTAs to say so joins the item.
+        if (tid == 0) {
+          __threadfence();  // with the barrier before: every thread's partials, before the counts
+          int mine = 0;
+          if (open0 >= 0 && atomicAdd(p.sync + word0, 1u) == (unsigned)parts0 - 1) mine = 1, p.sync[word0] = 0;
+          if (open1 >= 0 && atomicAdd(p.sync + word1, 1u) == (unsigned)parts1 - 1) mine |= 2, p.sync[word1] = 0;
+          s_todo = mine;
+          __threadfence();
+        }
+        __syncthreads();
+        todo = s_todo;
+      }
+      if (todo == 0) break;
+    }
+    const Item it = item_at(!join ? t : todo & 1 ? open0 : open1, first_b);
     const SeqInfo s = it.s;
-    const int start = it.start, h = it.h, row0 = it.row0, nrow = it.nrow;
-    const int end = min(c1, start + it.blocks);
-    b = it.b;
+    const int start = it.start, h = it.h, row0 = it.row0, nrow = it.nrow, b = it.b;
+    const int end = min(c1, start + it.blocks), n4 = nrow * (D / 4);
+    // the partials to add up: part k's outputs from src + k src_ld, its (maximum, sum) pairs from ms + k ms_ld
+    const float* src = merge;
+    const float2* ms = s_ms;
+    size_t src_ld = p.nr * D, ms_ld = kRows, skip0 = 0;  // skip0: part 0 lies that much further on
+    int parts = W, teams = 1;
+    bool split = false;
+    if (join) {
+      const bool first = todo & 1;
+      const int i0 = first ? at0 : at1;
+      todo &= first ? 2 : 0;
+      parts = first ? parts0 : parts1;
+      src = p.part + 2 * (size_t)i0 * part_ld;
+      src_ld = 2 * part_ld;
+      ms = reinterpret_cast<const float2*>(src + p.nr * D);
+      ms_ld = part_ld;
+      if (!by_round && share(i0) < start) skip0 = part_ld;  // that CTA had another item before this one
+      // groups of threads share the parts out
+      teams = max(1, min((parts + 3) / 4, NTHREADS / n4));
+    } else {
+    split = end - t != it.blocks;
+    if (split) {
+      int i0, n;
+      if (by_round) {
+        n = (it.blocks + W - 1) / W;
+        i0 = s.rounds + (h * p.chunks + row0 / kRows) * n;
+      } else {
+        i0 = owner(start);
+        n = owner(start + it.blocks - 1) - i0 + 1;
+      }
+      const int word = (b * p.c.heads + h) * p.chunks + row0 / kRows;
+      if (t == c0) open0 = t, at0 = i0, parts0 = n, word0 = word;
+      else open1 = t, at1 = i0, parts1 = n, word1 = word;
+    }
     const int lo = first_block<C>(p, s.len, s.count);
     // query rows g4 and g4 + 8 of the item: their A fragments and positions
     uint32_t qf[KS][4];
@@ -675,10 +729,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] = quad_sum(l[i]);
-      if (c4 == 0) {
-        s_m[warp][g4 + i * 8] = m[i];
-        s_l[warp][g4 + i * 8] = l[i];
-      }
+      if (c4 == 0) s_ms[warp * kRows + g4 + i * 8] = make_float2(m[i], l[i]);
       if (g4 + i * 8 < p.nr) {
         float* dst = merge + ((size_t)warp * p.nr + g4 + i * 8) * D;
         if (E4M3) {
@@ -695,141 +746,73 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       }
     }
     __syncthreads();
-    const bool split = end - t != it.blocks;
-    const int slot = t == c0 ? 0 : 1;
-    float* part = p.part + (2 * (size_t)blockIdx.x + slot) * part_ld;
-    if (split && slot == 0) open[0] = t;
-    if (split && slot == 1) open[1] = t;
-#pragma unroll 1
-    for (int i = tid; i < nrow * (D / 4); i += NTHREADS) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
-      float a = kNoMax, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) a = fmaxf(a, s_m[w][r]);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(merge + ((size_t)w * p.nr + r) * D + d);
-        const float f = ex2(s_m[w][r] - a);
-        sum += s_l[w][r] * f;
-        v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
-      }
-      if (split) {
-        *reinterpret_cast<float4*>(part + r * D + d) = v;
-        if (d == 0) *reinterpret_cast<float2*>(part + p.nr * D + 2 * r) = make_float2(a, sum);
-      } else {
-        store(it, r, d, v, sum);
-        if (d == 0) store_lse(it, r, a, sum);
-      }
     }
-    __syncthreads();  // merge and the sums are free
-    t = end;
-  }
-
-  // The CTA's partials are out (at most that of its first and that of its last item). Only now it says so, so that
-  // no item of its own waited for a join: the last of an item's CTAs to say so adds the partials up.
-  if (open[0] >= 0 || open[1] >= 0) {
-    auto owner = [&](int x) {  // the CTA that has block x
-      const int big = more * (each + 1);
-      return x < big ? x / (each + 1) : more + (x - big) / each;
-    };
-    auto cover = [&](const Item& it, int& i0) {  // the CTAs that hold a partial: i0 and the parts - 1 after it
-      if (by_round) {
-        const int rounds = (it.blocks + W - 1) / W;
-        i0 = it.s.rounds + (it.h * p.chunks + it.row0 / kRows) * rounds;
-        return rounds;
-      }
-      i0 = owner(it.start);
-      return owner(it.start + it.blocks - 1) - i0 + 1;
-    };
-    if (tid == 0) {
-      __threadfence();  // with the barrier above: every thread's partials, before the counts
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        s_last[k] = 0;
-        if (open[k] < 0) continue;
-        const Item it = item_at(open[k], first_b);
-        int i0;
-        const int parts = cover(it, i0);
-        unsigned* word = p.sync + ((size_t)it.b * p.c.heads + it.h) * p.chunks + it.row0 / kRows;
-        if (atomicAdd(word, 1u) == (unsigned)parts - 1) {
-          *word = 0;
-          s_last[k] = 1;
-        }
-      }
-      __threadfence();
-    }
-    __syncthreads();
+    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * part_ld;
 #pragma unroll 1
-    for (int k = 0; k < 2; ++k) {
-      if (!s_last[k]) continue;
-      const Item it = item_at(open[k], first_b);
-      int i0;
-      const int parts = cover(it, i0);
-      // CTA i0's partial is its slot 1 where it had another item before this one
-      const size_t skip0 = !by_round && share(i0) < it.start ? part_ld : 0;
-      const float* p0 = p.part + 2 * (size_t)i0 * part_ld;
-      // `teams` groups of threads take every teams-th part each, eight loads in flight
-      const int n4 = it.nrow * (D / 4), teams = max(1, min((parts + 3) / 4, NTHREADS / n4));
+    for (bool again = false;; again = true) {  // again: the thread groups' sums of a join
       const int team = teams == 1 ? 0 : tid / n4;
-      float2* team_ms = reinterpret_cast<float2*>(merge + NTHREADS * 4);
 #pragma unroll 1
-      for (int i = teams == 1 ? tid : tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
+      for (int i = tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
+        const float* x = src + (again ? i * 4 : r * D + d);
+        const float2* y = ms + (again ? i : r);
         float a = kNoMax, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-        for (int k0 = team; k0 < parts; k0 += 8 * teams) {
-          float2 ms[8];
-          float4 y[8];
-          float top = a;
+        for (int k0 = team; k0 < parts; k0 += 4 * teams) {
+          float2 z[4];
+          float4 w[4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int x = k0 + j * teams;
-            const float* at = p0 + 2 * (size_t)x * part_ld + (x == 0 ? skip0 : 0);
-            ms[j] = x < parts ? __ldcg(reinterpret_cast<const float2*>(at + p.nr * D + 2 * r)) : make_float2(kNoMax, 0.f);
-            y[j] = x < parts ? __ldcg(reinterpret_cast<const float4*>(at + r * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < 4; ++j) {
+            const int k = k0 + j * teams;
+            const size_t off = k ? 0 : skip0;
+            z[j] = make_float2(kNoMax, 0.f);
+            w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < parts) {
+              z[j] = y[k * ms_ld + off / 2];
+              w[j] = *reinterpret_cast<const float4*>(x + k * src_ld + off);
+            }
           }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = fmaxf(top, ms[j].x);
+          const float top = fmaxf(fmaxf(fmaxf(z[0].x, z[1].x), fmaxf(z[2].x, z[3].x)), a);
           float f = ex2(a - top);
           a = top;
           sum *= f;
           v.x *= f; v.y *= f; v.z *= f; v.w *= f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            f = ex2(ms[j].x - top);
-            sum += ms[j].y * f;
-            v.x += y[j].x * f; v.y += y[j].y * f; v.z += y[j].z * f; v.w += y[j].w * f;
+          for (int j = 0; j < 4; ++j) {
+            f = ex2(z[j].x - top);
+            sum += z[j].y * f;
+            v.x += w[j].x * f; v.y += w[j].y * f; v.z += w[j].z * f; v.w += w[j].w * f;
           }
         }
-        if (teams == 1) {
-          store(it, r, d, v, sum);
-          if (d == 0) store_lse(it, r, a, sum);
-        } else {
+        if (teams > 1) {
           *reinterpret_cast<float4*>(merge + tid * 4) = v;
-          team_ms[tid] = make_float2(a, sum);
+          s_team[tid] = make_float2(a, sum);
+        } else if (split) {
+          *reinterpret_cast<float4*>(part + r * D + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(part + p.nr * D + 2 * r) = make_float2(a, sum);
+        } else {
+          // v / sum as bf16; zeros for rows that see nothing
+          const int row = row0 + r, tok = token_of(p, row);
+          const float g = sum == 0.f || tok >= s.count ? 0.f : __fdividef(1.f, sum);
+          if (g == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+          *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * p.group + row - tok * p.group) * p.o_sh +
+                                    tok * p.o_st + d) = make_uint2(pack_bf16(v.x * g, v.y * g), pack_bf16(v.z * g, v.w * g));
+          if (p.lse && d == 0) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row] = a + log2f(sum);
         }
       }
-      if (teams > 1) {
-        __syncthreads();
-        if (tid < n4) {
-          float a = kNoMax, sum = 0.f;
-          for (int x = 0; x < teams; ++x) a = fmaxf(a, team_ms[x * n4 + tid].x);
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int x = 0; x < teams; ++x) {
-            const float4 y = *reinterpret_cast<const float4*>(merge + (x * n4 + tid) * 4);
-            const float2 ms = team_ms[x * n4 + tid];
-            const float f = ex2(ms.x - a);
-            sum += ms.y * f;
-            v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
-          }
-          store(it, tid / (D / 4), tid % (D / 4) * 4, v, sum);
-          if (tid % (D / 4) == 0) store_lse(it, tid / (D / 4), a, sum);
-        }
-        __syncthreads();
-      }
+      if (teams == 1) break;
+      __syncthreads();
+      src = merge;
+      src_ld = n4 * 4;
+      ms = s_team;
+      ms_ld = n4;
+      skip0 = 0;
+      parts = teams;
+      teams = 1;
     }
+    __syncthreads();  // the merge area is free
+    if (!join) t = end;
   }
   if (dead) {  // see this warp's copies in flight through, again with a limit, before leaving
     for (int i = 0; lane == 0 && i < waiting; ++i) {
@@ -878,6 +861,26 @@ int tile_map(CUtensorMap* map, void* base, const tbf16_paged_cache* c, int64_t s
   return tbf16_host::make_tmap_pages(map, base, item, c->D, span, c->page_size, c->heads, c->pages, ss, sh, sp, box);
 }
 
+// A launch that may be set up while the kernel before it in the stream ends (the kernels wait for it themselves).
+template <class... Params, class... Args>
+int launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return TBF16_ERR_LAUNCH;
+  }
+  return TBF16_OK;
+}
+
 constexpr int kSmemMax = 227 * 1024;
 
 template <class C>
@@ -885,7 +888,7 @@ int attend_smem(const AttendParams& p, int stages) {
   return C::W * stages * (2 * C::KB + C::SC) + p.merge * 4 + (p.c.batch + 1) * (int)sizeof(SeqInfo);
 }
 // Static shared memory of the kernel, rounded up.
-constexpr int kSmemStatic = 3 * 1024;
+constexpr int kSmemStatic = 4 * 1024;
 
 template <class C>
 int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
@@ -895,7 +898,7 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   while ((1 << p.box_shift) < box) ++p.box_shift;
   if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss, box)) return s;
   if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss, box)) return s;
-  p.merge = std::max(C::W * p.nr * C::D, C::W * 32 * 6);  // the warps' outputs, or a join's thread groups' sums
+  p.merge = std::max(C::W * p.nr * C::D, C::W * 32 * 4);  // the warps' outputs, or a join's thread groups' sums
   p.stages = kMaxStages;
   while (p.stages > 1 && attend_smem<C>(p, p.stages) + kSmemStatic > kSmemMax) --p.stages;
   const int smem = attend_smem<C>(p, p.stages);
@@ -903,8 +906,7 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   static const cudaError_t attr =
       cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic);
   if (attr != cudaSuccess) return TBF16_ERR_LAUNCH;
-  attend_kernel<C><<<sms, C::W * 32, smem, st>>>(km, vm, p);
-  return tbf16_host::check_launch();
+  return launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, st, km, vm, p);
 }
 
 struct Workspace {
@@ -987,16 +989,6 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   if (rc != TBF16_OK || !weights) return rc;
   const int block_keys = cache->D * (e4m3 ? 1 : 2) <= 64 ? 64 : cache->D * (e4m3 ? 1 : 2) <= 128 ? 32 : 16;
   const int64_t blocks = cache->batch * cache->heads * ((p.c.cap + 1023) / 1024);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, weights_kernel, p, weights, w_sb, w_sh, block_keys) != cudaSuccess)
-    return TBF16_ERR_LAUNCH;
-  return tbf16_host::check_launch();
+  return launch_pdl(weights_kernel, (unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8), 256, 0, st, p, weights, w_sb,
+                    w_sh, block_keys);
 }

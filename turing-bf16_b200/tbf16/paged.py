@@ -18,11 +18,10 @@ decoding step can be captured in a CUDA graph and replayed after `advance`. No h
 The reference has no counterpart: it leaves calls with few query rows to torch (tbf16/convert.py there).
 """
 import ctypes
-import math
 
 import torch
 
-from ._ext import BF16, E4M3, PagedCacheStruct, call, lib, require_cuda
+from ._ext import BF16, E4M3, PagedCacheStruct, check, lib, require_cuda
 
 KERNEL_D = (64, 128, 256)  # row lengths of the cache; other head dims are zero-padded up
 MAX_BATCH = 1024
@@ -56,7 +55,7 @@ def _rows(x, name, B, H, d, device):
 class _Layer:
     """One layer's buffers and their description for the library."""
 
-    def __init__(self, k, v, k_scale, v_scale, table, lens, weights, pos):
+    def __init__(self, k, v, k_scale, v_scale, table, lens, weights, pos, seen):
         self.k, self.v, self.k_scale, self.v_scale, self.weights, self.pos = k, v, k_scale, v_scale, weights, pos
         pages, heads, page_size, D = k.shape
         c = self.struct = PagedCacheStruct()
@@ -69,7 +68,9 @@ class _Layer:
             c.vs_sp, c.vs_sh = v_scale.stride()[:2]
         c.table_ld, c.batch, c.max_pages = table.stride(0), table.shape[0], table.shape[1]
         c.heads, c.D, c.page_size, c.pages, c.dtype = heads, D, page_size, pages, _DTYPES[k.dtype]
-        self.ref = ctypes.addressof(c)
+        self.ref, self.D = ctypes.addressof(c), D
+        self.weight_args = (None, 0, 0) if weights is None else (weights.data_ptr(), *weights.stride()[:2])
+        self.pos_args = (None, 0, 0, None) if pos is None else (pos.data_ptr(), *pos.stride()[:2], seen.data_ptr())
 
 
 class PagePool:
@@ -196,9 +197,9 @@ class PagedCache:
         self.head_dim, self.dtype, self.table, self.lens, self.seen = head_dim, k.dtype, table, lens, seen
         self.k, self.v, self.k_scale, self.v_scale, self.weights, self.pos = k, v, k_scale, v_scale, weights, pos
         pick = lambda x, i: None if x is None else x[i]  # noqa: E731
-        self._layers = [_Layer(k[i], v[i], pick(k_scale, i), pick(v_scale, i), table, lens, pick(weights, i), pick(pos, i))
+        self._layers = [_Layer(k[i], v[i], pick(k_scale, i), pick(v_scale, i), table, lens, pick(weights, i), pick(pos, i), seen)
                         for i in range(L)]
-        self._sizes, self._sync = {}, {}
+        self._sizes, self._buffers, self._lib = {}, {}, lib()
 
     # ------------------------------------------------------------------------------------------- host side
 
@@ -236,21 +237,35 @@ class PagedCache:
             self.table.copy_(torch.tensor(self.pool.rows(self.table.shape[1]), **ints))
 
     def _counts(self, counts):
-        if counts is not None and (not isinstance(counts, torch.Tensor) or counts.dtype != torch.int32
-                                   or counts.device != self.device or counts.shape != self.lens.shape
-                                   or not counts.is_contiguous()):
+        if counts is None:
+            return None
+        if (not isinstance(counts, torch.Tensor) or counts.dtype is not torch.int32 or counts.device != self.device
+                or counts.dim() != 1 or counts.numel() != self.batch or not counts.is_contiguous()):
             raise RuntimeError(f"tbf16.PagedCache: counts must be a contiguous int32 ({self.batch},) tensor on {self.device}")
-        return None if counts is None else counts.data_ptr()
+        return counts.data_ptr()
 
-    def _stream(self):
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
-
-    def _call(self, name, *args):
-        if torch.cuda.current_device() == self.device.index:
-            call(name, *args)
+    def _run(self, fn, what, *args):
+        """One library call on the cache's device."""
+        if torch._C._cuda_getDevice() == self.device.index:
+            status = fn(*args)
         else:
             with torch.cuda.device(self.device):
-                call(name, *args)
+                status = fn(*args)
+        if status:
+            check(status, what)
+
+    def _scratch(self, stream, sync, size):
+        """Device memory for one attend call: `sync` zeroed bytes, which the call leaves zero, then its workspace.
+        One buffer for each stream, reused by the stream's next call. A captured call gets its own, zeroed in the
+        graph, so that graphs share nothing with each other or with calls outside."""
+        buf = None if torch._C._cuda_isCurrentStreamCapturing() else self._buffers.get(stream)
+        if buf is None or buf.sync < sync or buf.numel() - buf.sync < size:
+            buf = torch.empty(sync + size, device=self.device, dtype=torch.uint8)
+            buf[:sync].zero_()
+            buf.sync = sync  # its workspace starts there, also for calls that need less
+            if not torch._C._cuda_isCurrentStreamCapturing():
+                self._buffers[stream] = buf
+        return buf
 
     # ------------------------------------------------------------------------------------------- operators
 
@@ -263,11 +278,11 @@ class PagedCache:
         v = _rows(v, "v", self.batch, self.kv_heads, self.head_dim, self.device)
         if k.shape != v.shape:
             raise RuntimeError(f"tbf16.PagedCache.append: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-        pos = c.pos
-        self._call("tbf16_paged_append", c.ref, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], k.shape[2],
-                   k.shape[3], self._counts(counts), pos.data_ptr() if pos is not None else None,
-                   *(pos.stride()[:2] if pos is not None else (0, 0)),
-                   self.seen.data_ptr() if pos is not None else None, self._stream())
+        _, _, T, d = k.shape
+        kb, kh, kt, _ = k.stride()
+        vb, vh, vt, _ = v.stride()
+        self._run(self._lib.tbf16_paged_append, "append", c.ref, k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T, d,
+                  self._counts(counts), *c.pos_args, torch._C._cuda_getCurrentRawStream(self.device.index))
 
     def attend(self, q, layer=0, counts=None, scale=None, window=0):
         """Attention of the newest T tokens over the cache: q bf16 (B, heads, T, head_dim), heads a multiple of
@@ -278,41 +293,29 @@ class PagedCache:
         c, d = self._layers[layer], self.head_dim
         q = _rows(q, "q", self.batch, 0, d, self.device)
         B, Hq, T, dq = q.shape
-        D = c.k.shape[3]
-        if Hq % self.kv_heads or Hq == 0:
-            raise RuntimeError(f"tbf16.PagedCache.attend: {Hq} query heads over {self.kv_heads} key/value heads")
+        D = c.D
         if window < 0:
             raise RuntimeError("tbf16.PagedCache.attend: window must not be negative")
         if dq != D:  # zero columns leave the logits unchanged and give zero output columns
             q = torch.nn.functional.pad(q, (0, D - dq))
-        out = torch.empty((B, T, Hq, D), device=self.device, dtype=torch.bfloat16)
-        w = c.weights
         sizes = self._sizes.get((Hq, T))
         if sizes is None:
-            L = lib()
-            sizes = self._sizes[(Hq, T)] = (int(L.tbf16_paged_attend_ws_size(c.ref, Hq, T, int(w is not None))),
-                                            int(L.tbf16_paged_attend_sync_size(c.ref, Hq, T)))
-        ws = torch.empty(sizes[0], device=self.device, dtype=torch.uint8)
-        stream = self._stream()
-        sync = self._sync_words(stream, sizes[1])
+            if Hq == 0 or Hq % self.kv_heads:
+                raise RuntimeError(f"tbf16.PagedCache.attend: {Hq} query heads over {self.kv_heads} key/value heads")
+            n = int(self._lib.tbf16_paged_attend_sync_size(c.ref, Hq, T))
+            sizes = self._sizes[(Hq, T)] = ((n + 255) // 256 * 256,
+                                            int(self._lib.tbf16_paged_attend_ws_size(c.ref, Hq, T, int(c.weights is not None))))
+        sync, size = sizes
+        row = Hq * D
+        out = torch.empty_strided((B, Hq, T, D), (T * row, D, row, 1), device=self.device, dtype=torch.bfloat16)
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        buf = self._scratch(stream, sync, size)
+        ptr = buf.data_ptr()
         sb, sh, st, _ = q.stride()
-        wsb, wsh = w.stride()[:2] if w is not None else (0, 0)
-        self._call("tbf16_paged_attend", c.ref, q.data_ptr(), sb, sh, st, Hq, T, self._counts(counts),
-                   1.0 / math.sqrt(d) if scale is None else float(scale), int(window), out.data_ptr(), T * Hq * D, D,
-                   Hq * D, w.data_ptr() if w is not None else None, wsb, wsh, sync.data_ptr(), ws.data_ptr(), sizes[0],
-                   stream)
-        out = out.transpose(1, 2)
+        self._run(self._lib.tbf16_paged_attend, "attend", c.ref, q.data_ptr(), sb, sh, st, Hq, T, self._counts(counts),
+                  d ** -0.5 if scale is None else float(scale), int(window), out.data_ptr(), T * row, D, row, *c.weight_args, ptr,
+                  ptr + buf.sync, size, stream)
         return out[..., :d] if d != D else out
-
-    def _sync_words(self, stream, size):
-        """Zeroed words for the library's split bookkeeping, which it leaves zero: one buffer for each stream, so
-        that calls on different streams do not share one. A captured call gets its own, zeroed in the graph."""
-        if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(size, device=self.device, dtype=torch.uint8)
-        sync = self._sync.get(stream)
-        if sync is None or sync.numel() < size:
-            sync = self._sync[stream] = torch.zeros(size, device=self.device, dtype=torch.uint8)
-        return sync
 
     def compact(self, keep, recent=0, layer=0):
         """Cuts one layer's sequences to their `keep` heaviest positions per head, the newest `recent` tokens
@@ -327,11 +330,11 @@ class PagedCache:
         cols = c.weights.shape[2]
         weights = torch.empty(c.weights.shape, device=self.device)
         pos = torch.empty(c.pos.shape, device=self.device, dtype=torch.int32)
-        n = int(lib().tbf16_paged_compact_ws_size(c.ref, cols, keep))
+        n = int(self._lib.tbf16_paged_compact_ws_size(c.ref, cols, keep))
         ws = torch.empty(n, device=self.device, dtype=torch.uint8)
-        self._call("tbf16_paged_compact", c.ref, c.weights.data_ptr(), *c.weights.stride()[:2], c.pos.data_ptr(),
-                   *c.pos.stride()[:2], cols, self.seen.data_ptr(), int(keep), int(recent),
-                   weights.data_ptr(), pos.data_ptr(), ws.data_ptr(), n, self._stream())
+        self._run(self._lib.tbf16_paged_compact, "compact", c.ref, *c.weight_args, *c.pos_args[:3], cols, c.pos_args[3], keep,
+                  recent, weights.data_ptr(), pos.data_ptr(), ws.data_ptr(), n,
+                  torch._C._cuda_getCurrentRawStream(self.device.index))
         return weights, pos
 
     def evict(self, keep, recent=0):
