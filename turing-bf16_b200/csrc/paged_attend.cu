@@ -10,27 +10,31 @@ using namespace tbf16;
 
 // For a query row r of a key/value head (T new tokens x the head's group of query heads)
 //   s_j = (q_r . k_j) scale,  out_r = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  m = max_j s_j
-// over the visible positions j. Every cached byte is used by 2 T group flops per element, 2..64 in practice
-// against the ~260 per byte the tensor cores could do: the time is the cache's bytes over the HBM rate, as long
-// as enough bytes are in flight on every SM, however few or uneven the sequences.
+// over the visible positions j. Every cached element is used by 2 T group flops, 2..64 in practice, where the
+// tensor cores could do hundreds: the time is the cache's bytes over the HBM rate, as long as enough bytes are in
+// flight on every SM, however few or uneven the sequences, and no warp computes longer than its bytes take.
 //
-// Work split. The keys of a (sequence, head, 16 query rows) item are cut into blocks of BK keys; the blocks of
-// all items, laid end to end, are shared out evenly over the CTAs (one per SM), from the lengths on the device:
+// Work split. The keys of a (sequence, head, query rows) item are cut into blocks of BK keys; the blocks of all
+// items, laid end to end, are shared out evenly over the CTAs (one per SM), from the lengths on the device:
 // ragged batches and one long sequence keep all SMs equally busy, and a captured graph follows the lengths. A
 // CTA's blocks go round-robin to its warps. Each warp is a pipeline of its own: it issues the TMA loads of its
 // blocks into its own ring of stages, waits for them, and keeps its own running maximum, sum and output in
-// registers (mma.sync m16n8k16: with 16 query rows a tile, tcgen05's 128-row tile would be seven eighths empty,
-// and the tensor work is far from the bound), so the warps never wait for one another inside an item. At its
-// end they are added up through shared memory. An item that spans CTAs leaves one partial (output, maximum,
-// sum) per CTA in the workspace; the CTA that arrives last adds them in a fixed order, so results do not depend
-// on which one that is.
-constexpr int kRows = 16;      // query rows of an item: one m16n8k16 tile
+// registers, so the warps never wait for one another inside an item. At its end they are added up through shared
+// memory. An item that spans CTAs leaves one partial (output, maximum, sum) per CTA in the workspace; the CTA
+// that arrives last adds them in a fixed order, so results do not depend on which one that is.
+//
+// Tiles. mma.sync m16n8k16 with the cache as the 16-row operand and eight query rows as columns: S^T = K Q^T,
+// O^T = V^T P^T. With the usual group of up to eight query rows no product is wasted on empty rows (a 16-row
+// query tile would waste half of them, tcgen05's 128 rows fifteen sixteenths), a lane holds four weights per 16
+// keys, and P^T gets from accumulator to operand layout by one 8x8 transpose per 8 keys.
 constexpr int kMaxStages = 8;
 
-template <int D_, bool E4M3_>
+template <int D_, bool E4M3_, int NQ_>
 struct Tile {
   static constexpr int D = D_;
   static constexpr bool E4M3 = E4M3_;
+  static constexpr int NQ = NQ_;                             // column tiles of eight query rows
+  static constexpr int R = 8 * NQ;                           // query rows of an item
   static constexpr int RB = D * (E4M3 ? 1 : 2);              // bytes of a cached row
   static constexpr int AW = RB < 128 ? RB : 128;             // swizzle span: 64 or 128 bytes
   static constexpr int BK = RB <= 64 ? 64 : RB <= 128 ? 32 : 16;  // keys of a block
@@ -39,6 +43,7 @@ struct Tile {
   static constexpr int KB = NG * GB;                         // bytes of a block's keys (or values)
   static constexpr int W = RB == 512 ? 4 : 8;                // warps
   static constexpr int SC = E4M3 ? 2 * BK * 4 : 0;           // bytes of a block's scales
+  static constexpr int MP = D + 4;                           // floats between rows of the merge area (no bank twice)
 };
 
 struct AttendParams {
@@ -48,18 +53,21 @@ struct AttendParams {
   __nv_bfloat16* out;
   int64_t o_sb, o_sh, o_st;
   const int* counts;
-  int T, group, rows, chunks, window;  // rows = T * group query rows of a head, in chunks of kRows
+  int T, group, rows, chunks, window;  // rows = T * group query rows of a head, in chunks of R
   unsigned group_inv;                  // ceil(2^32 / group): row / group = umulhi(row, group_inv) below 2^16
   float scale_log2;
   int stages;
   int box_shift;    // log2 of the keys that one TMA load brings: min(BK, page size); rows of one span when over 16
-  int nr;           // rows of an item that can be real: min(rows, kRows)
+  int nr;           // rows of an item that can be real: min(rows, R)
   int merge;        // floats of the merge area
   unsigned* sync;   // arrivals of each item, zero between calls
-  float* part;      // [2 * CTAs][nr * D + 2 * kRows]: partial outputs, (maximum, sum) pairs
+  float* part;      // [2 * CTAs][partial_floats(nr, D)]: partial outputs, (maximum, sum) pairs
   float* logits;    // weights wanted: [batch * heads][rows][cap], base-2 logits
   float* lse;       // and [batch * heads][rows]: log2 of each row's sum
 };
+
+// Floats of a partial: nr rows of outputs, then of (maximum, sum) pairs, to a multiple of 16 bytes.
+__host__ __device__ constexpr int partial_floats(int nr, int D) { return (nr * (D + 2) + 3) / 4 * 4; }
 
 // What a CTA knows of a sequence: the first of its blocks, and of its rounds, among all; cached and new tokens.
 struct SeqInfo {
@@ -134,13 +142,22 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* m, uin
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// Over the eight lanes that hold one column of an accumulator.
+__device__ __forceinline__ float column_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float column_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The transpose of an 8x8 matrix of 16-bit values held two to a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 // Byte offset of 16-byte chunk `chunk` of key `row` inside a group, as TMA's swizzle places it.
@@ -237,7 +254,7 @@ constexpr int kWeightShift = 7;
 template <class C>
 __global__ void __launch_bounds__(C::W * 32, 1)
     attend_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm, const AttendParams p) {
-  constexpr int D = C::D, NT = D / 8, W = C::W, NG = C::NG, KS = D / 16, NTHREADS = W * 32;
+  constexpr int D = C::D, W = C::W, NQ = C::NQ, R = C::R, NG = C::NG, KS = D / 16, NTHREADS = W * 32, MP = C::MP;
   constexpr bool E4M3 = C::E4M3;
   using L = Loader<C>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -246,7 +263,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   float* merge = scale_ring + (size_t)W * p.stages * (C::SC / 4);
   SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + p.merge);
   __shared__ uint64_t bars[W * kMaxStages];
-  __shared__ float2 s_ms[W * kRows];   // each warp's (maximum, sum) of a row
+  __shared__ float2 s_ms[W * R];       // each warp's (maximum, sum) of a row
   __shared__ float2 s_team[NTHREADS];  // that of a row in each thread group of a join
   __shared__ int s_scan[W], s_work[W], s_abort, s_todo;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -342,9 +359,9 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   bool dead = false;  // a wait gave up: nothing more is loaded or computed, every barrier is still reached
 
   const int g4 = lane >> 2, c4 = lane & 3;
-  // this lane's addresses in the ldmatrix of keys and of values, for chunk pair 0 of a group
-  const uint32_t k_lane = E4M3 ? chunk_at<C>(lane & 15, lane >> 4) : chunk_at<C>(((lane >> 4) & 1) * 8 + (lane & 7), (lane >> 3) & 1);
-  const uint32_t v_lane = chunk_at<C>(lane & 15, lane >> 4);
+  // this lane's addresses in the ldmatrix of keys and of values, for the first chunks of a group
+  const uint32_t k_lane = chunk_at<C>(lane & 15, lane >> 4);
+  const uint32_t v_lane = E4M3 ? k_lane : chunk_at<C>(((lane >> 4) & 1) * 8 + (lane & 7), (lane >> 3) & 1);
 
   // The item that holds block t.
   struct Item {
@@ -360,11 +377,11 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     const int i = (int)((unsigned)(t - it.s.cum) / (unsigned)it.blocks);
     it.start = it.s.cum + i * it.blocks;
     it.h = p.chunks == 1 ? i : i / p.chunks;
-    it.row0 = (i - it.h * p.chunks) * kRows;
-    it.nrow = min(kRows, p.rows - it.row0);
+    it.row0 = (i - it.h * p.chunks) * R;
+    it.nrow = min(R, p.rows - it.row0);
     return it;
   };
-  const size_t part_ld = p.nr * D + 2 * kRows;
+  const size_t part_ld = partial_floats(p.nr, D);
   auto owner = [&](int x) {  // the CTA that has block x
     const int big = more * (each + 1);
     return x < big ? x / (each + 1) : more + (x - big) / each;
@@ -404,7 +421,8 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     // the partials to add up: part k's outputs from src + k src_ld, its (maximum, sum) pairs from ms + k ms_ld
     const float* src = merge;
     const float2* ms = s_ms;
-    size_t src_ld = p.nr * D, ms_ld = kRows, skip0 = 0;  // skip0: part 0 lies that much further on
+    size_t src_ld = p.nr * MP, ms_ld = R, skip0 = 0;  // skip0: part 0 lies that much further on
+    int pitch = MP;                                   // floats between a part's rows
     int parts = W, teams = 1;
     bool split = false;
     if (join) {
@@ -416,6 +434,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       src_ld = 2 * part_ld;
       ms = reinterpret_cast<const float2*>(src + p.nr * D);
       ms_ld = part_ld;
+      pitch = D;
       if (!by_round && share(i0) < start) skip0 = part_ld;  // that CTA had another item before this one
       // groups of threads share the parts out
       teams = max(1, min((parts + 3) / 4, NTHREADS / n4));
@@ -425,58 +444,66 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       int i0, n;
       if (by_round) {
         n = (it.blocks + W - 1) / W;
-        i0 = s.rounds + (h * p.chunks + row0 / kRows) * n;
+        i0 = s.rounds + (h * p.chunks + row0 / R) * n;
       } else {
         i0 = owner(start);
         n = owner(start + it.blocks - 1) - i0 + 1;
       }
-      const int word = (b * p.c.heads + h) * p.chunks + row0 / kRows;
+      const int word = (b * p.c.heads + h) * p.chunks + row0 / R;
       if (t == c0) open0 = t, at0 = i0, parts0 = n, word0 = word;
       else open1 = t, at1 = i0, parts1 = n, word1 = word;
     }
     const int lo = first_block<C>(p, s.len, s.count);
-    // query rows g4 and g4 + 8 of the item: their A fragments and positions
-    uint32_t qf[KS][4];
-    float mul[2];
-    int at[2];  // position of the row's token; -1: the row is not there
+    // B fragments of the item's query rows (a lane loads row g4 of each tile), and what this lane has to know of
+    // the rows in its accumulator columns, 2 c4 and 2 c4 + 1 of each tile
+    uint32_t qf[NQ][KS][2];
+    float mul[NQ][2];
+    int at[NQ][2];  // position of the row's token; -1: the row is not there
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = row0 + g4 + i * 8, tok = token_of(p, r);
+    for (int q = 0; q < NQ; ++q) {
+      const int r = row0 + q * 8 + g4, tok = token_of(p, r);
       const bool there = r < p.rows && tok < s.count;
-      at[i] = there ? s.len - s.count + tok : -1;
-      const __nv_bfloat16* q = p.q + b * p.q_sb + (int64_t)(h * p.group + r - tok * p.group) * p.q_sh + tok * p.q_st;
-      mul[i] = p.scale_log2;
+      const __nv_bfloat16* x = p.q + b * p.q_sb + (int64_t)(h * p.group + r - tok * p.group) * p.q_sh + tok * p.q_st;
       if (E4M3) {
         // fp16 rows: the largest magnitude to [2^14, 2^15) by a power of two, undone in the logits' factor. In
         // column 16 k + 4 c of a k16 step sit the two pairs the byte order of a cached row puts there.
-        uint2 x[KS];
+        uint2 y[KS];
         unsigned m = 0;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) x[k] = there ? *reinterpret_cast<const uint2*>(q + k * 16 + c4 * 4) : make_uint2(0, 0);
+        for (int k = 0; k < KS; ++k) y[k] = there ? *reinterpret_cast<const uint2*>(x + k * 16 + c4 * 4) : make_uint2(0, 0);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          m = max(m, max(max((x[k].x << 16) & 0x7fffffffu, x[k].x & 0x7fff0000u),
-                         max((x[k].y << 16) & 0x7fffffffu, x[k].y & 0x7fff0000u)));
+          m = max(m, max(max((y[k].x << 16) & 0x7fffffffu, y[k].x & 0x7fff0000u),
+                         max((y[k].y << 16) & 0x7fffffffu, y[k].y & 0x7fff0000u)));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const int e = m == 0 || m >= 0x7f800000u ? 15 : max(frexp_exp(__uint_as_float(m)), -110);
-        const float f = exp2i(15 - e);
-        mul[i] *= exp2i(e - 15);
+        const float f = exp2i(15 - e), undo = p.scale_log2 * exp2i(e - 15);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          qf[k][i] = pack_f16(bf16lo(x[k].x) * f, bf16hi(x[k].x) * f);
-          qf[k][2 + i] = pack_f16(bf16lo(x[k].y) * f, bf16hi(x[k].y) * f);
+          qf[q][k][0] = pack_f16(bf16lo(y[k].x) * f, bf16hi(y[k].x) * f);
+          qf[q][k][1] = pack_f16(bf16lo(y[k].y) * f, bf16hi(y[k].y) * f);
         }
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) mul[q][e2] = __shfl_sync(0xffffffffu, undo, (2 * c4 + e2) * 4);
       } else {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          qf[k][i] = there ? *reinterpret_cast<const uint32_t*>(q + k * 16 + c4 * 2) : 0u;
-          qf[k][2 + i] = there ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + c4 * 2) : 0u;
+          qf[q][k][0] = there ? *reinterpret_cast<const uint32_t*>(x + k * 16 + c4 * 2) : 0u;
+          qf[q][k][1] = there ? *reinterpret_cast<const uint32_t*>(x + k * 16 + 8 + c4 * 2) : 0u;
         }
+        mul[q][0] = mul[q][1] = p.scale_log2;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r2 = row0 + q * 8 + 2 * c4 + e, tok2 = token_of(p, r2);
+        at[q][e] = r2 < p.rows && tok2 < s.count ? s.len - s.count + tok2 : -1;
       }
     }
-    float o[NT][4] = {};
-    float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+    float o[NQ][KS][4] = {};  // O^T: 16 columns of the values x 8 query rows a tile
+    float m[NQ][2], l[NQ][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) m[q][0] = m[q][1] = kNoMax, l[q][0] = l[q][1] = 0.f;
     float vtop = 0.f, vmul = 0.f;  // e4m3: bound of the value scales met so far, and 2^kWeightShift over it
     const int pos_min = s.len - s.count, pos_max = s.len - 1;
 
@@ -490,15 +517,16 @@ __global__ void __launch_bounds__(C::W * 32, 1)
         break;
       }
       const uint32_t kb = smem_u32(my_ring) + stage * (2 * C::KB);
-      const float* ksc = my_scales + stage * (C::SC / 4) + c4 * 2;
+      const float* ksc = my_scales + stage * (C::SC / 4) + g4;
       const int j0 = (lo + x - start) * C::BK;
       const int groups = min(NG, (s.len - j0 + 15) >> 4);
 #pragma unroll 1
       for (int g = 0; g < groups; ++g) {
-        // products of 16 query rows x 16 keys; two accumulators a tile shorten the chain of dependent products
+        // S^T of 16 keys (rows g4, g4 + 8) x the query rows; for a single tile two accumulators shorten the chain of
+        // dependent products. Fragments come in batches of four loads, so that a load's latency is met per batch.
         const uint32_t ka = kb + g * C::GB + k_lane;
-        float sc[2][4], sd[2][4];
-        // fragments come in batches of four loads, so that one load's latency is met per batch
+        constexpr int CH = NQ == 1 ? 2 : 1;
+        float acc[NQ * CH][4];
         constexpr int KI = E4M3 ? KS / 2 : KS, KB4 = KI < 4 ? KI : 4;
 #pragma unroll
         for (int k0 = 0; k0 < KI; k0 += KB4) {
@@ -506,114 +534,112 @@ __global__ void __launch_bounds__(C::W * 32, 1)
 #pragma unroll
           for (int k = 0; k < KB4; ++k) ldsm4(r[k], chunk_from<C>(ka, 2 * (k0 + k)));
 #pragma unroll
-          for (int kk = 0; kk < KB4; ++kk) {
-            const int k = k0 + kk;
-            if (E4M3) {
+          for (int kk = 0; kk < KB4; ++kk)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {  // 0, 1: keys 0-7 and 8-15 of chunk 2 k; 2, 3: of chunk 2 k + 1
-                float(&d)[4] = i < 2 ? sc[i] : sd[i - 2];
-                uint32_t b0, b1;
-                e4m3_f16(r[kk][i], b0, b1);
-                if (k == 0) mma16_first<true>(d, qf[i >> 1], b0, b1);
-                else mma16<true>(d, qf[2 * k + (i >> 1)], b0, b1);
-              }
-            } else {
-              float(&d0)[4] = k & 1 ? sd[0] : sc[0];
-              float(&d1)[4] = k & 1 ? sd[1] : sc[1];
-              if (k < 2) {
-                mma16_first<false>(d0, qf[k], r[kk][0], r[kk][1]);
-                mma16_first<false>(d1, qf[k], r[kk][2], r[kk][3]);
+            for (int half = 0; half < (E4M3 ? 2 : 1); ++half) {
+              // bf16: a register is eight keys' chunk half; e4m3: eight keys' chunk, two k16 steps in the four
+              const int k = E4M3 ? 2 * (k0 + kk) + half : k0 + kk;
+              uint32_t a[4];
+              if (E4M3) {
+                e4m3_f16(r[kk][2 * half], a[0], a[2]);
+                e4m3_f16(r[kk][2 * half + 1], a[1], a[3]);
               } else {
-                mma16<false>(d0, qf[k], r[kk][0], r[kk][1]);
-                mma16<false>(d1, qf[k], r[kk][2], r[kk][3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = r[kk][i];
+              }
+#pragma unroll
+              for (int q = 0; q < NQ; ++q) {
+                float(&d)[4] = acc[q * CH + k % CH];
+                if (k < CH) mma16_first<E4M3>(d, a, qf[q][k][0], qf[q][k][1]);
+                else mma16<E4M3>(d, a, qf[q][k][0], qf[q][k][1]);
               }
             }
-          }
         }
         const int jg = j0 + g * 16;
         const bool whole = jg + 15 <= pos_min && (!p.window || jg > pos_max - p.window);
-        float vs[2][2];  // e4m3: scales of this lane's value rows
-        // logits in units of log 2
+        float ks[2] = {1.f, 1.f}, vs[2];  // e4m3: scales of this lane's two keys
+        if (E4M3) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float2 ks = make_float2(1.f, 1.f);
-          if (E4M3) {
-            ks = *reinterpret_cast<const float2*>(ksc + g * 16 + n * 8);
-            const float2 y = *reinterpret_cast<const float2*>(ksc + C::BK + g * 16 + n * 8);
-            vs[n][0] = y.x;
-            vs[n][1] = y.y;
+          for (int i = 0; i < 2; ++i) {
+            ks[i] = ksc[g * 16 + i * 8];
+            vs[i] = ksc[C::BK + g * 16 + i * 8];
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sc[n][e] = (sc[n][e] + sd[n][e]) * (E4M3 ? mul[e >> 1] * ((e & 1) ? ks.y : ks.x) : mul[e >> 1]);
         }
+        // logits in units of log 2
+        float sc[NQ][4];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = CH == 2 ? acc[q * CH][e] + acc[q * CH + CH - 1][e] : acc[q][e];
+            sc[q][e] = y * (E4M3 ? mul[q][e & 1] * ks[e >> 1] : mul[q][e & 1]);
+          }
         if (!whole) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int i = 0; i < 2; ++i) {
+            const int j = jg + g4 + i * 8;
+            // the scale of a row that nobody sees may be anything
+            if (E4M3 && (j > pos_max || (p.window && j <= pos_min - p.window))) vs[i] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = jg + n * 8 + c4 * 2 + (e & 1), i = at[e >> 1];
-              const bool see = j <= i && (!p.window || j > i - p.window);
-              if (!see) sc[n][e] = -INFINITY;
-              // the scale of a row that nobody sees may be anything
-              if (E4M3 && e < 2 && (j > pos_max || (p.window && j <= pos_min - p.window))) vs[n][e] = 0.f;
-            }
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const bool see = j <= at[q][e] && (!p.window || j > at[q][e] - p.window);
+                if (!see) sc[q][2 * i + e] = -INFINITY;
+              }
+          }
         }
         if (p.logits) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (at[i] >= 0)
-                *reinterpret_cast<float2*>(p.logits + ((int64_t)(b * p.c.heads + h) * p.rows + row0 + g4 + i * 8) * p.c.cap +
-                                           jg + n * 8 + c4 * 2) = make_float2(sc[n][2 * i], sc[n][2 * i + 1]);
+            for (int e = 0; e < 4; ++e)
+              if (at[q][e & 1] >= 0)
+                p.logits[((int64_t)(b * p.c.heads + h) * p.rows + row0 + q * 8 + 2 * c4 + (e & 1)) * p.c.cap + jg + g4 +
+                         (e >> 1) * 8] = sc[q][e];
         }
-        float top[2];
+        bool grew = false;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          top[i] = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
-        bool grew = top[0] - m[0] > kSlack || top[1] - m[1] > kSlack;
-        if (E4M3) {
-          const float y = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
-          grew |= y > vtop && y < INFINITY;
-        }
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) grew |= fmaxf(sc[q][e], sc[q][2 + e]) - m[q][e] > kSlack;
+        if (E4M3) grew |= fmaxf(vs[0], vs[1]) > vtop && fmaxf(vs[0], vs[1]) < INFINITY;
         if (__any_sync(0xffffffffu, grew)) {
-          float fac[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float was = m[i];
-            m[i] = fmaxf(was, quad_max(top[i]));
-            fac[i] = ex2(was - m[i]);
-            l[i] *= fac[i];
-          }
+          float more_room = 1.f;
           if (E4M3) {
-            float y = 0.f;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) y = fmaxf(y, vs[n][e] < INFINITY ? vs[n][e] : 0.f);
-            y = quad_max(y);
-            if (y > vtop) {  // a power of two: two bits of room, so that the next ones rarely come here
-              const float now = fmaxf(y * 4.f, 0x1p-110f), f = vtop / now;
-              fac[0] *= f;
-              fac[1] *= f;
+            const float y = column_max(fmaxf(vs[0] < INFINITY ? vs[0] : 0.f, vs[1] < INFINITY ? vs[1] : 0.f));
+            if (y > vtop) {  // two bits of room, so that the next ones rarely come here
+              const float now = fmaxf(y * 4.f, 0x1p-110f);
+              more_room = vtop / now;
               vtop = now;
               vmul = (float)(1 << kWeightShift) / now;
             }
           }
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int q = 0; q < NQ; ++q) {
+            float fac[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] *= fac[e >> 1];
+            for (int e = 0; e < 2; ++e) {
+              const float was = m[q][e];
+              m[q][e] = fmaxf(was, column_max(fmaxf(sc[q][e], sc[q][2 + e])));
+              fac[e] = ex2(was - m[q][e]);
+              l[q][e] *= fac[e];
+              fac[e] *= more_room;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[q][k][e] *= fac[e & 1];
+          }
         }
-        float pw[2][4];  // weights for the output
+        float pw[NQ][4];  // weights for the output
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float w = ex2(sc[n][e] - m[e >> 1]);
-            l[e >> 1] += w;
-            pw[n][e] = E4M3 ? w * (vs[n][e & 1] * vmul) : w;
+            const float w = ex2(sc[q][e] - m[q][e & 1]);
+            l[q][e & 1] += w;
+            pw[q][e] = E4M3 ? w * (vs[e >> 1] * vmul) : w;
           }
         const uint32_t vg = kb + C::KB + g * C::GB, va = vg + v_lane;
         bool odd = false;
@@ -633,60 +659,67 @@ __global__ void __launch_bounds__(C::W * 32, 1)
           odd = __any_sync(0xffffffffu, odd);
           if (E4M3) {  // a scale may be NaN too
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (sc[n][e] == -INFINITY) pw[n][e] = 0.f;
+                if (sc[q][e] == -INFINITY) pw[q][e] = 0.f;
           }
           if (odd) {
 #pragma unroll 1
             for (int k = 0; k < 16; ++k) {
-              const int from = (lane & ~3) | ((k & 7) >> 1), j = jg + k;
-              float w[2];
+              const int j = jg + k;
+              float w[NQ][2];
+              bool see[NQ][2];
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const float a = __shfl_sync(0xffffffffu, pw[0][2 * i], from), d = __shfl_sync(0xffffffffu, pw[0][2 * i + 1], from);
-                const float e = __shfl_sync(0xffffffffu, pw[1][2 * i], from), f = __shfl_sync(0xffffffffu, pw[1][2 * i + 1], from);
-                w[i] = k < 8 ? (k & 1 ? d : a) : (k & 1 ? f : e);
-              }
-              const bool see0 = j <= at[0] && (!p.window || j > at[0] - p.window);
-              const bool see1 = j <= at[1] && (!p.window || j > at[1] - p.window);
+              for (int q = 0; q < NQ; ++q)
 #pragma unroll
-              for (int n = 0; n < NT; n += E4M3 ? 2 : 1) {
-                uint32_t v;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(vg + chunk_at<C>(k, E4M3 ? n / 2 : n) + c4 * 4));
+                for (int e = 0; e < 2; ++e) {
+                  const float w0 = __shfl_sync(0xffffffffu, pw[q][e], (k & 7) * 4 + c4);
+                  const float w1 = __shfl_sync(0xffffffffu, pw[q][2 + e], (k & 7) * 4 + c4);
+                  w[q][e] = k < 8 ? w0 : w1;
+                  see[q][e] = j <= at[q][e] && (!p.window || j > at[q][e] - p.window);
+                }
+#pragma unroll
+              for (int n = 0; n < KS; ++n) {
+                // this lane's two output rows of tile n: bf16 columns g4 and g4 + 8, e4m3 columns 2 g4 and 2 g4 + 1
+                float y[2];
                 if (E4M3) {
+                  unsigned short v;
+                  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(vg + chunk_at<C>(k, n) + g4 * 2));
                   uint32_t lo2, hi2;
                   e4m3_f16(v, lo2, hi2);
-                  const float x4[4] = {f16lo(lo2), f16hi(lo2), f16lo(hi2), f16hi(hi2)};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    float(&t4)[4] = o[n + (e & 1)];
-                    if (see0 && !isfinite(x4[e])) t4[e >> 1] += w[0] * x4[e];
-                    if (see1 && !isfinite(x4[e])) t4[2 + (e >> 1)] += w[1] * x4[e];
-                  }
+                  y[0] = f16lo(lo2);
+                  y[1] = f16hi(lo2);
                 } else {
-                  const float x2[2] = {bf16lo(v), bf16hi(v)};
 #pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    if (see0 && !isfinite(x2[e])) o[n][e] += w[0] * x2[e];
-                    if (see1 && !isfinite(x2[e])) o[n][2 + e] += w[1] * x2[e];
+                  for (int i = 0; i < 2; ++i) {
+                    unsigned short v;
+                    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(vg + chunk_at<C>(k, 2 * n + i) + g4 * 2));
+                    y[i] = bf16lo(v);
                   }
                 }
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (see[q][e & 1] && !isfinite(y[e >> 1])) o[q][n][e] += w[q][e & 1] * y[e >> 1];
               }
             }
           }
         }
-        // weights as the products' A operand. e4m3: fp16, 11 bits, on values that are exact in fp16. bf16: in two parts
+        // P^T as the products' B operand. e4m3: fp16, 11 bits, on values that are exact in fp16. bf16: in two parts
         // (16 bits of them): one part would add its 2^-9 to the output's own rounding
-        uint32_t hi[4], lw[4];
+        uint32_t hi[NQ][2], lw[NQ][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float y = pw[i >> 1][2 * (i & 1)], z = pw[i >> 1][2 * (i & 1) + 1];
-          hi[i] = E4M3 ? pack_f16(y, z) : pack_bf16(y, z);
-          if (!E4M3) lw[i] = pack_bf16(y - bf16lo(hi[i]), z - bf16hi(hi[i]));
-        }
-        constexpr int VI = E4M3 ? KS / 2 : NT / 2, VB4 = VI < 4 ? VI : 4;
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float y = pw[q][2 * i], z = pw[q][2 * i + 1];
+            const uint32_t w = E4M3 ? pack_f16(y, z) : pack_bf16(y, z);
+            hi[q][i] = transpose8(w);
+            if (!E4M3) lw[q][i] = transpose8(pack_bf16(y - bf16lo(w), z - bf16hi(w)));
+          }
+        constexpr int VI = E4M3 ? KS / 2 : KS, VB4 = VI < 4 ? VI : 4;
 #pragma unroll
         for (int k0 = 0; k0 < VI; k0 += VB4) {
           uint32_t r[VB4][4];
@@ -697,23 +730,23 @@ __global__ void __launch_bounds__(C::W * 32, 1)
           }
 #pragma unroll
           for (int kk = 0; kk < VB4; ++kk) {
-            const int k = 2 * (k0 + kk);
             if (E4M3) {
-              // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: pair the keys, one tile for the even
-              // columns of the chunk, one for the odd ones
+              // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: paired by keys, the even columns of a
+              // chunk are the tile's rows 0-7 and the odd ones its rows 8-15
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                uint32_t even0, odd0, even1, odd1;
-                e4m3_f16(__byte_perm(r[kk][2 * i], 0, 0x3120), even0, odd0);
-                e4m3_f16(__byte_perm(r[kk][2 * i + 1], 0, 0x3120), even1, odd1);
-                mma16<true>(o[2 * (k + i)], hi, even0, even1);
-                mma16<true>(o[2 * (k + i) + 1], hi, odd0, odd1);
+                uint32_t a[4];
+                e4m3_f16(__byte_perm(r[kk][2 * i], 0, 0x3120), a[0], a[1]);
+                e4m3_f16(__byte_perm(r[kk][2 * i + 1], 0, 0x3120), a[2], a[3]);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) mma16<true>(o[q][2 * (k0 + kk) + i], a, hi[q][0], hi[q][1]);
               }
             } else {
-              mma16<false>(o[k], hi, r[kk][0], r[kk][1]);
-              mma16<false>(o[k + 1], hi, r[kk][2], r[kk][3]);
-              mma16<false>(o[k], lw, r[kk][0], r[kk][1]);
-              mma16<false>(o[k + 1], lw, r[kk][2], r[kk][3]);
+#pragma unroll
+              for (int q = 0; q < NQ; ++q) {
+                mma16<false>(o[q][k0 + kk], r[kk], hi[q][0], hi[q][1]);
+                mma16<false>(o[q][k0 + kk], r[kk], lw[q][0], lw[q][1]);
+              }
             }
           }
         }
@@ -726,25 +759,27 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     }
 
     // the warps' parts of the item
+    const float f = E4M3 ? vtop * (1.f / (1 << kWeightShift)) : 1.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] = quad_sum(l[i]);
-      if (c4 == 0) s_ms[warp * kRows + g4 + i * 8] = make_float2(m[i], l[i]);
-      if (g4 + i * 8 < p.nr) {
-        float* dst = merge + ((size_t)warp * p.nr + g4 + i * 8) * D;
-        if (E4M3) {
-          const float f = vtop * (1.f / (1 << kWeightShift));
+    for (int q = 0; q < NQ; ++q)
 #pragma unroll
-          for (int n = 0; n < NT; n += 2)
-            *reinterpret_cast<float4*>(dst + n * 8 + c4 * 4) =
-                make_float4(o[n][2 * i] * f, o[n + 1][2 * i] * f, o[n][2 * i + 1] * f, o[n + 1][2 * i + 1] * f);
-        } else {
+      for (int e = 0; e < 2; ++e) {
+        const int r = q * 8 + 2 * c4 + e;
+        l[q][e] = column_sum(l[q][e]);
+        if (g4 == 0) s_ms[warp * R + r] = make_float2(m[q][e], l[q][e]);
+        if (r < p.nr) {
+          float* dst = merge + ((size_t)warp * p.nr + r) * MP;
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<float2*>(dst + n * 8 + c4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+          for (int k = 0; k < KS; ++k) {
+            if (E4M3) {
+              *reinterpret_cast<float2*>(dst + k * 16 + g4 * 2) = make_float2(o[q][k][e] * f, o[q][k][2 + e] * f);
+            } else {
+              dst[k * 16 + g4] = o[q][k][e];
+              dst[k * 16 + 8 + g4] = o[q][k][2 + e];
+            }
+          }
         }
       }
-    }
     __syncthreads();
     }
     float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * part_ld;
@@ -754,7 +789,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
 #pragma unroll 1
       for (int i = tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
-        const float* x = src + (again ? i * 4 : r * D + d);
+        const float* x = src + (again ? i * 4 : r * pitch + d);
         const float2* y = ms + (again ? i : r);
         float a = kNoMax, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -888,7 +923,7 @@ int attend_smem(const AttendParams& p, int stages) {
   return C::W * stages * (2 * C::KB + C::SC) + p.merge * 4 + (p.c.batch + 1) * (int)sizeof(SeqInfo);
 }
 // Static shared memory of the kernel, rounded up.
-constexpr int kSmemStatic = 4 * 1024;
+constexpr int kSmemStatic = 5 * 1024;
 
 template <class C>
 int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
@@ -898,7 +933,7 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   while ((1 << p.box_shift) < box) ++p.box_shift;
   if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss, box)) return s;
   if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss, box)) return s;
-  p.merge = std::max(C::W * p.nr * C::D, C::W * 32 * 4);  // the warps' outputs, or a join's thread groups' sums
+  p.merge = std::max(C::W * p.nr * C::MP, C::W * 32 * 4);  // the warps' outputs, or a join's thread groups' sums
   p.stages = kMaxStages;
   while (p.stages > 1 && attend_smem<C>(p, p.stages) + kSmemStatic > kSmemMax) --p.stages;
   const int smem = attend_smem<C>(p, p.stages);
@@ -909,18 +944,32 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   return launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, st, km, vm, p);
 }
 
+// Query rows of an item: as many tiles of eight as the head's rows fill, up to four (two for D = 256, whose output
+// would not fit the registers): each cached byte is then read once for all of them.
+int item_rows(int64_t D, int64_t rows) { return rows <= 8 ? 8 : rows <= 16 || D == 256 ? 16 : 32; }
+
 struct Workspace {
   int64_t rows, chunks, nr, part, lse, logits;  // sizes in floats, in this order
   Workspace(const tbf16_paged_cache* c, int64_t Hq, int64_t T, bool weights, int sms) {
     rows = T * (Hq / c->heads);
-    chunks = (rows + kRows - 1) / kRows;
-    nr = std::min<int64_t>(rows, kRows);
-    part = 2 * (int64_t)sms * (nr * c->D + 2 * kRows);
+    const int R = item_rows(c->D, rows);
+    chunks = (rows + R - 1) / R;
+    nr = std::min<int64_t>(rows, R);
+    part = 2 * (int64_t)sms * partial_floats((int)nr, (int)c->D);
     lse = weights ? (c->batch * c->heads * rows + 3) / 4 * 4 : 0;
     logits = weights ? c->batch * c->heads * rows * c->max_pages * c->page_size : 0;
   }
   int64_t bytes() const { return (part + lse + logits) * 4; }
 };
+
+template <int D, bool E4M3>
+int launch_rows(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
+  const int R = item_rows(D, p.rows);
+  if (R == 8) return launch_attend<Tile<D, E4M3, 1>>(cache, p, sms, st);
+  if constexpr (D < 256)
+    if (R == 32) return launch_attend<Tile<D, E4M3, 4>>(cache, p, sms, st);
+  return launch_attend<Tile<D, E4M3, 2>>(cache, p, sms, st);
+}
 
 bool attend_sizes_ok(const tbf16_paged_cache* c, int64_t Hq, int64_t T) {
   return c && c->batch >= 0 && c->heads >= 1 && Hq >= 1 && Hq <= 65536 && Hq % c->heads == 0 && T >= 0 && T <= 4096 &&
@@ -937,7 +986,7 @@ extern "C" int64_t tbf16_paged_attend_ws_size(const tbf16_paged_cache* cache, in
 
 extern "C" int64_t tbf16_paged_attend_sync_size(const tbf16_paged_cache* cache, int64_t Hq, int64_t T) {
   if (!attend_sizes_ok(cache, Hq, T)) return 0;
-  return cache->batch * cache->heads * ((T * (Hq / cache->heads) + kRows - 1) / kRows) * 4;
+  return cache->batch * cache->heads * Workspace(cache, Hq, T, false, 0).chunks * 4;
 }
 
 extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh,
@@ -980,12 +1029,9 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   const bool e4m3 = cache->dtype == TBF16_E4M3;
   auto st = static_cast<cudaStream_t>(stream);
   int rc;
-  if (cache->D == 64)
-    rc = e4m3 ? launch_attend<Tile<64, true>>(cache, p, dev->sms, st) : launch_attend<Tile<64, false>>(cache, p, dev->sms, st);
-  else if (cache->D == 128)
-    rc = e4m3 ? launch_attend<Tile<128, true>>(cache, p, dev->sms, st) : launch_attend<Tile<128, false>>(cache, p, dev->sms, st);
-  else
-    rc = e4m3 ? launch_attend<Tile<256, true>>(cache, p, dev->sms, st) : launch_attend<Tile<256, false>>(cache, p, dev->sms, st);
+  if (cache->D == 64) rc = e4m3 ? launch_rows<64, true>(cache, p, dev->sms, st) : launch_rows<64, false>(cache, p, dev->sms, st);
+  else if (cache->D == 128) rc = e4m3 ? launch_rows<128, true>(cache, p, dev->sms, st) : launch_rows<128, false>(cache, p, dev->sms, st);
+  else rc = e4m3 ? launch_rows<256, true>(cache, p, dev->sms, st) : launch_rows<256, false>(cache, p, dev->sms, st);
   if (rc != TBF16_OK || !weights) return rc;
   const int block_keys = cache->D * (e4m3 ? 1 : 2) <= 64 ? 64 : cache->D * (e4m3 ? 1 : 2) <= 128 ? 32 : 16;
   const int64_t blocks = cache->batch * cache->heads * ((p.c.cap + 1023) / 1024);
