@@ -70,9 +70,12 @@ struct AppendParams {
   const int* seen;
   int* pos;
   int64_t pos_sb, pos_sh;
-  int T, d8;        // d8: source row length in 8-element vectors
-  unsigned rows;    // batch * T * heads
+  int T, d8;           // d8: source row length in 8-element vectors
+  int tile, tiles;     // tokens of a block, blocks of a sequence
+  unsigned heads_inv;  // ceil(2^32 / heads): row / heads = umulhi(row, heads_inv) below 2^16
 };
+constexpr int kAppendTile = 64;    // most tokens of a block
+constexpr int kAppendVectors = 4;  // 16-byte loads that a thread has in flight
 
 // Eight bf16 values times `scale` (a power of two: exact short of e4m3's range) rounded to nearest-even e4m3.
 __device__ __forceinline__ uint2 e4m3x8(uint4 x, float scale) {
@@ -84,56 +87,76 @@ __device__ __forceinline__ uint2 e4m3x8(uint4 x, float scale) {
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// Copies each new row to its slot; blockIdx.y picks keys or values. D / 8 lanes hold a row, 8 elements each.
+// A block copies the rows of `tile` new tokens of one sequence to their slots; blockIdx.y picks keys or values.
+// D / 8 lanes hold a row, 8 elements each. Bound by HBM: each row is read and written once, with kAppendVectors
+// loads in flight in a thread; lengths and page numbers are looked up once for the block, while those are.
 // An e4m3 row is scaled by 2^(8 - e), e the exponent (frexp) of its largest magnitude, which lands in
 // [128, 256): half the format's range stays unused, none of its precision does, and nothing can saturate.
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  constexpr int LR = D / 8;
-  const int kv = blockIdx.y;
-  const unsigned unit = blockIdx.x * 256u + threadIdx.x;
-  const unsigned row = unit / LR;
-  const int chunk = unit % LR;
-  const bool live = row < p.rows;
-  const unsigned r = live ? row : 0;
-  const int h = (int)(r % (unsigned)p.c.heads);
-  const unsigned bt = r / (unsigned)p.c.heads;
-  const int t = (int)(bt % (unsigned)p.T), b = (int)(bt / (unsigned)p.T);
-  uint4 x = make_uint4(0, 0, 0, 0);
-  if (live && chunk < p.d8)
-    x = *reinterpret_cast<const uint4*>(p.src[kv] + b * p.sb[kv] + h * p.sh[kv] + t * p.st[kv] + chunk * 8);
+  constexpr int LR = D / 8, V = kAppendVectors, ROWS = 256 / LR;
+  __shared__ int s_page[kAppendTile];
+  const int kv = blockIdx.y, tid = threadIdx.x, chunk = tid % LR;
+  const int b = (int)(blockIdx.x / (unsigned)p.tiles), t0 = (int)(blockIdx.x % (unsigned)p.tiles) * p.tile;
+  pdl_launch_dependents();
+  pdl_wait();
   const int len = paged_len(p.c, b), n = paged_count(p.c, p.counts, b, p.T, len);
-  const int j = len - n + t;
-  const int page = live && t < n ? paged_page(p.c, b, j) : -1;
-  const int slot = paged_slot(p.c, j);
-  if (p.pos && page >= 0 && kv == 0 && chunk == 0) p.pos[b * p.pos_sb + h * p.pos_sh + j] = p.seen[b] - n + t;
-  uint8_t* pool = kv ? p.c.v : p.c.k;
-  const int64_t at = kv ? page * p.c.v_sp + h * p.c.v_sh + slot * p.c.v_ss : page * p.c.k_sp + h * p.c.k_sh + slot * p.c.k_ss;
-  if (!E4M3) {
-    if (page >= 0) *reinterpret_cast<uint4*>(pool + at + chunk * 16) = x;
-    return;
-  }
-  // the largest magnitude as bits: ordered like the values, infinity and NaN on top
-  unsigned m = 0;
-  for (uint32_t w : {x.x, x.y, x.z, x.w}) m = max(m, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+  const int tokens = min(p.tile, n - t0), first = len - n + t0;
+  if (tokens <= 0) return;
+  const int rows = tokens * p.c.heads;
+  const __nv_bfloat16* src = p.src[kv] + b * p.sb[kv] + t0 * p.st[kv] + chunk * 8;
+  uint8_t* pool = (kv ? p.c.v : p.c.k) + chunk * (E4M3 ? 8 : 16);
+  const int64_t sp = kv ? p.c.v_sp : p.c.k_sp, sh = kv ? p.c.v_sh : p.c.k_sh, ss = kv ? p.c.v_ss : p.c.k_ss;
+  if (tid < tokens) s_page[tid] = paged_page(p.c, b, first + tid);
+  for (int r0 = tid / LR; r0 - tid / LR < rows; r0 += V * ROWS) {
+    uint4 x[V];
 #pragma unroll
-  for (int o = LR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (page < 0) return;
-  const bool finite = m < 0x7f800000u;
-  // 2^-119 keeps 2^(8 - e) inside fp32; smaller rows round to e4m3's subnormals
-  const int e = m == 0 || !finite ? 8 : frexp_exp(fmaxf(__uint_as_float(m), __uint_as_float(8u << 23)));
-  *reinterpret_cast<uint2*>(pool + at + chunk * 8) = e4m3x8(x, exp2i(8 - e));
-  if (chunk == 0) {
-    float* s = kv ? p.c.v_scale + page * p.c.vs_sp + h * p.c.vs_sh : p.c.k_scale + page * p.c.ks_sp + h * p.c.ks_sh;
-    s[slot] = finite ? exp2i(e - 8) : __uint_as_float(0x7fc00000u);
+    for (int i = 0; i < V; ++i) {
+      const int r = r0 + i * ROWS, t = p.c.heads == 1 ? r : (int)__umulhi((unsigned)r, p.heads_inv);
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (r < rows && chunk < p.d8)
+        x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)(r - t * p.c.heads) * p.sh[kv] + t * p.st[kv]));
+    }
+    if (r0 - tid / LR == 0) __syncthreads();  // s_page
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int r = r0 + i * ROWS, t = p.c.heads == 1 ? r : (int)__umulhi((unsigned)r, p.heads_inv), h = r - t * p.c.heads;
+      const int page = r < rows ? s_page[t] : -1, slot = paged_slot(p.c, first + t);
+      if (p.pos && page >= 0 && kv == 0 && chunk == 0) p.pos[b * p.pos_sb + h * p.pos_sh + first + t] = p.seen[b] - n + t0 + t;
+      const int64_t at = page * sp + h * sh + slot * ss;
+      if (!E4M3) {
+        if (page >= 0) *reinterpret_cast<uint4*>(pool + at) = x[i];
+        continue;
+      }
+      // the largest magnitude as bits: ordered like the values, infinity and NaN on top
+      unsigned m = 0;
+      for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) m = max(m, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+#pragma unroll
+      for (int o = LR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (page < 0) continue;
+      const bool finite = m < 0x7f800000u;
+      // 2^-119 keeps 2^(8 - e) inside fp32; smaller rows round to e4m3's subnormals
+      const int e = m == 0 || !finite ? 8 : frexp_exp(fmaxf(__uint_as_float(m), __uint_as_float(8u << 23)));
+      *reinterpret_cast<uint2*>(pool + at) = e4m3x8(x[i], exp2i(8 - e));
+      if (chunk == 0) {
+        float* s = kv ? p.c.v_scale + page * p.c.vs_sp + h * p.c.vs_sh : p.c.k_scale + page * p.c.ks_sp + h * p.c.ks_sh;
+        s[slot] = finite ? exp2i(e - 8) : __uint_as_float(0x7fc00000u);
+      }
+    }
   }
 }
 
 template <int D>
-void launch_append(const AppendParams& p, bool e4m3, cudaStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)p.rows * (D / 8) + 255) / 256), 2);
-  if (e4m3) append_kernel<D, true><<<grid, 256, 0, st>>>(p);
-  else append_kernel<D, false><<<grid, 256, 0, st>>>(p);
+int launch_append(AppendParams& p, bool e4m3, cudaStream_t st) {
+  // as many tokens as keep every thread's loads in flight twice, one for decoding
+  constexpr int ROWS = 256 / (D / 8);
+  const int want = (2 * kAppendVectors * ROWS + p.c.heads - 1) / p.c.heads;
+  p.tile = std::min(std::min(want, kAppendTile), p.T);
+  p.tiles = (p.T + p.tile - 1) / p.tile;
+  const int64_t blocks = (int64_t)p.c.batch * p.tiles;
+  if (blocks > INT32_MAX) return TBF16_ERR_INVALID;
+  return tbf16_host::launch_pdl(e4m3 ? append_kernel<D, true> : append_kernel<D, false>, dim3((unsigned)blocks, 2), 256, 0, st,
+                                p);
 }
 
 // ------------------------------------------------------------------ compact
@@ -297,8 +320,7 @@ extern "C" int tbf16_paged_append(const tbf16_paged_cache* cache, const void* k,
   if (int st = tbf16_host::paged_view(cache, &p.c)) return st;
   if (T == 0 || cache->batch == 0) return TBF16_OK;
   if (!k || !v || T < 0 || d < 8 || d > cache->D || (pos && !seen)) return TBF16_ERR_INVALID;
-  const int64_t rows = cache->batch * cache->heads * T;
-  if (T > INT32_MAX || rows > (INT64_C(1) << 31) / 32) return TBF16_ERR_INVALID;
+  if (T > INT32_MAX / 2) return TBF16_ERR_INVALID;
   for (int64_t s : {k_sb, k_sh, k_st, v_sb, v_sh, v_st}) {
     if (s < 0) return TBF16_ERR_INVALID;
     if (s % 8) return TBF16_ERR_ALIGN;
@@ -315,13 +337,12 @@ extern "C" int tbf16_paged_append(const tbf16_paged_cache* cache, const void* k,
   p.pos_sh = pos_sh;
   p.T = (int)T;
   p.d8 = (int)(d / 8);
-  p.rows = (unsigned)rows;
+  p.heads_inv = (unsigned)(((UINT64_C(1) << 32) + cache->heads - 1) / cache->heads);
   auto st = static_cast<cudaStream_t>(stream);
   const bool e4m3 = cache->dtype == TBF16_E4M3;
-  if (cache->D == 64) launch_append<64>(p, e4m3, st);
-  else if (cache->D == 128) launch_append<128>(p, e4m3, st);
-  else launch_append<256>(p, e4m3, st);
-  return tbf16_host::check_launch();
+  if (cache->D == 64) return launch_append<64>(p, e4m3, st);
+  if (cache->D == 128) return launch_append<128>(p, e4m3, st);
+  return launch_append<256>(p, e4m3, st);
 }
 
 namespace {

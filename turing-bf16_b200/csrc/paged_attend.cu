@@ -896,26 +896,6 @@ int tile_map(CUtensorMap* map, void* base, const tbf16_paged_cache* c, int64_t s
   return tbf16_host::make_tmap_pages(map, base, item, c->D, span, c->page_size, c->heads, c->pages, ss, sh, sp, box);
 }
 
-// A launch that may be set up while the kernel before it in the stream ends (the kernels wait for it themselves).
-template <class... Params, class... Args>
-int launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
-    cudaGetLastError();
-    return TBF16_ERR_LAUNCH;
-  }
-  return TBF16_OK;
-}
-
 constexpr int kSmemMax = 227 * 1024;
 
 template <class C>
@@ -941,7 +921,7 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   static const cudaError_t attr =
       cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic);
   if (attr != cudaSuccess) return TBF16_ERR_LAUNCH;
-  return launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, st, km, vm, p);
+  return tbf16_host::launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, st, km, vm, p);
 }
 
 // Query rows of an item: as many tiles of eight as the head's rows fill, up to four (two for D = 256, whose output
@@ -1035,6 +1015,6 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   if (rc != TBF16_OK || !weights) return rc;
   const int block_keys = cache->D * (e4m3 ? 1 : 2) <= 64 ? 64 : cache->D * (e4m3 ? 1 : 2) <= 128 ? 32 : 16;
   const int64_t blocks = cache->batch * cache->heads * ((p.c.cap + 1023) / 1024);
-  return launch_pdl(weights_kernel, (unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8), 256, 0, st, p, weights, w_sb,
+  return tbf16_host::launch_pdl(weights_kernel, (unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8), 256, 0, st, p, weights, w_sb,
                     w_sh, block_keys);
 }
