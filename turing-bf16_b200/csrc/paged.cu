@@ -128,19 +128,21 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
         if (page >= 0) *reinterpret_cast<uint4*>(pool + at) = x[i];
         continue;
       }
-      // the largest magnitude as bits: ordered like the values, infinity and NaN on top
+      // the largest magnitude as bits, ordered like the values with infinity and NaN on top; two in a register
       unsigned m = 0;
-      for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) m = max(m, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+      for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) m = __vmaxu2(m, w & 0x7fff7fffu);
 #pragma unroll
-      for (int o = LR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int o = LR / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+      m = max(m << 16, m & 0xffff0000u);
       if (page < 0) continue;
       const bool finite = m < 0x7f800000u;
-      // 2^-119 keeps 2^(8 - e) inside fp32; smaller rows round to e4m3's subnormals
-      const int e = m == 0 || !finite ? 8 : frexp_exp(fmaxf(__uint_as_float(m), __uint_as_float(8u << 23)));
-      *reinterpret_cast<uint2*>(pool + at) = e4m3x8(x[i], exp2i(8 - e));
+      // its frexp exponent; at least -118 (2^-119), so that 2^(8 - e) and 2^(e - 8) are normal: smaller rows round to
+      // e4m3's subnormals
+      const int e = m == 0 || !finite ? 8 : (int)(max(m, 8u << 23) >> 23) - 126;
+      *reinterpret_cast<uint2*>(pool + at) = e4m3x8(x[i], __uint_as_float((unsigned)(135 - e) << 23));
       if (chunk == 0) {
         float* s = kv ? p.c.v_scale + page * p.c.vs_sp + h * p.c.vs_sh : p.c.k_scale + page * p.c.ks_sp + h * p.c.ks_sh;
-        s[slot] = finite ? exp2i(e - 8) : __uint_as_float(0x7fc00000u);
+        s[slot] = __uint_as_float(finite ? (unsigned)(119 + e) << 23 : 0x7fc00000u);
       }
     }
   }
