@@ -70,12 +70,12 @@ struct AppendParams {
   const int* seen;
   int* pos;
   int64_t pos_sb, pos_sh;
-  int T, d8;           // d8: source row length in 8-element vectors
-  int tile, tiles;     // tokens of a block, blocks of a sequence
-  unsigned heads_inv;  // ceil(2^32 / heads): row / heads = umulhi(row, heads_inv) below 2^16
+  int T, d8;       // d8: source row length in 8-element vectors
+  int tp_log2;     // log2 of the tokens of a pass
+  int tiles;       // blocks of a sequence, kAppendVectors passes of tokens each
+  int block_heads; // heads of a block
 };
-constexpr int kAppendTile = 64;    // most tokens of a block
-constexpr int kAppendVectors = 4;  // 16-byte loads that a thread has in flight
+constexpr int kAppendVectors = 4;  // rows that a thread has in flight
 
 // Eight bf16 values times `scale` (a power of two: exact short of e4m3's range) rounded to nearest-even e4m3.
 __device__ __forceinline__ uint2 e4m3x8(uint4 x, float scale) {
@@ -87,78 +87,96 @@ __device__ __forceinline__ uint2 e4m3x8(uint4 x, float scale) {
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// A block copies the rows of `tile` new tokens of one sequence to their slots; blockIdx.y picks keys or values.
-// D / 8 lanes hold a row, 8 elements each. Bound by HBM: each row is read and written once, with kAppendVectors
-// loads in flight in a thread; lengths and page numbers are looked up once for the block, while those are.
+// A block copies the rows of some tokens and heads of one sequence to their slots; blockIdx.y picks keys or values.
+// D / 8 lanes hold a row, 8 elements each; the 256 D / 8 rows of a pass are 2^tp_log2 tokens (one when decoding) x
+// heads, and a thread goes through the heads with the same kAppendVectors tokens, so that page numbers and offsets
+// are worked out once and a row costs two pointer steps (with both strides multiplied out for each row, the 8-bit
+// form was bound by instructions: 163 a row, 37 us where this takes AAA). Bound by HBM: each row is read once and
+// written once.
 // An e4m3 row is scaled by 2^(8 - e), e the exponent (frexp) of its largest magnitude, which lands in
 // [128, 256): half the format's range stays unused, none of its precision does, and nothing can saturate.
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   constexpr int LR = D / 8, V = kAppendVectors, ROWS = 256 / LR;
-  __shared__ int s_page[kAppendTile];
-  const int kv = blockIdx.y, tid = threadIdx.x, chunk = tid % LR;
-  const int b = (int)(blockIdx.x / (unsigned)p.tiles), t0 = (int)(blockIdx.x % (unsigned)p.tiles) * p.tile;
+  const int kv = blockIdx.y, chunk = threadIdx.x % LR, row = threadIdx.x / LR;
+  const int b = (int)(blockIdx.x / (unsigned)p.tiles), tp = 1 << p.tp_log2;
+  const int t0 = (int)(blockIdx.x % (unsigned)p.tiles) * (V * tp) + (row & (tp - 1));
+  const int h0 = blockIdx.z * p.block_heads + (row >> p.tp_log2), h1 = min(p.c.heads, (int)(blockIdx.z + 1) * p.block_heads);
+  const int hp = ROWS >> p.tp_log2;
   pdl_launch_dependents();
   pdl_wait();
   const int len = paged_len(p.c, b), n = paged_count(p.c, p.counts, b, p.T, len);
-  const int tokens = min(p.tile, n - t0), first = len - n + t0;
-  if (tokens <= 0) return;
-  const int rows = tokens * p.c.heads;
-  const __nv_bfloat16* src = p.src[kv] + b * p.sb[kv] + t0 * p.st[kv] + chunk * 8;
-  uint8_t* pool = (kv ? p.c.v : p.c.k) + chunk * (E4M3 ? 8 : 16);
-  const int64_t sp = kv ? p.c.v_sp : p.c.k_sp, sh = kv ? p.c.v_sh : p.c.k_sh, ss = kv ? p.c.v_ss : p.c.k_ss;
-  if (tid < tokens) s_page[tid] = paged_page(p.c, b, first + tid);
-  for (int r0 = tid / LR; r0 - tid / LR < rows; r0 += V * ROWS) {
+  if (t0 - (row & (tp - 1)) >= n) return;
+  const __nv_bfloat16* src[V];
+  uint8_t* dst[V];
+  float* scale[V];
+  const int64_t sh = kv ? p.c.v_sh : p.c.k_sh, ssh = kv ? p.c.vs_sh : p.c.ks_sh;
+  int live = 0;  // bit i: token i is there and its page is in the pool
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int t = t0 + i * tp, j = len - n + t, page = t < n ? paged_page(p.c, b, j) : -1, slot = paged_slot(p.c, j);
+    live |= (page >= 0) << i;
+    src[i] = p.src[kv] + b * p.sb[kv] + h0 * p.sh[kv] + t * p.st[kv] + chunk * 8;
+    dst[i] = (kv ? p.c.v + page * p.c.v_sp + slot * p.c.v_ss : p.c.k + page * p.c.k_sp + slot * p.c.k_ss) + h0 * sh +
+             chunk * (E4M3 ? 8 : 16);
+    if (E4M3) scale[i] = (kv ? p.c.v_scale + page * p.c.vs_sp : p.c.k_scale + page * p.c.ks_sp) + h0 * ssh + slot;
+    if (p.pos && page >= 0 && kv == 0 && chunk == 0)
+      for (int h = h0; h < h1; h += hp) p.pos[b * p.pos_sb + h * p.pos_sh + j] = p.seen[b] - n + t;
+  }
+  const int passes = (h1 - (int)(blockIdx.z * p.block_heads) + hp - 1) / hp;
+#pragma unroll 1
+  for (int k = 0, h = h0; k < passes; ++k, h += hp) {
+    if (h >= h1) live = 0;
     uint4 x[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int r = r0 + i * ROWS, t = p.c.heads == 1 ? r : (int)__umulhi((unsigned)r, p.heads_inv);
       x[i] = make_uint4(0, 0, 0, 0);
-      if (r < rows && chunk < p.d8)
-        x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)(r - t * p.c.heads) * p.sh[kv] + t * p.st[kv]));
+      if (((live >> i) & 1) && chunk < p.d8) x[i] = __ldcs(reinterpret_cast<const uint4*>(src[i]));
+      src[i] += hp * p.sh[kv];
     }
-    if (r0 - tid / LR == 0) __syncthreads();  // s_page
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int r = r0 + i * ROWS, t = p.c.heads == 1 ? r : (int)__umulhi((unsigned)r, p.heads_inv), h = r - t * p.c.heads;
-      const int page = r < rows ? s_page[t] : -1, slot = paged_slot(p.c, first + t);
-      if (p.pos && page >= 0 && kv == 0 && chunk == 0) p.pos[b * p.pos_sb + h * p.pos_sh + first + t] = p.seen[b] - n + t0 + t;
-      const int64_t at = page * sp + h * sh + slot * ss;
-      if (!E4M3) {
-        if (page >= 0) *reinterpret_cast<uint4*>(pool + at) = x[i];
-        continue;
-      }
-      // the largest magnitude as bits, ordered like the values with infinity and NaN on top; two in a register
-      unsigned m = 0;
-      for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) m = __vmaxu2(m, w & 0x7fff7fffu);
+      if (E4M3) {
+        // the largest magnitude as bits, ordered like the values with infinity and NaN on top; two in a register
+        unsigned m = 0;
+        for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) m = __vmaxu2(m, w & 0x7fff7fffu);
 #pragma unroll
-      for (int o = LR / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
-      m = max(m << 16, m & 0xffff0000u);
-      if (page < 0) continue;
-      const bool finite = m < 0x7f800000u;
-      // its frexp exponent; at least -118 (2^-119), so that 2^(8 - e) and 2^(e - 8) are normal: smaller rows round to
-      // e4m3's subnormals
-      const int e = m == 0 || !finite ? 8 : (int)(max(m, 8u << 23) >> 23) - 126;
-      *reinterpret_cast<uint2*>(pool + at) = e4m3x8(x[i], __uint_as_float((unsigned)(135 - e) << 23));
-      if (chunk == 0) {
-        float* s = kv ? p.c.v_scale + page * p.c.vs_sp + h * p.c.vs_sh : p.c.k_scale + page * p.c.ks_sp + h * p.c.ks_sh;
-        s[slot] = __uint_as_float(finite ? (unsigned)(119 + e) << 23 : 0x7fc00000u);
+        for (int o = LR / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = max(m << 16, m & 0xffff0000u);
+        const bool finite = m < 0x7f800000u;
+        // its frexp exponent; at least -118 (2^-119), so that 2^(8 - e) and 2^(e - 8) are normal: smaller rows round
+        // to e4m3's subnormals
+        const int e = m == 0 || !finite ? 8 : (int)(max(m, 8u << 23) >> 23) - 126;
+        const uint2 y = e4m3x8(x[i], __uint_as_float((unsigned)(135 - e) << 23));
+        if ((live >> i) & 1) {
+          *reinterpret_cast<uint2*>(dst[i]) = y;
+          if (chunk == 0) *scale[i] = __uint_as_float(finite ? (unsigned)(119 + e) << 23 : 0x7fc00000u);
+        }
+        scale[i] += hp * ssh;
+      } else if ((live >> i) & 1) {
+        *reinterpret_cast<uint4*>(dst[i]) = x[i];
       }
+      dst[i] += hp * sh;
     }
   }
 }
 
 template <int D>
 int launch_append(AppendParams& p, bool e4m3, cudaStream_t st) {
-  // as many tokens as keep every thread's loads in flight twice, one for decoding
   constexpr int ROWS = 256 / (D / 8);
-  const int want = (2 * kAppendVectors * ROWS + p.c.heads - 1) / p.c.heads;
-  p.tile = std::min(std::min(want, kAppendTile), p.T);
-  p.tiles = (p.T + p.tile - 1) / p.tile;
+  p.tp_log2 = 0;
+  while ((2 << p.tp_log2) <= std::min(p.T, ROWS)) ++p.tp_log2;
+  const int tokens = kAppendVectors << p.tp_log2, hp = ROWS >> p.tp_log2, passes = (p.c.heads + hp - 1) / hp;
+  p.tiles = (p.T + tokens - 1) / tokens;
   const int64_t blocks = (int64_t)p.c.batch * p.tiles;
   if (blocks > INT32_MAX) return TBF16_ERR_INVALID;
-  return tbf16_host::launch_pdl(e4m3 ? append_kernel<D, true> : append_kernel<D, false>, dim3((unsigned)blocks, 2), 256, 0, st,
-                                p);
+  // a block takes several passes of heads only while there are four blocks an SM all the same
+  const int sms = tbf16_host::device_info()->sms;
+  const int64_t k = std::max<int64_t>(1, std::min<int64_t>(passes, 2 * blocks * passes / (4 * sms)));
+  p.block_heads = (int)k * hp;
+  return tbf16_host::launch_pdl(e4m3 ? append_kernel<D, true> : append_kernel<D, false>,
+                                dim3((unsigned)blocks, 2, (unsigned)((p.c.heads + p.block_heads - 1) / p.block_heads)), 256, 0,
+                                st, p);
 }
 
 // ------------------------------------------------------------------ compact
@@ -339,7 +357,6 @@ extern "C" int tbf16_paged_append(const tbf16_paged_cache* cache, const void* k,
   p.pos_sh = pos_sh;
   p.T = (int)T;
   p.d8 = (int)(d / 8);
-  p.heads_inv = (unsigned)(((UINT64_C(1) << 32) + cache->heads - 1) / cache->heads);
   auto st = static_cast<cudaStream_t>(stream);
   const bool e4m3 = cache->dtype == TBF16_E4M3;
   if (cache->D == 64) return launch_append<64>(p, e4m3, st);
