@@ -176,22 +176,28 @@ int launch_append(AppendParams& p, bool e4m3, cudaStream_t st) {
   p.block_heads = (int)k * hp;
   return tbf16_host::launch_pdl(e4m3 ? append_kernel<D, true> : append_kernel<D, false>,
                                 dim3((unsigned)blocks, 2, (unsigned)((p.c.heads + p.block_heads - 1) / p.block_heads)), 256, 0,
-                                st, p);
+                                1, st, p);
 }
 
 // ------------------------------------------------------------------ compact
 
+// Which positions a (sequence, head) keeps, in two kernels: select_kernel ranks the positions by weight and lists
+// the moves, move_kernel makes them. Moves go from positions at or beyond `keep` to positions below it, so no
+// row is both read and written and all of them run at once, on the whole GPU however few the items are.
 struct CompactParams {
   PagedView c;
   const float* w;
   const int* pos;
   int64_t w_sb, w_sh, p_sb, p_sh;
   const int* seen;
-  int cols, keep, recent, row16;  // row16: 16-byte chunks of a key or value row
+  int cols, keep, recent;
+  int row16_log2;  // 16-byte chunks of a key or value row
   int scaled;
+  int in_smem;     // a CTA's keys stay in shared memory
   float* w_out;
   int* pos_out;
-  int2* moves;  // (from, to) for each (sequence, head): at most max_moves
+  int* counts;     // moves of each (sequence, head)
+  int2* moves;     // (from, to): max_moves for each
   int max_moves;
 };
 
@@ -204,128 +210,238 @@ __device__ __forceinline__ uint32_t rank_key(float w, int pos, int protect_from)
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Exclusive prefix of v over the block's 32 warps (one value per warp, the same in all its lanes), and the total.
-__device__ __forceinline__ int warp_prefix(int v, int* scratch, int& total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) scratch[warp] = v;
-  __syncthreads();
-  int x = scratch[lane], own = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const int y = __shfl_sync(0xffffffffu, x, i);
-    own += i < warp ? y : 0;
-    total += y;
-  }
-  __syncthreads();
-  return own;
-}
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kDigitBits = 11;  // keys are ranked by digits of 11, 11 and 10 bits: the first is sign, exponent and two
+constexpr int kBins = 1 << kDigitBits;  // bits of the weight, so that like weights still spread over several counters
 
-// One block per (sequence, head): the keep-th largest key by a radix select (four 8-bit digits, counted in
-// shared memory), then two passes that number the holes and the rows that fill them, then the copies.
-__global__ void __launch_bounds__(1024) compact_kernel(const CompactParams p) {
-  __shared__ int hist[256];
-  __shared__ int scratch[32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  const int b = blockIdx.x / p.c.heads, h = blockIdx.x % p.c.heads;
+// Sum of v over the warps (one value per warp), the sum of the warps before this one, and the same over the CTAs of
+// the cluster: exclusive prefix of this warp over all warps of the cluster, in order of CTA and warp.
+struct ClusterScan {
+  int* warp_sums;   // [kSelWarps]
+  int* cta_sum;     // one word that the other CTAs read
+  int ctas, rank;
+  __device__ int operator()(int v, int& total) const {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) warp_sums[warp] = v;
+    __syncthreads();
+    const int x = lane < kSelWarps ? warp_sums[lane] : 0;
+    int before = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
+    total = __reduce_add_sync(0xffffffffu, x);
+    if (ctas > 1) {
+      if (threadIdx.x == 0) *cta_sum = total;
+      cluster_sync();
+      int y = 0;
+      if (lane < ctas) asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(y) : "r"(mapa_u32(smem_u32(cta_sum), lane)));
+      before += __reduce_add_sync(0xffffffffu, lane < rank ? y : 0);
+      total = __reduce_add_sync(0xffffffffu, y);
+      cluster_sync();  // the word may be written again
+    } else {
+      __syncthreads();
+    }
+    return before;
+  }
+};
+
+// A cluster of 1 to 8 CTAs per (sequence, head), each with an equal slice of the positions, whose rank keys it keeps
+// in shared memory. The keep-th largest key comes from a radix select over the slices' histograms (read through
+// distributed shared memory); then every warp numbers its holes and the rows that fill them.
+__global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams p) {
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[kBins];
+  __shared__ int warp_sums[kSelWarps];
+  __shared__ int cta_sum, s_digit, s_need;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = min(paged_len(p.c, b), p.cols);
+  int ctas;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+  const int rank = (int)cluster_ctarank(), bh = blockIdx.x / ctas, b = bh / p.c.heads, h = bh % p.c.heads;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int n = min(paged_len(p.c, b), p.cols), left = min(n, p.keep);
   const float* w = p.w + b * p.w_sb + h * p.w_sh;
   const int* pos = p.pos + b * p.p_sb + h * p.p_sh;
-  const int64_t out = (int64_t)blockIdx.x * p.cols;
-  const int left = min(n, p.keep);
-  for (int i = left + tid; i < p.cols; i += 1024) {
-    p.w_out[out + i] = 0.f;
-    p.pos_out[out + i] = -1;
+  float* w_out = p.w_out + (int64_t)bh * p.cols;
+  int* pos_out = p.pos_out + (int64_t)bh * p.cols;
+  for (int i = left + rank * kSelThreads + tid; i < p.cols; i += ctas * kSelThreads) {
+    w_out[i] = 0.f;
+    pos_out[i] = -1;
   }
-  if (n <= p.keep) {
-    for (int i = tid; i < n; i += 1024) {
-      p.w_out[out + i] = w[i];
-      p.pos_out[out + i] = pos[i];
+  if (n <= p.keep || p.keep == 0) {  // the same in every CTA of the cluster
+    for (int i = rank * kSelThreads + tid; i < left; i += ctas * kSelThreads) {
+      w_out[i] = w[i];
+      pos_out[i] = pos[i];
     }
+    if (rank == 0 && tid == 0) p.counts[bh] = 0;
     return;
   }
-  if (p.keep == 0) return;
   const int protect_from = p.seen[b] - p.recent;
+  // this CTA's slice, and this warp's part of it, both in order
+  const int slice = (n + ctas - 1) / ctas, lo = min(n, rank * slice), hi = min(n, lo + slice);
+  const int per = ((hi - lo + kSelWarps - 1) / kSelWarps + 31) & ~31, first = lo + warp * per, last = min(hi, first + per);
+  auto key_at = [&](int i) { return p.in_smem ? keys[i - lo] : rank_key(w[i], pos[i], protect_from); };
   uint32_t prefix = 0;
   int need = p.keep;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  const ClusterScan scan{warp_sums, &cta_sum, ctas, rank};
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += 1024) {
-      const uint32_t key = rank_key(w[i], pos[i], protect_from);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+    if (pass == 0) {
+      for (int i = lo + tid; i < hi; i += 4 * kSelThreads) {
+        float x[4];
+        int y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = i + k * kSelThreads;
+          x[k] = j < hi ? w[j] : 0.f;
+          y[k] = j < hi ? pos[j] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = i + k * kSelThreads;
+          if (j >= hi) break;
+          const uint32_t key = rank_key(x[k], y[k], protect_from);
+          if (p.in_smem) keys[j - lo] = key;
+          atomicAdd(&hist[key >> 21], 1);
+        }
+      }
+    } else {
+      for (int i = lo + tid; i < hi; i += kSelThreads) {
+        const uint32_t key = key_at(i);
+        if ((key >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], 1);
+      }
     }
-    __syncthreads();
-    if (tid == 0) {
-      int above = 0, d = 255;
-      while (d > 0 && above + hist[d] < need) above += hist[d--];
-      s_prefix = prefix | ((uint32_t)d << shift);
-      s_need = need - above;
+    if (ctas > 1) cluster_sync();
+    else __syncthreads();
+    // counts of four bins a thread over the cluster, the highest bins first; the bin in which the need-th key lies
+    constexpr int PB = kBins / kSelThreads;
+    int bin[PB], mine = 0;
+#pragma unroll
+    for (int k = 0; k < PB; ++k) {
+      const int x = kBins - 1 - (tid * PB + k);
+      bin[k] = 0;
+      if (ctas == 1) {
+        bin[k] = hist[x];
+      } else {
+        for (int c = 0; c < ctas; ++c) {
+          int y;
+          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(y) : "r"(mapa_u32(smem_u32(&hist[x]), c)));
+          bin[k] += y;
+        }
+      }
+      mine += bin[k];
     }
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    prefix = s_prefix;
+    int above = x - mine + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane & (kSelWarps - 1)] : 0);
+#pragma unroll
+    for (int k = 0; k < PB; ++k) {
+      if (above < need && need <= above + bin[k]) {
+        s_digit = kBins - 1 - (tid * PB + k);
+        s_need = need - above;
+      }
+      above += bin[k];
+    }
+    if (ctas > 1) cluster_sync();  // every CTA has read the histograms
+    else __syncthreads();
+    prefix |= (uint32_t)s_digit << shift;
     need = s_need;
-    __syncthreads();
   }
   // `need` of the positions whose key equals `prefix` are kept, the lowest first
-  const int per = ((n + 31) / 32 + 31) / 32 * 32, first = warp * per, last = min(n, first + per);
   int ties = 0, total;
   for (int i = first + lane; i - lane < last; i += 32)
-    ties += __popc(__ballot_sync(0xffffffffu, i < last && rank_key(w[i], pos[i], protect_from) == prefix));
-  const int ties_before = warp_prefix(ties, scratch, total);
-  int2* moves = p.moves + (int64_t)blockIdx.x * p.max_moves;
-  int holes_before = 0, loose_before = 0, holes = 0, loose = 0, count = 0;
+    ties += __popc(__ballot_sync(0xffffffffu, i < last && key_at(i) == prefix));
+  const int ties_before = scan(ties, total);
+  int2* moves = p.moves + (int64_t)bh * p.max_moves;
+  int holes_before = 0, loose_before = 0;
+#pragma unroll 1
   for (int write = 0; write < 2; ++write) {
-    int tie = ties_before;
-    holes = loose = 0;
+    int tie = ties_before, holes = holes_before, loose = loose_before;
     for (int i = first + lane; i - lane < last; i += 32) {
       const bool in = i < last;
-      const uint32_t key = in ? rank_key(w[i], pos[i], protect_from) : 0u;
-      const unsigned eq = __ballot_sync(0xffffffffu, in && key == prefix);
-      const bool kept = in && (key > prefix || (key == prefix && tie + __popc(eq & ((1u << lane) - 1)) < need));
+      const uint32_t key = in ? key_at(i) : 0u;
+      const unsigned below = (1u << lane) - 1, eq = __ballot_sync(0xffffffffu, in && key == prefix);
+      const bool kept = in && (key > prefix || (key == prefix && tie + __popc(eq & below) < need));
       tie += __popc(eq);
       const unsigned hb = __ballot_sync(0xffffffffu, in && !kept && i < p.keep);
       const unsigned lb = __ballot_sync(0xffffffffu, kept && i >= p.keep);
       if (write) {
-        if ((hb >> lane) & 1) moves[holes_before + holes + __popc(hb & ((1u << lane) - 1))].y = i;
-        if ((lb >> lane) & 1) moves[loose_before + loose + __popc(lb & ((1u << lane) - 1))].x = i;
+        if ((hb >> lane) & 1) moves[holes + __popc(hb & below)].y = i;
+        if ((lb >> lane) & 1) moves[loose + __popc(lb & below)].x = i;
         if (kept && i < p.keep) {
-          p.w_out[out + i] = w[i];
-          p.pos_out[out + i] = pos[i];
+          w_out[i] = w[i];
+          pos_out[i] = pos[i];
         }
       }
       holes += __popc(hb);
       loose += __popc(lb);
     }
     if (!write) {
-      holes_before = warp_prefix(holes, scratch, count);
-      loose_before = warp_prefix(loose, scratch, total);
+      holes_before = scan(holes, total);
+      loose_before = scan(loose, total);
+      if (rank == 0 && tid == 0) p.counts[bh] = total;
     }
   }
-  __syncthreads();
-  for (int m = warp; m < count; m += 32) {
-    const int2 mv = moves[m];
-    const int from = paged_page(p.c, b, mv.x), to = paged_page(p.c, b, mv.y);
-    if (lane == 0) {
-      p.w_out[out + mv.y] = w[mv.x];
-      p.pos_out[out + mv.y] = pos[mv.x];
+}
+
+// Copies the listed rows, 16 bytes a thread, four in flight; grid (items, splits of an item's moves). With a row's
+// first chunk go its scale and, for keys, the position's weight and number.
+__global__ void __launch_bounds__(256) move_kernel(const CompactParams p) {
+  constexpr int V = 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int bh = blockIdx.x, b = bh / p.c.heads, h = bh % p.c.heads;
+  const int units = p.counts[bh] << (p.row16_log2 + 1);  // below 2^31: max_moves is (checked on the host)
+  const int2* moves = p.moves + (int64_t)bh * p.max_moves;
+  const int chunks = 1 << p.row16_log2;
+  for (int u0 = (blockIdx.y * V * 256) + threadIdx.x; u0 < units; u0 += gridDim.y * V * 256) {
+    uint8_t* dst[V];
+    const uint8_t* src[V];
+    int2 mv[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int u = u0 + k * 256;
+      mv[k] = u < units ? moves[u >> (p.row16_log2 + 1)] : make_int2(0, 0);
     }
-    if (from < 0 || to < 0) continue;
-    const int sf = paged_slot(p.c, mv.x), st = paged_slot(p.c, mv.y);
-    for (int i = lane; i < 2 * p.row16; i += 32) {
-      const bool v = i >= p.row16;
-      const int64_t off = (v ? i - p.row16 : i) * 16;
-      uint8_t* pool = v ? p.c.v + h * p.c.v_sh + off : p.c.k + h * p.c.k_sh + off;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int u = u0 + k * 256, i = u & (chunks - 1);
+      const bool v = (u >> p.row16_log2) & 1;
+      dst[k] = nullptr;
+      src[k] = nullptr;
+      if (u >= units) continue;
+      const int from = paged_page(p.c, b, mv[k].x), to = paged_page(p.c, b, mv[k].y);
+      const int sf = paged_slot(p.c, mv[k].x), st = paged_slot(p.c, mv[k].y);
+      if (i == 0 && !v) {
+        const int64_t out = (int64_t)bh * p.cols + mv[k].y;
+        p.w_out[out] = p.w[b * p.w_sb + h * p.w_sh + mv[k].x];
+        p.pos_out[out] = p.pos[b * p.p_sb + h * p.p_sh + mv[k].x];
+      }
+      if (from < 0 || to < 0) continue;
+      uint8_t* pool = (v ? p.c.v + h * p.c.v_sh : p.c.k + h * p.c.k_sh) + i * 16;
       const int64_t sp = v ? p.c.v_sp : p.c.k_sp, ss = v ? p.c.v_ss : p.c.k_ss;
-      *reinterpret_cast<uint4*>(pool + to * sp + st * ss) = *reinterpret_cast<const uint4*>(pool + from * sp + sf * ss);
+      dst[k] = pool + to * sp + st * ss;
+      src[k] = pool + from * sp + sf * ss;
+      if (p.scaled && i == 0) {
+        float* s = v ? p.c.v_scale + h * p.c.vs_sh : p.c.k_scale + h * p.c.ks_sh;
+        const int64_t ssp = v ? p.c.vs_sp : p.c.ks_sp;
+        s[to * ssp + st] = s[from * ssp + sf];
+      }
     }
-    if (p.scaled && lane < 2) {
-      float* s = lane ? p.c.v_scale + h * p.c.vs_sh : p.c.k_scale + h * p.c.ks_sh;
-      const int64_t sp = lane ? p.c.vs_sp : p.c.ks_sp;
-      s[to * sp + st] = s[from * sp + sf];
-    }
+    uint4 x[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (src[k]) x[k] = *reinterpret_cast<const uint4*>(src[k]);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (dst[k]) *reinterpret_cast<uint4*>(dst[k]) = x[k];
   }
 }
 
@@ -370,7 +486,8 @@ int64_t compact_max_moves(int64_t cols, int64_t keep) { return std::max<int64_t>
 
 extern "C" int64_t tbf16_paged_compact_ws_size(const tbf16_paged_cache* cache, int64_t cols, int64_t keep) {
   if (!cache || cache->batch < 0 || cache->heads < 1 || cols < 0 || keep < 0) return 0;
-  return cache->batch * cache->heads * compact_max_moves(cols, keep) * (int64_t)sizeof(int2);
+  const int64_t items = cache->batch * cache->heads;
+  return items * compact_max_moves(cols, keep) * (int64_t)sizeof(int2) + (items + 3) / 4 * 4 * (int64_t)sizeof(int);
 }
 
 extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* weights, int64_t w_sb, int64_t w_sh,
@@ -385,7 +502,7 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
     return TBF16_ERR_INVALID;
   const int64_t need = tbf16_paged_compact_ws_size(cache, cols, keep);
   if (need > 0 && (!ws || ws_bytes < need)) return TBF16_ERR_INVALID;
-  if (reinterpret_cast<uintptr_t>(ws) % sizeof(int2)) return TBF16_ERR_ALIGN;
+  if (!tbf16_host::aligned16(ws)) return TBF16_ERR_ALIGN;
   const int64_t items = cache->batch * cache->heads;
   if (items == 0 || cols == 0) return TBF16_OK;
   p.w = weights; p.w_sb = w_sb; p.w_sh = w_sh;
@@ -395,11 +512,30 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   p.keep = (int)keep;
   p.recent = (int)recent;
   p.scaled = cache->dtype == TBF16_E4M3;
-  p.row16 = (int)(cache->D * (p.scaled ? 1 : 2) / 16);
+  p.row16_log2 = 0;
+  while ((16 << p.row16_log2) < cache->D * (p.scaled ? 1 : 2)) ++p.row16_log2;
   p.w_out = weights_out;
   p.pos_out = pos_out;
-  p.moves = static_cast<int2*>(ws);
+  p.counts = static_cast<int*>(ws);
+  p.moves = reinterpret_cast<int2*>(p.counts + (items + 3) / 4 * 4);
   p.max_moves = (int)compact_max_moves(cols, keep);
-  compact_kernel<<<(unsigned)items, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return tbf16_host::check_launch();
+  if (((int64_t)p.max_moves << (p.row16_log2 + 1)) > INT32_MAX - 65536) return TBF16_ERR_INVALID;
+  // CTAs for an item: more while its slices are long and the items alone do not fill the SMs
+  const int sms = tbf16_host::device_info()->sms;
+  int ctas = 1;
+  while (ctas < 8 && (cols + ctas - 1) / ctas > 2048 && items * ctas * 2 <= 2 * sms) ctas *= 2;
+  constexpr int kMaxKeys = 48 * 1024;
+  while (ctas < 8 && (cols + ctas - 1) / ctas > kMaxKeys) ctas *= 2;
+  const int64_t slice = (cols + ctas - 1) / ctas;
+  p.in_smem = slice <= kMaxKeys;
+  static const cudaError_t attr = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
+  if (attr != cudaSuccess || items * ctas > INT32_MAX) return TBF16_ERR_LAUNCH;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (int rc = tbf16_host::launch_pdl(select_kernel, dim3((unsigned)(items * ctas)), kSelThreads,
+                                      p.in_smem ? (size_t)slice * 4 : 0, (unsigned)ctas, st, p))
+    return rc;
+  if (p.max_moves == 0) return TBF16_OK;
+  const int64_t blocks = (((int64_t)p.max_moves << (p.row16_log2 + 1)) + 1023) / 1024;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(blocks, 8 * sms / items));
+  return tbf16_host::launch_pdl(move_kernel, dim3((unsigned)items, (unsigned)splits), 256, 0, 1, st, p);
 }

@@ -45,19 +45,24 @@ namespace tbf16_host {
 // Checks a tbf16_paged_cache and fills the device view; TBF16_OK or the status to return.
 int paged_view(const tbf16_paged_cache* cache, tbf16::PagedView* view);
 
-// A launch that may be set up while the kernel before it in the stream ends (the kernels wait for it themselves).
+// A launch that may be set up while the kernel before it in the stream ends (the kernels wait for it themselves), in
+// clusters of `cluster` CTAs.
 template <class... Params, class... Args>
-int launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
+int launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st,
+               const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
     cudaGetLastError();
     return TBF16_ERR_LAUNCH;

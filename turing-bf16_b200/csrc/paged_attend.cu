@@ -921,7 +921,7 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   static const cudaError_t attr =
       cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic);
   if (attr != cudaSuccess) return TBF16_ERR_LAUNCH;
-  return tbf16_host::launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, st, km, vm, p);
+  return tbf16_host::launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, 1, st, km, vm, p);
 }
 
 // Query rows of an item: as many tiles of eight as the head's rows fill, up to four (two for D = 256, whose output
@@ -1015,6 +1015,6 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   if (rc != TBF16_OK || !weights) return rc;
   const int block_keys = cache->D * (e4m3 ? 1 : 2) <= 64 ? 64 : cache->D * (e4m3 ? 1 : 2) <= 128 ? 32 : 16;
   const int64_t blocks = cache->batch * cache->heads * ((p.c.cap + 1023) / 1024);
-  return tbf16_host::launch_pdl(weights_kernel, (unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8), 256, 0, st, p, weights, w_sb,
+  return tbf16_host::launch_pdl(weights_kernel, (unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8), 256, 0, 1, st, p, weights, w_sb,
                     w_sh, block_keys);
 }
