@@ -248,7 +248,7 @@ struct ClusterScan {
 // distributed shared memory); then every warp numbers its holes and the rows that fill them.
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams p) {
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[kBins];
+  __shared__ __align__(16) int hist[kBins];
   __shared__ int warp_sums[kSelWarps];
   __shared__ int cta_sum, s_digit, s_need;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -314,24 +314,31 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
     }
     if (ctas > 1) cluster_sync();
     else __syncthreads();
-    // counts of four bins a thread over the cluster, the highest bins first; the bin in which the need-th key lies
+    // counts of four bins a thread over the cluster, the highest bins first; the bin in which the need-th key lies.
+    // All CTAs' counts are asked for before the first is used.
     constexpr int PB = kBins / kSelThreads;
-    int bin[PB], mine = 0;
+    static_assert(PB == 4, "four bins a thread");
+    const int low_bin = kBins - PB - tid * PB;
+    int bin[PB] = {0, 0, 0, 0};
+    if (ctas == 1) {
 #pragma unroll
-    for (int k = 0; k < PB; ++k) {
-      const int x = kBins - 1 - (tid * PB + k);
-      bin[k] = 0;
-      if (ctas == 1) {
-        bin[k] = hist[x];
-      } else {
-        for (int c = 0; c < ctas; ++c) {
-          int y;
-          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(y) : "r"(mapa_u32(smem_u32(&hist[x]), c)));
-          bin[k] += y;
-        }
-      }
-      mine += bin[k];
+      for (int k = 0; k < PB; ++k) bin[k] = hist[low_bin + PB - 1 - k];
+    } else {
+      const uint32_t at = smem_u32(hist + low_bin);
+      int y[8][PB];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < ctas)
+          asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(y[c][0]), "=r"(y[c][1]), "=r"(y[c][2]), "=r"(y[c][3])
+                       : "r"(mapa_u32(at, c)));
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < ctas)
+#pragma unroll
+          for (int k = 0; k < PB; ++k) bin[k] += y[c][PB - 1 - k];
     }
+    const int mine = bin[0] + bin[1] + bin[2] + bin[3];
     int x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -391,57 +398,56 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   }
 }
 
-// Copies the listed rows, 16 bytes a thread, four in flight; grid (items, splits of an item's moves). With a row's
-// first chunk go its scale and, for keys, the position's weight and number.
+// Copies the listed rows; grid (items, splits of an item's moves). A block looks up the pages of kMoveRows moves (and
+// does their scales, weights and numbers), then streams the rows, 16 bytes a thread, eight loads in flight.
+constexpr int kMoveRows = 64;
 __global__ void __launch_bounds__(256) move_kernel(const CompactParams p) {
-  constexpr int V = 4;
+  constexpr int V = 8;
+  __shared__ int64_t s_from[2][kMoveRows], s_to[2][kMoveRows];  // byte offsets of keys, values; -1: not to be copied
   pdl_launch_dependents();
   pdl_wait();
-  const int bh = blockIdx.x, b = bh / p.c.heads, h = bh % p.c.heads;
-  const int units = p.counts[bh] << (p.row16_log2 + 1);  // below 2^31: max_moves is (checked on the host)
-  const int2* moves = p.moves + (int64_t)bh * p.max_moves;
-  const int chunks = 1 << p.row16_log2;
-  for (int u0 = (blockIdx.y * V * 256) + threadIdx.x; u0 < units; u0 += gridDim.y * V * 256) {
-    uint8_t* dst[V];
-    const uint8_t* src[V];
-    int2 mv[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int u = u0 + k * 256;
-      mv[k] = u < units ? moves[u >> (p.row16_log2 + 1)] : make_int2(0, 0);
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int u = u0 + k * 256, i = u & (chunks - 1);
-      const bool v = (u >> p.row16_log2) & 1;
-      dst[k] = nullptr;
-      src[k] = nullptr;
-      if (u >= units) continue;
-      const int from = paged_page(p.c, b, mv[k].x), to = paged_page(p.c, b, mv[k].y);
-      const int sf = paged_slot(p.c, mv[k].x), st = paged_slot(p.c, mv[k].y);
-      if (i == 0 && !v) {
-        const int64_t out = (int64_t)bh * p.cols + mv[k].y;
-        p.w_out[out] = p.w[b * p.w_sb + h * p.w_sh + mv[k].x];
-        p.pos_out[out] = p.pos[b * p.p_sb + h * p.p_sh + mv[k].x];
-      }
-      if (from < 0 || to < 0) continue;
-      uint8_t* pool = (v ? p.c.v + h * p.c.v_sh : p.c.k + h * p.c.k_sh) + i * 16;
-      const int64_t sp = v ? p.c.v_sp : p.c.k_sp, ss = v ? p.c.v_ss : p.c.k_ss;
-      dst[k] = pool + to * sp + st * ss;
-      src[k] = pool + from * sp + sf * ss;
-      if (p.scaled && i == 0) {
-        float* s = v ? p.c.v_scale + h * p.c.vs_sh : p.c.k_scale + h * p.c.ks_sh;
-        const int64_t ssp = v ? p.c.vs_sp : p.c.ks_sp;
-        s[to * ssp + st] = s[from * ssp + sf];
+  const int bh = blockIdx.x, b = bh / p.c.heads, h = bh % p.c.heads, tid = threadIdx.x;
+  const int count = p.counts[bh], chunk = tid & ((1 << p.row16_log2) - 1);
+  const bool value = (tid >> p.row16_log2) & 1;
+  uint8_t* pool = (value ? p.c.v + h * p.c.v_sh : p.c.k + h * p.c.k_sh) + chunk * 16;
+  const int row0 = tid >> (p.row16_log2 + 1), step = 256 >> (p.row16_log2 + 1);  // rows of a pass: 4 to 32
+  for (int m0 = blockIdx.y * kMoveRows; m0 < count; m0 += gridDim.y * kMoveRows) {
+    const int rows = min(kMoveRows, count - m0);
+    if (tid < rows) {
+      const int2 mv = p.moves[(int64_t)bh * p.max_moves + m0 + tid];
+      const int from = paged_page(p.c, b, mv.x), to = paged_page(p.c, b, mv.y);
+      const int sf = paged_slot(p.c, mv.x), st = paged_slot(p.c, mv.y);
+      const int64_t out = (int64_t)bh * p.cols + mv.y;
+      p.w_out[out] = p.w[b * p.w_sb + h * p.w_sh + mv.x];
+      p.pos_out[out] = p.pos[b * p.p_sb + h * p.p_sh + mv.x];
+      const bool ok = from >= 0 && to >= 0;
+      s_from[0][tid] = ok ? from * p.c.k_sp + sf * p.c.k_ss : -1;
+      s_from[1][tid] = ok ? from * p.c.v_sp + sf * p.c.v_ss : -1;
+      s_to[0][tid] = to * p.c.k_sp + st * p.c.k_ss;
+      s_to[1][tid] = to * p.c.v_sp + st * p.c.v_ss;
+      if (ok && p.scaled) {
+        float* ks = p.c.k_scale + h * p.c.ks_sh;
+        float* vs = p.c.v_scale + h * p.c.vs_sh;
+        ks[to * p.c.ks_sp + st] = ks[from * p.c.ks_sp + sf];
+        vs[to * p.c.vs_sp + st] = vs[from * p.c.vs_sp + sf];
       }
     }
-    uint4 x[V];
+    __syncthreads();
+    for (int r0 = row0; r0 < rows; r0 += V * step) {
+      uint4 x[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (src[k]) x[k] = *reinterpret_cast<const uint4*>(src[k]);
+      for (int k = 0; k < V; ++k) {
+        const int r = r0 + k * step;
+        const int64_t from = r < rows ? s_from[value][r] : -1;
+        if (from >= 0) x[k] = *reinterpret_cast<const uint4*>(pool + from);
+      }
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (dst[k]) *reinterpret_cast<uint4*>(dst[k]) = x[k];
+      for (int k = 0; k < V; ++k) {
+        const int r = r0 + k * step;
+        if (r < rows && s_from[value][r] >= 0) *reinterpret_cast<uint4*>(pool + s_to[value][r]) = x[k];
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -519,7 +525,6 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   p.counts = static_cast<int*>(ws);
   p.moves = reinterpret_cast<int2*>(p.counts + (items + 3) / 4 * 4);
   p.max_moves = (int)compact_max_moves(cols, keep);
-  if (((int64_t)p.max_moves << (p.row16_log2 + 1)) > INT32_MAX - 65536) return TBF16_ERR_INVALID;
   // CTAs for an item: more while its slices are long and the items alone do not fill the SMs
   const int sms = tbf16_host::device_info()->sms;
   int ctas = 1;
@@ -535,7 +540,7 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
                                       p.in_smem ? (size_t)slice * 4 : 0, (unsigned)ctas, st, p))
     return rc;
   if (p.max_moves == 0) return TBF16_OK;
-  const int64_t blocks = (((int64_t)p.max_moves << (p.row16_log2 + 1)) + 1023) / 1024;
+  const int64_t blocks = (p.max_moves + kMoveRows - 1) / kMoveRows;
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(blocks, 8 * sms / items));
   return tbf16_host::launch_pdl(move_kernel, dim3((unsigned)items, (unsigned)splits), 256, 0, 1, st, p);
 }
