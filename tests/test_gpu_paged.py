@@ -358,7 +358,7 @@ def _plain_compact(case, w, pos, seen, keep, recent):
     ([0, 1, 31, 32, 33, 100, 257], 32, 8, "heavy"), ([300, 1000], 999, 0, "heavy"), ([300, 64], 1, 0, "heavy"),
     ([300, 64], 1, 1, "heavy"), ([500], 0, 0, "heavy"), ([500], 500, 10, "heavy"), ([700, 650], 600, 600, "heavy"),
     ([2500, 900], 800, 100, "ties"), ([5000], 2048, 16, "same"), ([400, 90], 77, 5, "odd"), ([5000, 33], 20, 15, "front"),
-    ([20000, 70000], 9000, 128, "heavy"), ([70001], 60000, 0, "ties")], ids=_ids)
+    ([20000, 70000], 9000, 128, "heavy"), ([70001], 60000, 0, "ties"), ([400001, 5], 399000, 7, "heavy")], ids=_ids)
 @pytest.mark.parametrize("D,bits,page,layout", [(64, 16, 16, "hnd"), (128, 8, 64, "nhd"), (256, 16, 32, "nhd"), (64, 8, 16, "hnd")])
 def test_compact(lens, keep, recent, kind, D, bits, page, layout):
     from tbf16 import _ext

@@ -194,6 +194,7 @@ struct CompactParams {
   int row16_log2;  // 16-byte chunks of a key or value row
   int scaled;
   int in_smem;     // a CTA's keys stay in shared memory
+  int inline_moves;  // select_kernel makes the moves itself
   float* w_out;
   int* pos_out;
   int* counts;     // moves of each (sequence, head)
@@ -215,33 +216,91 @@ constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kDigitBits = 11;  // keys are ranked by digits of 11, 11 and 10 bits: the first is sign, exponent and two
 constexpr int kBins = 1 << kDigitBits;  // bits of the weight, so that like weights still spread over several counters
 
-// Sum of v over the warps (one value per warp), the sum of the warps before this one, and the same over the CTAs of
-// the cluster: exclusive prefix of this warp over all warps of the cluster, in order of CTA and warp.
+// Exclusive prefix of a pair of counts (the same in all lanes of a warp) over the warps of the cluster, in order of
+// CTA and warp, and the totals.
 struct ClusterScan {
-  int* warp_sums;   // [kSelWarps]
-  int* cta_sum;     // one word that the other CTAs read
+  int2* warp_sums;  // [kSelWarps]
+  int2* cta_sum;    // one pair that the other CTAs read
   int ctas, rank;
-  __device__ int operator()(int v, int& total) const {
+  __device__ int2 operator()(int2 v, int2& total) const {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) warp_sums[warp] = v;
     __syncthreads();
-    const int x = lane < kSelWarps ? warp_sums[lane] : 0;
-    int before = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
-    total = __reduce_add_sync(0xffffffffu, x);
+    const int2 x = lane < kSelWarps ? warp_sums[lane] : make_int2(0, 0);
+    int2 before = sum(lane < warp ? x : make_int2(0, 0));
+    total = sum(x);
     if (ctas > 1) {
       if (threadIdx.x == 0) *cta_sum = total;
       cluster_sync();
-      int y = 0;
-      if (lane < ctas) asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(y) : "r"(mapa_u32(smem_u32(cta_sum), lane)));
-      before += __reduce_add_sync(0xffffffffu, lane < rank ? y : 0);
-      total = __reduce_add_sync(0xffffffffu, y);
-      cluster_sync();  // the word may be written again
+      int2 y = make_int2(0, 0);
+      if (lane < ctas)
+        asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(y.x), "=r"(y.y) : "r"(mapa_u32(smem_u32(cta_sum), lane)));
+      const int2 others = sum(lane < rank ? y : make_int2(0, 0));
+      before.x += others.x;
+      before.y += others.y;
+      total = sum(y);
+      cluster_sync();  // the pair may be written again, or its CTA end
     } else {
       __syncthreads();
     }
     return before;
   }
+  static __device__ int2 sum(int2 v) {
+    return make_int2(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y));
+  }
 };
+
+// Makes moves m0, m0 + kMoveRows * stride, ... of an item: looks up the pages of kMoveRows moves (and does their
+// scales, weights and numbers), then streams the rows, 16 bytes a thread, V loads in flight.
+constexpr int kMoveRows = 64;
+struct MoveScratch {
+  int64_t from[2][kMoveRows], to[2][kMoveRows];  // byte offsets of keys, values; -1: not to be copied
+};
+template <int THREADS, int V>
+__device__ __forceinline__ void move_rows(const CompactParams& p, int bh, int count, int m0, int stride, MoveScratch& s) {
+  const int b = bh / p.c.heads, h = bh % p.c.heads, tid = threadIdx.x;
+  const int chunk = tid & ((1 << p.row16_log2) - 1), value = (tid >> p.row16_log2) & 1;
+  uint8_t* pool = (value ? p.c.v + h * p.c.v_sh : p.c.k + h * p.c.k_sh) + chunk * 16;
+  const int row0 = tid >> (p.row16_log2 + 1), step = THREADS >> (p.row16_log2 + 1);  // rows of a pass
+  for (m0 *= kMoveRows; m0 < count; m0 += stride * kMoveRows) {
+    const int rows = min(kMoveRows, count - m0);
+    if (tid < rows) {
+      const int2 mv = p.moves[(int64_t)bh * p.max_moves + m0 + tid];
+      const int from = paged_page(p.c, b, mv.x), to = paged_page(p.c, b, mv.y);
+      const int sf = paged_slot(p.c, mv.x), st = paged_slot(p.c, mv.y);
+      const int64_t out = (int64_t)bh * p.cols + mv.y;
+      p.w_out[out] = p.w[b * p.w_sb + h * p.w_sh + mv.x];
+      p.pos_out[out] = p.pos[b * p.p_sb + h * p.p_sh + mv.x];
+      const bool ok = from >= 0 && to >= 0;
+      s.from[0][tid] = ok ? from * p.c.k_sp + sf * p.c.k_ss : -1;
+      s.from[1][tid] = ok ? from * p.c.v_sp + sf * p.c.v_ss : -1;
+      s.to[0][tid] = to * p.c.k_sp + st * p.c.k_ss;
+      s.to[1][tid] = to * p.c.v_sp + st * p.c.v_ss;
+      if (ok && p.scaled) {
+        float* ks = p.c.k_scale + h * p.c.ks_sh;
+        float* vs = p.c.v_scale + h * p.c.vs_sh;
+        ks[to * p.c.ks_sp + st] = ks[from * p.c.ks_sp + sf];
+        vs[to * p.c.vs_sp + st] = vs[from * p.c.vs_sp + sf];
+      }
+    }
+    __syncthreads();
+    for (int r0 = row0; r0 < rows; r0 += V * step) {
+      uint4 x[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int r = r0 + k * step;
+        const int64_t from = r < rows ? s.from[value][r] : -1;
+        if (from >= 0) x[k] = *reinterpret_cast<const uint4*>(pool + from);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int r = r0 + k * step;
+        if (r < rows && s.from[value][r] >= 0) *reinterpret_cast<uint4*>(pool + s.to[value][r]) = x[k];
+      }
+    }
+    __syncthreads();
+  }
+}
 
 // A cluster of 1 to 8 CTAs per (sequence, head), each with an equal slice of the positions, whose rank keys it keeps
 // in shared memory. The keep-th largest key comes from a radix select over the slices' histograms (read through
@@ -250,7 +309,9 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   extern __shared__ uint32_t keys[];
   __shared__ __align__(16) int hist[kBins];
   __shared__ int warp_sums[kSelWarps];
-  __shared__ int cta_sum, s_digit, s_need;
+  __shared__ int2 scan_sums[kSelWarps], cta_sum;
+  __shared__ int s_digit, s_need, s_equal;
+  __shared__ MoveScratch scratch;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int ctas;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
@@ -271,7 +332,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
       w_out[i] = w[i];
       pos_out[i] = pos[i];
     }
-    if (rank == 0 && tid == 0) p.counts[bh] = 0;
+    if (!p.inline_moves && rank == 0 && tid == 0) p.counts[bh] = 0;
     return;
   }
   const int protect_from = p.seen[b] - p.recent;
@@ -281,7 +342,8 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   auto key_at = [&](int i) { return p.in_smem ? keys[i - lo] : rank_key(w[i], pos[i], protect_from); };
   uint32_t prefix = 0;
   int need = p.keep;
-  const ClusterScan scan{warp_sums, &cta_sum, ctas, rank};
+  int equal = 0;  // positions whose key is the need-th largest
+  const ClusterScan scan{scan_sums, &cta_sum, ctas, rank};
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
@@ -353,6 +415,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
       if (above < need && need <= above + bin[k]) {
         s_digit = kBins - 1 - (tid * PB + k);
         s_need = need - above;
+        s_equal = bin[k];
       }
       above += bin[k];
     }
@@ -360,95 +423,75 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
     else __syncthreads();
     prefix |= (uint32_t)s_digit << shift;
     need = s_need;
+    equal = s_equal;
   }
-  // `need` of the positions whose key equals `prefix` are kept, the lowest first
-  int ties = 0, total;
-  for (int i = first + lane; i - lane < last; i += 32)
-    ties += __popc(__ballot_sync(0xffffffffu, i < last && key_at(i) == prefix));
-  const int ties_before = scan(ties, total);
+  // `need` of the positions whose key equals `prefix` are kept, the lowest first: where that is not all of them, each
+  // warp has to know how many come before its own
+  int2 total;
+  int ties_before = 0;
+  if (equal == need) {
+    need = INT_MAX;
+  } else {
+    int ties = 0;
+    for (int i = first + lane; i - lane < last; i += 32)
+      ties += __popc(__ballot_sync(0xffffffffu, i < last && key_at(i) == prefix));
+    ties_before = scan(make_int2(ties, 0), total).x;
+  }
   int2* moves = p.moves + (int64_t)bh * p.max_moves;
-  int holes_before = 0, loose_before = 0;
+  int2 before = make_int2(0, 0);  // holes, and kept positions at or beyond `keep`, in the warps before this one
 #pragma unroll 1
   for (int write = 0; write < 2; ++write) {
-    int tie = ties_before, holes = holes_before, loose = loose_before;
-    for (int i = first + lane; i - lane < last; i += 32) {
-      const bool in = i < last;
-      const uint32_t key = in ? key_at(i) : 0u;
-      const unsigned below = (1u << lane) - 1, eq = __ballot_sync(0xffffffffu, in && key == prefix);
-      const bool kept = in && (key > prefix || (key == prefix && tie + __popc(eq & below) < need));
-      tie += __popc(eq);
-      const unsigned hb = __ballot_sync(0xffffffffu, in && !kept && i < p.keep);
-      const unsigned lb = __ballot_sync(0xffffffffu, kept && i >= p.keep);
-      if (write) {
-        if ((hb >> lane) & 1) moves[holes + __popc(hb & below)].y = i;
-        if ((lb >> lane) & 1) moves[loose + __popc(lb & below)].x = i;
-        if (kept && i < p.keep) {
-          w_out[i] = w[i];
-          pos_out[i] = pos[i];
+    int tie = ties_before, holes = before.x, loose = before.y;
+    for (int i0 = first; i0 < last; i0 += 128) {
+      float x[4];
+      int y[4];
+      uint32_t key[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * 32 + lane;
+        key[k] = i < last ? key_at(i) : 0u;
+        if (write && i < min(last, p.keep)) {
+          x[k] = w[i];
+          y[k] = pos[i];
         }
       }
-      holes += __popc(hb);
-      loose += __popc(lb);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * 32 + lane;
+        const bool in = i < last;
+        const unsigned below = (1u << lane) - 1, eq = __ballot_sync(0xffffffffu, in && key[k] == prefix);
+        const bool kept = in && (key[k] > prefix || (key[k] == prefix && tie + __popc(eq & below) < need));
+        tie += __popc(eq);
+        const unsigned hb = __ballot_sync(0xffffffffu, in && !kept && i < p.keep);
+        const unsigned lb = __ballot_sync(0xffffffffu, kept && i >= p.keep);
+        if (write) {
+          if ((hb >> lane) & 1) moves[holes + __popc(hb & below)].y = i;
+          if ((lb >> lane) & 1) moves[loose + __popc(lb & below)].x = i;
+          if (kept && i < p.keep) {
+            w_out[i] = x[k];
+            pos_out[i] = y[k];
+          }
+        }
+        holes += __popc(hb);
+        loose += __popc(lb);
+      }
     }
-    if (!write) {
-      holes_before = scan(holes, total);
-      loose_before = scan(loose, total);
-      if (rank == 0 && tid == 0) p.counts[bh] = total;
-    }
+    if (!write) before = scan(make_int2(holes, loose), total);
+  }
+  if (p.inline_moves) {  // one CTA, few moves: made here
+    __syncthreads();
+    move_rows<kSelThreads, 4>(p, bh, total.x, 0, 1, scratch);
+  } else if (rank == 0 && tid == 0) {
+    p.counts[bh] = total.x;
   }
 }
 
-// Copies the listed rows; grid (items, splits of an item's moves). A block looks up the pages of kMoveRows moves (and
-// does their scales, weights and numbers), then streams the rows, 16 bytes a thread, eight loads in flight.
-constexpr int kMoveRows = 64;
+// Makes the listed moves; grid (items, splits of an item's moves).
 __global__ void __launch_bounds__(256) move_kernel(const CompactParams p) {
-  constexpr int V = 8;
-  __shared__ int64_t s_from[2][kMoveRows], s_to[2][kMoveRows];  // byte offsets of keys, values; -1: not to be copied
+  __shared__ MoveScratch scratch;
   pdl_launch_dependents();
   pdl_wait();
-  const int bh = blockIdx.x, b = bh / p.c.heads, h = bh % p.c.heads, tid = threadIdx.x;
-  const int count = p.counts[bh], chunk = tid & ((1 << p.row16_log2) - 1);
-  const bool value = (tid >> p.row16_log2) & 1;
-  uint8_t* pool = (value ? p.c.v + h * p.c.v_sh : p.c.k + h * p.c.k_sh) + chunk * 16;
-  const int row0 = tid >> (p.row16_log2 + 1), step = 256 >> (p.row16_log2 + 1);  // rows of a pass: 4 to 32
-  for (int m0 = blockIdx.y * kMoveRows; m0 < count; m0 += gridDim.y * kMoveRows) {
-    const int rows = min(kMoveRows, count - m0);
-    if (tid < rows) {
-      const int2 mv = p.moves[(int64_t)bh * p.max_moves + m0 + tid];
-      const int from = paged_page(p.c, b, mv.x), to = paged_page(p.c, b, mv.y);
-      const int sf = paged_slot(p.c, mv.x), st = paged_slot(p.c, mv.y);
-      const int64_t out = (int64_t)bh * p.cols + mv.y;
-      p.w_out[out] = p.w[b * p.w_sb + h * p.w_sh + mv.x];
-      p.pos_out[out] = p.pos[b * p.p_sb + h * p.p_sh + mv.x];
-      const bool ok = from >= 0 && to >= 0;
-      s_from[0][tid] = ok ? from * p.c.k_sp + sf * p.c.k_ss : -1;
-      s_from[1][tid] = ok ? from * p.c.v_sp + sf * p.c.v_ss : -1;
-      s_to[0][tid] = to * p.c.k_sp + st * p.c.k_ss;
-      s_to[1][tid] = to * p.c.v_sp + st * p.c.v_ss;
-      if (ok && p.scaled) {
-        float* ks = p.c.k_scale + h * p.c.ks_sh;
-        float* vs = p.c.v_scale + h * p.c.vs_sh;
-        ks[to * p.c.ks_sp + st] = ks[from * p.c.ks_sp + sf];
-        vs[to * p.c.vs_sp + st] = vs[from * p.c.vs_sp + sf];
-      }
-    }
-    __syncthreads();
-    for (int r0 = row0; r0 < rows; r0 += V * step) {
-      uint4 x[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int r = r0 + k * step;
-        const int64_t from = r < rows ? s_from[value][r] : -1;
-        if (from >= 0) x[k] = *reinterpret_cast<const uint4*>(pool + from);
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int r = r0 + k * step;
-        if (r < rows && s_from[value][r] >= 0) *reinterpret_cast<uint4*>(pool + s_to[value][r]) = x[k];
-      }
-    }
-    __syncthreads();
-  }
+  move_rows<256, 8>(p, blockIdx.x, p.counts[blockIdx.x], blockIdx.y, gridDim.y, scratch);
 }
 
 }  // namespace
@@ -525,21 +568,24 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   p.counts = static_cast<int*>(ws);
   p.moves = reinterpret_cast<int2*>(p.counts + (items + 3) / 4 * 4);
   p.max_moves = (int)compact_max_moves(cols, keep);
-  // CTAs for an item: more while its slices are long and the items alone do not fill the SMs
+  // CTAs for an item: more while its slices are long and the SMs not full. A cluster's barriers and remote reads cost
+  // about 9 us, which slices of 4096 positions and more win back (128 items of 2112: 17 us with one CTA, 26 with two;
+  // 64 of 16000: 65 / 52 / 50 with 1 / 2 / 4; 8 of 36156: 79 / 52 / 36 / 32 with 1 / 2 / 4 / 8).
   const int sms = tbf16_host::device_info()->sms;
   int ctas = 1;
-  while (ctas < 8 && (cols + ctas - 1) / ctas > 2048 && items * ctas * 2 <= 2 * sms) ctas *= 2;
+  while (ctas < 8 && (cols + ctas - 1) / ctas > 4096 && items * ctas * 2 <= 2 * sms) ctas *= 2;
   constexpr int kMaxKeys = 48 * 1024;
   while (ctas < 8 && (cols + ctas - 1) / ctas > kMaxKeys) ctas *= 2;
   const int64_t slice = (cols + ctas - 1) / ctas;
   p.in_smem = slice <= kMaxKeys;
+  p.inline_moves = ctas == 1 && p.max_moves <= 2 * kMoveRows;
   static const cudaError_t attr = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
   if (attr != cudaSuccess || items * ctas > INT32_MAX) return TBF16_ERR_LAUNCH;
   auto st = static_cast<cudaStream_t>(stream);
   if (int rc = tbf16_host::launch_pdl(select_kernel, dim3((unsigned)(items * ctas)), kSelThreads,
                                       p.in_smem ? (size_t)slice * 4 : 0, (unsigned)ctas, st, p))
     return rc;
-  if (p.max_moves == 0) return TBF16_OK;
+  if (p.inline_moves) return TBF16_OK;
   const int64_t blocks = (p.max_moves + kMoveRows - 1) / kMoveRows;
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(blocks, 8 * sms / items));
   return tbf16_host::launch_pdl(move_kernel, dim3((unsigned)items, (unsigned)splits), 256, 0, 1, st, p);
