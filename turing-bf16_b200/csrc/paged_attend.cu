@@ -861,31 +861,45 @@ __global__ void __launch_bounds__(C::W * 32, 1)
 }
 
 // weights[b, h, j] += sum_r e^(s_rj - log-sum_r) over the head's query rows, from the logits the attention left
-// (fp32, 4 rows bytes a position: a few per cent of the cache's own bytes) and its row sums. Four positions a thread.
-__global__ void __launch_bounds__(256) weights_kernel(const AttendParams p, float* weights, int64_t w_sb, int64_t w_sh,
-                                                      int block_keys) {
+// (fp32, 4 rows bytes a position, where the cache has 2 D to 4 D) and its row sums. Two positions a thread, eight rows
+// in flight: with few sequences there are few threads, and each has all rows to go through.
+constexpr int kWeightThreads = 128;
+__global__ void __launch_bounds__(kWeightThreads) weights_kernel(const AttendParams p, float* weights, int64_t w_sb, int64_t w_sh,
+                                                                 int block_keys) {
+  constexpr int SPAN = kWeightThreads * 2, V = 8;
+  pdl_launch_dependents();
   pdl_wait();
-  const int per = (p.c.cap + 1023) / 1024;
-  for (int x = blockIdx.x; x < p.c.batch * p.c.heads * per; x += gridDim.x) {
-    const int bh = x / per, b = bh / p.c.heads, h = bh % p.c.heads;
+  const int per = (p.c.cap + SPAN - 1) / SPAN;
+  for (int64_t x = blockIdx.x; x < (int64_t)p.c.batch * p.c.heads * per; x += gridDim.x) {
+    const int bh = (int)(x / per), b = bh / p.c.heads, h = bh - b * p.c.heads;
     const int len = paged_len(p.c, b), n = paged_count(p.c, p.counts, b, p.T, len);
     const int lo = p.window ? max(0, len - n + 1 - p.window) / block_keys * block_keys : 0;
-    const int j = (x % per) * 1024 + threadIdx.x * 4;
-    if (n == 0 || j + 3 < lo || j >= len) continue;
+    const int j = (int)(x - (int64_t)bh * per) * SPAN + threadIdx.x * 2;
+    if (n == 0 || j + 1 < lo || j >= len) continue;
     const float* logits = p.logits + (int64_t)bh * p.rows * p.c.cap + j;
     const float* lse = p.lse + (int64_t)bh * p.rows;
-    float a[4] = {};
-    for (int r = 0; r < n * p.group; ++r) {
-      const float4 v = *reinterpret_cast<const float4*>(logits + (int64_t)r * p.c.cap);
-      const float z = lse[r], vs[4] = {v.x, v.y, v.z, v.w};
-      if (z == -INFINITY) continue;  // a row that sees nothing
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] += j + i < len ? ex2(vs[i] - z) : 0.f;
-    }
     float* w = weights + b * w_sb + h * w_sh + j;
+    const float old[2] = {w[0], j + 1 < len ? w[1] : 0.f};
+    float a[2] = {};
+    const int rows = n * p.group;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += V) {
+      float2 v[V];
+      float z[V];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (j + i >= lo && j + i < len) w[i] += a[i];
+      for (int k = 0; k < V; ++k) {
+        z[k] = r0 + k < rows ? lse[r0 + k] : -INFINITY;
+        if (r0 + k < rows) v[k] = *reinterpret_cast<const float2*>(logits + (int64_t)(r0 + k) * p.c.cap);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if (z[k] == -INFINITY) continue;  // past the rows, or a row that sees nothing
+        a[0] += ex2(v[k].x - z[k]);
+        a[1] += ex2(v[k].y - z[k]);
+      }
+    }
+    if (j >= lo) w[0] = old[0] + a[0];
+    if (j + 1 >= lo && j + 1 < len) w[1] = old[1] + a[1];
   }
 }
 
@@ -1014,7 +1028,8 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   else rc = e4m3 ? launch_rows<256, true>(cache, p, dev->sms, st) : launch_rows<256, false>(cache, p, dev->sms, st);
   if (rc != TBF16_OK || !weights) return rc;
   const int block_keys = cache->D * (e4m3 ? 1 : 2) <= 64 ? 64 : cache->D * (e4m3 ? 1 : 2) <= 128 ? 32 : 16;
-  const int64_t blocks = cache->batch * cache->heads * ((p.c.cap + 1023) / 1024);
-  return tbf16_host::launch_pdl(weights_kernel, (unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 8), 256, 0, 1, st, p, weights, w_sb,
+  const int span = kWeightThreads * 2;
+  const int64_t blocks = cache->batch * cache->heads * ((p.c.cap + span - 1) / span);
+  return tbf16_host::launch_pdl(weights_kernel, (unsigned)std::min<int64_t>(blocks, (int64_t)dev->sms * 16), kWeightThreads, 0, 1, st, p, weights, w_sb,
                     w_sh, block_keys);
 }

@@ -328,13 +328,16 @@ class PagedCache:
         if keep < 0 or recent < 0:
             raise RuntimeError("tbf16.PagedCache.compact: keep and recent must not be negative")
         cols = c.weights.shape[2]
-        weights = torch.empty(c.weights.shape, device=self.device)
-        pos = torch.empty(c.pos.shape, device=self.device, dtype=torch.int32)
-        n = int(self._lib.tbf16_paged_compact_ws_size(c.ref, cols, keep))
-        ws = torch.empty(n, device=self.device, dtype=torch.uint8)
+        size = self._sizes.get(keep)
+        if size is None:
+            size = self._sizes[keep] = int(self._lib.tbf16_paged_compact_ws_size(c.ref, cols, keep))
+        shape = c.weights.shape
+        weights = torch.empty(shape, device=self.device)
+        pos = torch.empty(shape, device=self.device, dtype=torch.int32)
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        buf = self._scratch(stream, 0, size)
         self._run(self._lib.tbf16_paged_compact, "compact", c.ref, *c.weight_args, *c.pos_args[:3], cols, c.pos_args[3], keep,
-                  recent, weights.data_ptr(), pos.data_ptr(), ws.data_ptr(), n,
-                  torch._C._cuda_getCurrentRawStream(self.device.index))
+                  recent, weights.data_ptr(), pos.data_ptr(), buf.data_ptr() + buf.sync, size, stream)
         return weights, pos
 
     def evict(self, keep, recent=0):
