@@ -205,6 +205,11 @@ def test_attend_layouts(bits):
     packed[..., 3:3 + 8 * 64] = q.transpose(1, 2).flatten(2)
     assert torch.equal(cache.attend(packed[..., 3:3 + 8 * 64].unflatten(-1, (8, 64)).transpose(1, 2)), ref)
     assert torch.equal(cache.attend(q.contiguous()), ref)
+    one = Case([100], 4, 64, 16, bits)  # one sequence, one token: strides of a packed row that is no multiple of 8
+    q1 = one.queries(8, 1)
+    odd = torch.zeros(1, 1, 8 * 64 + 3, device=DEV, dtype=torch.bfloat16)
+    odd[..., :8 * 64] = q1.transpose(1, 2).flatten(2)
+    assert torch.equal(one.cache().attend(odd[..., :8 * 64].unflatten(-1, (8, 64)).transpose(1, 2)), one.cache().attend(q1))
     assert ref.transpose(1, 2).is_contiguous()  # (B, T, heads, D) memory for the output projection
     assert _ext.device_status() == 0
 

@@ -46,9 +46,8 @@ def _rows(x, name, B, H, d, device):
         raise RuntimeError(f"tbf16.PagedCache: {name} requires grad; the cache is for inference (use torch.no_grad)")
     sb, sh, st, se = x.stride()
     if se != 1 or (sb | sh | st) & 7 or d & 7 or x.data_ptr() & 15:
-        x = torch.nn.functional.pad(x, (0, -d % 8)).contiguous() if d % 8 else x.contiguous()
-        if x.data_ptr() & 15:
-            x = x.clone()
+        # clone: also rewrites odd strides of dimensions of one element, which count as contiguous
+        x = torch.nn.functional.pad(x, (0, -d % 8)) if d % 8 else x.clone(memory_format=torch.contiguous_format)
     return x
 
 
@@ -121,7 +120,8 @@ class PagedCache:
     max_len). track=True keeps `weights` (fp32, attention weight summed over the queries so far) and `pos`
     (int32, the token's number in its sequence), both (layers, batch, kv_heads, capacity), for `evict`.
 
-    lens / seen / table are device tensors: cached tokens, tokens ever appended, page numbers. Different streams may work on one cache if the caller orders their accesses."""
+    lens / seen / table are device tensors: cached tokens, tokens ever appended, page numbers. Different streams may
+    work on one cache if the caller orders their accesses."""
 
     def __init__(self, batch, kv_heads, head_dim, max_len, *, layers=1, pages=None, page_size=64,
                  dtype=torch.bfloat16, track=False, device="cuda"):
@@ -133,8 +133,8 @@ class PagedCache:
         pages = batch * per if pages is None else pages
         D = _kernel_dim(head_dim)
         dev = torch.device(device)
-        k = torch.zeros((2, layers, pages, kv_heads, page_size, D), device=dev, dtype=torch.uint8 if dtype != torch.bfloat16 else dtype)
-        k, v = k.view(dtype).unbind(0)
+        raw = torch.bfloat16 if dtype == torch.bfloat16 else torch.uint8
+        k, v = torch.zeros((2, layers, pages, kv_heads, page_size, D), device=dev, dtype=raw).view(dtype).unbind(0)
         ks = vs = None
         if dtype != torch.bfloat16:
             ks, vs = torch.ones((2, layers, pages, kv_heads, page_size), device=dev).unbind(0)
@@ -142,8 +142,8 @@ class PagedCache:
         shape = (layers, batch, kv_heads, per * page_size)
         weights = torch.zeros(shape, device=dev) if track else None
         pos = torch.full(shape, -1, **ints) if track else None
-        self._init(k, v, ks, vs, torch.zeros((batch, per), **ints), torch.zeros(batch, **ints),
-                   torch.zeros(batch, **ints) if track else None, weights, pos, head_dim)
+        self._state = torch.zeros((2, batch), **ints)  # lens, seen
+        self._init(k, v, ks, vs, torch.zeros((batch, per), **ints), *self._state.unbind(0), weights, pos, head_dim)
         self.pool = PagePool(batch, pages, page_size, max_len)
 
     @classmethod
@@ -229,12 +229,12 @@ class PagedCache:
         self._upload(table=False)
 
     def _upload(self, table):
-        ints = dict(dtype=torch.int32)
-        self.lens.copy_(torch.tensor(self.pool.lengths, **ints))
-        if self.seen is not None:
-            self.seen.copy_(torch.tensor(self.pool.seen, **ints))
+        """lens, seen and, where it changed, the table to the GPU, in stream order and without waiting for it: from
+        pinned memory that torch's allocator does not hand out again before the copy is done."""
+        pinned = dict(dtype=torch.int32, pin_memory=True)
+        self._state.copy_(torch.tensor([self.pool.lengths, self.pool.seen], **pinned), non_blocking=True)
         if table:
-            self.table.copy_(torch.tensor(self.pool.rows(self.table.shape[1]), **ints))
+            self.table.copy_(torch.tensor(self.pool.rows(self.table.shape[1]), **pinned), non_blocking=True)
 
     def _counts(self, counts):
         if counts is None:
