@@ -27,7 +27,10 @@ using namespace tbf16;
 // O^T = V^T P^T. With the usual group of up to eight query rows no product is wasted on empty rows (a 16-row
 // query tile would waste half of them, tcgen05's 128 rows fifteen sixteenths), a lane holds four weights per 16
 // keys, and P^T gets from accumulator to operand layout by one 8x8 transpose per 8 keys.
-constexpr int kMaxStages = 8;
+// Stages of a warp: 128 KB in flight on an SM. More of it makes the queues in front of the memory longer, not the rate
+// higher, and the SMs' rates more uneven, so the last one ends later (131071 tokens, all SMs with equal shares: they
+// end after 72 to 82 us with two stages and after 65 to 92 with three; one stage 104 us in all, two 97, three 101).
+constexpr int kMaxStages = 2;
 
 template <int D_, bool E4M3_, int NQ_>
 struct Tile {
@@ -141,6 +144,11 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* m, uin
       "[%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
+}
+__device__ __forceinline__ unsigned count_up(unsigned* word) {
+  unsigned n;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(word) : "memory");
+  return n;
 }
 // Over the eight lanes that hold one column of an accumulator.
 __device__ __forceinline__ float column_max(float v) {
@@ -265,7 +273,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   __shared__ uint64_t bars[W * kMaxStages];
   __shared__ float2 s_ms[W * R];       // each warp's (maximum, sum) of a row
   __shared__ float2 s_team[NTHREADS];  // that of a row in each thread group of a join
-  __shared__ int s_scan[W], s_work[W], s_abort, s_todo;
+  __shared__ int s_scan[W], s_work[W], s_long[W], s_abort, s_todo;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((smem_u32(smem) & 1023u) != 0) {
     if (tid == 0) atomicOr(p.c.err, kErrSmemAlign);
@@ -282,15 +290,15 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   pdl_wait();
 
   // Every sequence's blocks and rounds (a round: a block for each warp) and their running totals.
-  int total = 0, work = 0;
+  int total = 0, work = 0, longest = 0;
   for (int b0 = 0; b0 < p.c.batch; b0 += NTHREADS) {
     const int b = b0 + tid;
     SeqInfo s{0, 0, 0, 0};
-    int x = 0, y = 0;
+    int x = 0, y = 0, blocks = 0;
     if (b < p.c.batch) {
       s.len = paged_len(p.c, b);
       s.count = paged_count(p.c, p.counts, b, p.T, s.len);
-      const int blocks = item_blocks<C>(p, s.len, s.count);
+      blocks = item_blocks<C>(p, s.len, s.count);
       x = blocks * p.c.heads * p.chunks;
       y = (blocks + W - 1) / W * p.c.heads * p.chunks;
     }
@@ -300,9 +308,11 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       const int dx = __shfl_up_sync(0xffffffffu, x, o), dy = __shfl_up_sync(0xffffffffu, y, o);
       if (lane >= o) x += dx, y += dy;
     }
+    blocks = __reduce_max_sync(0xffffffffu, blocks);
     if (lane == 31) {
       s_scan[warp] = x;
       s_work[warp] = y;
+      s_long[warp] = blocks;
     }
     __syncthreads();
     x += total - my_x;
@@ -312,6 +322,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       if (i < warp) x += s_scan[i], y += s_work[i];
       total += s_scan[i];
       work += s_work[i];
+      longest = max(longest, s_long[i]);
     }
     s.cum = x;
     s.rounds = y;
@@ -321,8 +332,12 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   }
   // Few rounds: a CTA takes one, so no item waits for another. Else CTA i takes blocks [share(i), share(i + 1)):
   // `each` of them, the first `more` CTAs one more.
+  // Sequences of one length with few items: as many CTAs for each item, as long as that leaves out no more than one in
+  // twenty; a CTA with the end of one item and the start of the next would have two partials to add up at the end.
   const bool by_round = work <= (int)gridDim.x;
-  const int ctas = by_round ? work : (int)gridDim.x;
+  const int items = p.c.batch * p.c.heads * p.chunks, level = items <= (int)gridDim.x ? gridDim.x / items * items : 0;
+  const bool even = level * 20 >= (int)gridDim.x * 19 && longest * items == total;
+  const int ctas = by_round ? work : even ? level : (int)gridDim.x;
   if ((int)blockIdx.x >= ctas) return;
   const int each = total / ctas, more = total - each * ctas;
   auto share = [&](int i) { return each * i + min(i, more); };
@@ -402,12 +417,12 @@ __global__ void __launch_bounds__(C::W * 32, 1)
         // Only now the CTA says that its partials are out, so that no item of its own waited for a join. The last
         // of an item's CTAs to say so joins the item.
         if (tid == 0) {
-          __threadfence();  // with the barrier before: every thread's partials, before the counts
+          // acquire and release; with the barrier before, every thread's partials come before the counts
+          const unsigned n0 = open0 >= 0 ? count_up(p.sync + word0) : 0, n1 = open1 >= 0 ? count_up(p.sync + word1) : 0;
           int mine = 0;
-          if (open0 >= 0 && atomicAdd(p.sync + word0, 1u) == (unsigned)parts0 - 1) mine = 1, p.sync[word0] = 0;
-          if (open1 >= 0 && atomicAdd(p.sync + word1, 1u) == (unsigned)parts1 - 1) mine |= 2, p.sync[word1] = 0;
+          if (open0 >= 0 && n0 == (unsigned)parts0 - 1) mine = 1, p.sync[word0] = 0;
+          if (open1 >= 0 && n1 == (unsigned)parts1 - 1) mine |= 2, p.sync[word1] = 0;
           s_todo = mine;
-          __threadfence();
         }
         __syncthreads();
         todo = s_todo;
@@ -938,15 +953,16 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   return tbf16_host::launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, 1, st, km, vm, p);
 }
 
-// Query rows of an item: as many tiles of eight as the head's rows fill, up to four (two for D = 256, whose output
-// would not fit the registers): each cached byte is then read once for all of them.
-int item_rows(int64_t D, int64_t rows) { return rows <= 8 ? 8 : rows <= 16 || D == 256 ? 16 : 32; }
+// Query rows of an item. Heads with more rows make several items of the same keys, which run at the same time and find
+// them in L2: 32 rows in one item (four tiles; registers spill, and the merge area leaves a single stage) took 100 us
+// where two items take 62 (8 sequences of 32768 tokens, 32 query heads on one key/value head of 128).
+int item_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
 
 struct Workspace {
   int64_t rows, chunks, nr, part, lse, logits;  // sizes in floats, in this order
   Workspace(const tbf16_paged_cache* c, int64_t Hq, int64_t T, bool weights, int sms) {
     rows = T * (Hq / c->heads);
-    const int R = item_rows(c->D, rows);
+    const int R = item_rows(rows);
     chunks = (rows + R - 1) / R;
     nr = std::min<int64_t>(rows, R);
     part = 2 * (int64_t)sms * partial_floats((int)nr, (int)c->D);
@@ -958,11 +974,8 @@ struct Workspace {
 
 template <int D, bool E4M3>
 int launch_rows(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
-  const int R = item_rows(D, p.rows);
-  if (R == 8) return launch_attend<Tile<D, E4M3, 1>>(cache, p, sms, st);
-  if constexpr (D < 256)
-    if (R == 32) return launch_attend<Tile<D, E4M3, 4>>(cache, p, sms, st);
-  return launch_attend<Tile<D, E4M3, 2>>(cache, p, sms, st);
+  return item_rows(p.rows) == 8 ? launch_attend<Tile<D, E4M3, 1>>(cache, p, sms, st)
+                                : launch_attend<Tile<D, E4M3, 2>>(cache, p, sms, st);
 }
 
 bool attend_sizes_ok(const tbf16_paged_cache* c, int64_t Hq, int64_t T) {
