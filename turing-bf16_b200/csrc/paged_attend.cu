@@ -74,20 +74,24 @@ struct AttendParams {
 // Floats of a partial: nr rows of outputs, then of (maximum, sum) pairs, to a multiple of 16 bytes.
 __host__ __device__ constexpr int partial_floats(int nr, int D) { return (nr * (D + 2) + 3) / 4 * 4; }
 
+// In the order of all blocks each item is followed by kPad places that hold none: what an item costs a CTA beyond its
+// blocks (loading its queries, waiting for its last warp, adding the warps up), so that CTAs with many short items get
+// fewer keys.
+constexpr int kPad = 24;
+
 // What a CTA knows of a sequence: the first of its blocks, and of its rounds, among all; cached and new tokens.
 struct SeqInfo {
   int cum, rounds, len, count;
 };
 
-// First block that a sequence's window reaches, and the blocks of one of its items (one empty block writes an
-// idle sequence's zeros).
+// First block that a sequence's window reaches, and the blocks of one of its items (none without new tokens).
 template <class C>
 __device__ __forceinline__ int first_block(const AttendParams& p, int len, int count) {
   return p.window ? max(0, len - count + 1 - p.window) / C::BK : 0;
 }
 template <class C>
 __device__ __forceinline__ int item_blocks(const AttendParams& p, int len, int count) {
-  return count ? (len + C::BK - 1) / C::BK - first_block<C>(p, len, count) : 1;
+  return count ? (len + C::BK - 1) / C::BK - first_block<C>(p, len, count) : 0;
 }
 __device__ __forceinline__ int token_of(const AttendParams& p, int row) {
   return p.group == 1 ? row : (int)__umulhi((unsigned)row, p.group_inv);
@@ -207,11 +211,11 @@ struct Loader {
       if (t >= end) return;
       while (t >= info[u.b + 1].cum) ++u.b;
       const SeqInfo s = info[u.b];
-      if (s.count == 0) continue;
       u.blocks = item_blocks<C>(p, s.len, s.count);
-      const unsigned rem = t - s.cum, item = rem / (unsigned)u.blocks;
+      const unsigned rem = t - s.cum, item = rem / (unsigned)(u.blocks + kPad);
       u.h = p.chunks == 1 ? (int)item : (int)(item / (unsigned)p.chunks);
-      u.blk = (int)(rem - item * u.blocks);
+      u.blk = (int)(rem - item * (u.blocks + kPad));
+      if (u.blk >= u.blocks) continue;
       u.j0 = (first_block<C>(p, s.len, s.count) + u.blk) * C::BK;
       u.len = s.len;
       break;
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       s.len = paged_len(p.c, b);
       s.count = paged_count(p.c, p.counts, b, p.T, s.len);
       blocks = item_blocks<C>(p, s.len, s.count);
-      x = blocks * p.c.heads * p.chunks;
+      x = blocks ? (blocks + kPad) * p.c.heads * p.chunks : 0;
       y = (blocks + W - 1) / W * p.c.heads * p.chunks;
     }
     const int my_x = x, my_y = y;
@@ -338,13 +342,28 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   // Sequences of one length with few items: as many CTAs for each item, as long as that leaves out no more than one in
   // twenty; a CTA with the end of one item and the start of the next would have two partials to add up at the end.
   const bool by_round = work <= (int)gridDim.x;
-  const int items = p.c.batch * p.c.heads * p.chunks, level = items <= (int)gridDim.x ? gridDim.x / items * items : 0;
-  const bool even = level * 20 >= (int)gridDim.x * 19 && longest * items == total;
-  const int ctas = by_round ? work : even ? level : (int)gridDim.x;
+  const int items = p.c.batch * p.c.heads * p.chunks, per_item = items <= (int)gridDim.x ? gridDim.x / items : 0;
+  const bool even = !by_round && per_item * items * 20 >= (int)gridDim.x * 19 && (longest + kPad) * items == total;
+  const int ctas = by_round ? work : even ? per_item * items : (int)gridDim.x;
+  // sequences without new tokens: zeros
+  for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x) {
+    if (info[b].count) continue;
+    const int heads = p.c.heads * p.group;
+    for (int i = tid; i < heads * p.T * (D / 8); i += NTHREADS) {
+      const int row = i / (D / 8), t = row / heads;
+      *reinterpret_cast<uint4*>(p.out + b * p.o_sb + (int64_t)(row - t * heads) * p.o_sh + t * p.o_st + i % (D / 8) * 8) =
+          make_uint4(0, 0, 0, 0);
+    }
+  }
   if ((int)blockIdx.x >= ctas) return;
   const int each = total / ctas, more = total - each * ctas;
   auto share = [&](int i) { return each * i + min(i, more); };
   int c0 = share(blockIdx.x), c1 = share(blockIdx.x + 1), first_b = 0;
+  if (even) {
+    const int item = blockIdx.x / per_item, r = blockIdx.x - item * per_item;
+    c0 = item * (longest + kPad) + (int)((unsigned)(r * longest) / (unsigned)per_item);
+    c1 = item * (longest + kPad) + (int)((unsigned)((r + 1) * longest) / (unsigned)per_item);
+  }
   for (int hi = p.c.batch; hi - first_b > 1;) {
     const int mid = (first_b + hi) >> 1;
     if (by_round ? info[mid].rounds <= (int)blockIdx.x : info[mid].cum <= c0) first_b = mid;
@@ -354,8 +373,8 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     const SeqInfo s = info[first_b];
     const int blocks = item_blocks<C>(p, s.len, s.count), rounds = (blocks + W - 1) / W, x = blockIdx.x - s.rounds;
     const int item = x / rounds, r = x - item * rounds;
-    c0 = s.cum + item * blocks + r * W;
-    c1 = s.cum + item * blocks + min(blocks, (r + 1) * W);
+    c0 = s.cum + item * (blocks + kPad) + r * W;
+    c1 = s.cum + item * (blocks + kPad) + min(blocks, (r + 1) * W);
   }
 
   uint8_t* my_ring = ring + (size_t)warp * p.stages * 2 * C::KB;
@@ -392,8 +411,8 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     while (t >= info[it.b + 1].cum) ++it.b;
     it.s = info[it.b];
     it.blocks = item_blocks<C>(p, it.s.len, it.s.count);
-    const int i = (int)((unsigned)(t - it.s.cum) / (unsigned)it.blocks);
-    it.start = it.s.cum + i * it.blocks;
+    const int i = (int)((unsigned)(t - it.s.cum) / (unsigned)(it.blocks + kPad));
+    it.start = it.s.cum + i * (it.blocks + kPad);
     it.h = p.chunks == 1 ? i : i / p.chunks;
     it.row0 = (i - it.h * p.chunks) * R;
     it.nrow = min(R, p.rows - it.row0);
@@ -436,6 +455,10 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     const SeqInfo s = it.s;
     const int start = it.start, h = it.h, row0 = it.row0, nrow = it.nrow, b = it.b;
     const int end = min(c1, start + it.blocks), n4 = nrow * (D / 4);
+    if (!join && t >= end) {  // places without blocks
+      t = min(c1, start + it.blocks + kPad);
+      continue;
+    }
     // the partials to add up: part k's outputs from src + k src_ld, its (maximum, sum) pairs from ms + k ms_ld
     const float* src = merge;
     const float2* ms = s_ms;
@@ -453,7 +476,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       ms = reinterpret_cast<const float2*>(src + p.nr * D);
       ms_ld = part_ld;
       pitch = D;
-      if (!by_round && share(i0) < start) skip0 = part_ld;  // that CTA had another item before this one
+      if (!by_round && !even && share(i0) < start) skip0 = part_ld;  // that CTA had another item before this one
       // groups of threads share the parts out
       teams = max(1, min((parts + V - 1) / V, NTHREADS / n4));
     } else {
@@ -463,6 +486,9 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       if (by_round) {
         n = (it.blocks + W - 1) / W;
         i0 = s.rounds + (h * p.chunks + row0 / R) * n;
+      } else if (even) {
+        n = per_item;
+        i0 = blockIdx.x / per_item * per_item;
       } else {
         i0 = owner(start);
         n = owner(start + it.blocks - 1) - i0 + 1;
@@ -867,7 +893,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       teams = 1;
     }
     __syncthreads();  // the merge area is free
-    if (!join) t = end;
+    if (!join) t = min(c1, start + it.blocks + kPad);
   }
   if (dead) {  // see this warp's copies in flight through, again with a limit, before leaving
     for (int i = 0; lane == 0 && i < waiting; ++i) {
@@ -1020,7 +1046,7 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   const Workspace need(cache, Hq, T, weights != nullptr, dev->sms);
   if (!sync || !ws || ws_bytes < need.bytes()) return TBF16_ERR_INVALID;
   // blocks are counted in 32 bits, 16 keys at the least in each
-  if (cache->batch * cache->heads * need.chunks > INT32_MAX / (p.c.cap / 16 + 1)) return TBF16_ERR_INVALID;
+  if (cache->batch * cache->heads * need.chunks > INT32_MAX / (p.c.cap / 16 + 1 + kPad)) return TBF16_ERR_INVALID;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_sb = q_sb; p.q_sh = q_sh; p.q_st = q_st;
   p.out = static_cast<__nv_bfloat16*>(out);
