@@ -46,7 +46,7 @@ struct Tile {
   static constexpr int NG = BK / 16;                         // groups of 16 keys, worked on one after another
   static constexpr int GB = 16 * RB;                         // bytes of a group: [RB / AW][16 keys][AW]
   static constexpr int KB = NG * GB;                         // bytes of a block's keys (or values)
-  static constexpr int W = RB == 512 ? 4 : 8;                // warps
+  static constexpr int W = RB == 512 && NQ == 2 ? 4 : 8;     // warps
   static constexpr int SC = E4M3 ? 2 * BK * 4 : 0;           // bytes of a block's scales
   static constexpr int MP = D + 4;                           // floats between rows of the merge area (no bank twice)
 };
