@@ -46,7 +46,7 @@ struct Tile {
   static constexpr int NG = BK / 16;                         // groups of 16 keys, worked on one after another
   static constexpr int GB = 16 * RB;                         // bytes of a group: [RB / AW][16 keys][AW]
   static constexpr int KB = NG * GB;                         // bytes of a block's keys (or values)
-  static constexpr int W = RB == 512 && NQ == 2 ? 4 : 8;     // warps
+  static constexpr int W = 8;                                // warps
   static constexpr int SC = E4M3 ? 2 * BK * 4 : 0;           // bytes of a block's scales
   static constexpr int MP = D + 4;                           // floats between rows of the merge area (no bank twice)
 };
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     const Item it = item_at(!join ? t : todo & 1 ? open0 : open1, first_b);
     const SeqInfo s = it.s;
     const int start = it.start, h = it.h, row0 = it.row0, nrow = it.nrow, b = it.b;
-    const int end = min(c1, start + it.blocks), n4 = nrow * (D / 4);
+    const int end = min(c1, start + it.blocks);
     if (!join && t >= end) {  // places without blocks
       t = min(c1, start + it.blocks + kPad);
       continue;
@@ -462,10 +462,12 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     // the partials to add up: part k's outputs from src + k src_ld, its (maximum, sum) pairs from ms + k ms_ld
     const float* src = merge;
     const float2* ms = s_ms;
-    size_t src_ld = p.nr * MP, ms_ld = R, skip0 = 0;  // skip0: part 0 lies that much further on
+    size_t src_ld = 8 * MP, ms_ld = R, skip0 = 0;  // skip0: part 0 lies that much further on
     int pitch = MP;                                   // floats between a part's rows
     int parts = W, teams = 1;
     bool split = false;
+    float o[NQ][KS][4];  // O^T: 16 columns of the values x 8 query rows a tile
+    float vtop = 0.f;    // e4m3: bound of the value scales met so far
     if (join) {
       const bool first = todo & 1;
       const int i0 = first ? at0 : at1;
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       pitch = D;
       if (!by_round && !even && share(i0) < start) skip0 = part_ld;  // that CTA had another item before this one
       // groups of threads share the parts out
-      teams = max(1, min((parts + V - 1) / V, NTHREADS / n4));
+      teams = max(1, min((parts + V - 1) / V, NTHREADS / (nrow * (D / 4))));
     } else {
     split = end - t != it.blocks;
     if (split) {
@@ -544,11 +546,14 @@ __global__ void __launch_bounds__(C::W * 32, 1)
         at[q][e] = r2 < p.rows && tok2 < s.count ? s.len - s.count + tok2 : -1;
       }
     }
-    float o[NQ][KS][4] = {};  // O^T: 16 columns of the values x 8 query rows a tile
     float m[NQ][2], l[NQ][2];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) m[q][0] = m[q][1] = kNoMax, l[q][0] = l[q][1] = 0.f;
-    float vtop = 0.f, vmul = 0.f;  // e4m3: bound of the value scales met so far, and 2^kWeightShift over it
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) o[q][k][0] = o[q][k][1] = o[q][k][2] = o[q][k][3] = 0.f;
+    float vmul = 0.f;  // e4m3: 2^kWeightShift over vtop
     const int pos_min = s.len - s.count, pos_max = s.len - 1;
 
     const int first = t + (warp - (t - c0) % W + W) % W;
@@ -802,17 +807,27 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       phase ^= stage == 0;
     }
 
-    // the warps' parts of the item
-    const float f = E4M3 ? vtop * (1.f / (1 << kWeightShift)) : 1.f;
+    // the warps' parts of the item: their maxima and sums here, their outputs below, a tile of eight rows at a time
 #pragma unroll
     for (int q = 0; q < NQ; ++q)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = q * 8 + 2 * c4 + e;
         l[q][e] = column_sum(l[q][e]);
-        if (g4 == 0) s_ms[warp * R + r] = make_float2(m[q][e], l[q][e]);
-        if (r < p.nr) {
-          float* dst = merge + ((size_t)warp * p.nr + r) * MP;
+        if (g4 == 0) s_ms[warp * R + q * 8 + 2 * c4 + e] = make_float2(m[q][e], l[q][e]);
+      }
+    }
+    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * part_ld;
+    const int tiles = join ? 1 : (nrow + 7) / 8;
+#pragma unroll 1
+    for (int tile = 0; tile < tiles; ++tile) {
+    if (!join) {
+      const float f = E4M3 ? vtop * (1.f / (1 << kWeightShift)) : 1.f;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (q != tile || q * 8 + 2 * c4 + e >= p.nr) continue;
+          float* dst = merge + ((size_t)warp * 8 + 2 * c4 + e) * MP;
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             if (E4M3) {
@@ -823,10 +838,9 @@ __global__ void __launch_bounds__(C::W * 32, 1)
             }
           }
         }
-      }
-    __syncthreads();
+      __syncthreads();
     }
-    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * part_ld;
+    const int r0 = tile * 8, n4 = (join ? nrow : min(8, nrow - r0)) * (D / 4);
 #pragma unroll 1
     for (bool again = false;; again = true) {  // again: the thread groups' sums of a join
       const int team = teams == 1 ? 0 : tid / n4;
@@ -834,7 +848,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       for (int i = tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         const float* x = src + (again ? i * 4 : r * pitch + d);
-        const float2* y = ms + (again ? i : r);
+        const float2* y = ms + (again ? i : r0 + r);
         float a = kNoMax, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
@@ -870,11 +884,11 @@ __global__ void __launch_bounds__(C::W * 32, 1)
           *reinterpret_cast<float4*>(merge + tid * 4) = v;
           s_team[tid] = make_float2(a, sum);
         } else if (split) {
-          *reinterpret_cast<float4*>(part + r * D + d) = v;
-          if (d == 0) *reinterpret_cast<float2*>(part + p.nr * D + 2 * r) = make_float2(a, sum);
+          *reinterpret_cast<float4*>(part + (r0 + r) * D + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(part + p.nr * D + 2 * (r0 + r)) = make_float2(a, sum);
         } else {
           // v / sum as bf16; zeros for rows that see nothing
-          const int row = row0 + r, tok = token_of(p, row);
+          const int row = row0 + r0 + r, tok = token_of(p, row);
           const float g = sum == 0.f || tok >= s.count ? 0.f : __fdividef(1.f, sum);
           if (g == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
           *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * p.group + row - tok * p.group) * p.o_sh +
@@ -893,6 +907,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       teams = 1;
     }
     __syncthreads();  // the merge area is free
+    }
     if (!join) t = min(c1, start + it.blocks + kPad);
   }
   if (dead) {  // see this warp's copies in flight through, again with a limit, before leaving
@@ -973,7 +988,7 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   while ((1 << p.box_shift) < box) ++p.box_shift;
   if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss, box)) return s;
   if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss, box)) return s;
-  p.merge = std::max(C::W * p.nr * C::MP, C::W * 32 * 4);  // the warps' outputs, or a join's thread groups' sums
+  p.merge = std::max(C::W * 8 * C::MP, C::W * 32 * 4);  // the warps' outputs, or a join's thread groups' sums
   p.stages = kMaxStages;
   while (p.stages > 1 && attend_smem<C>(p, p.stages) + kSmemStatic > kSmemMax) --p.stages;
   const int smem = attend_smem<C>(p, p.stages);
