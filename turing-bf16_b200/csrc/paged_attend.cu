@@ -27,28 +27,32 @@ using namespace tbf16;
 // O^T = V^T P^T. With the usual group of up to eight query rows no product is wasted on empty rows (a 16-row
 // query tile would waste half of them, tcgen05's 128 rows fifteen sixteenths), a lane holds four weights per 16
 // keys, and P^T gets from accumulator to operand layout by one 8x8 transpose per 8 keys.
-// Stages of a warp: 128 KB in flight on an SM. More of it makes the queues in front of the memory longer, not the rate
-// higher, and the SMs' rates more uneven, so the last one ends later (131071 tokens, all SMs with equal shares: they
-// end after 72 to 82 us with two stages and after 65 to 92 with three; one stage 104 us in all, two 97, three 101).
-constexpr int kMaxStages = 2;
+// Bytes of all stages of an SM. More in flight makes the queues in front of the memory longer, not the rate higher, and
+// the SMs' rates more uneven, so the last one ends later (131071 tokens, all SMs with equal shares: they end after 72
+// to 82 us with 128 KB and after 65 to 92 with 192; in all 97 us and 101, 104 with 64).
+constexpr int kStageBytes = 128 * 1024;
 // Partials that a thread has in flight when it adds them up (24 partials of 16 rows: 21.5 us with four, 19.5 with eight).
 constexpr int kPartLoads = 8;
 
-template <int D_, bool E4M3_, int NQ_>
+template <int D_, bool E4M3_, int NQ_, int S_>
 struct Tile {
   static constexpr int D = D_;
   static constexpr bool E4M3 = E4M3_;
-  static constexpr int NQ = NQ_;                             // column tiles of eight query rows
-  static constexpr int R = 8 * NQ;                           // query rows of an item
+  static constexpr int W = 8;                                // warps
+  static constexpr int NQ = NQ_;                             // column tiles of eight query rows of a warp
+  static constexpr int S = S_;                               // warps of a team: they share its blocks, each with its own rows
+  static constexpr int TEAMS = W / S;
+  static constexpr int R = 8 * NQ * S;                       // query rows of an item
   static constexpr int RB = D * (E4M3 ? 1 : 2);              // bytes of a cached row
   static constexpr int AW = RB < 128 ? RB : 128;             // swizzle span: 64 or 128 bytes
   static constexpr int BK = RB <= 64 ? 64 : RB <= 128 ? 32 : 16;  // keys of a block
   static constexpr int NG = BK / 16;                         // groups of 16 keys, worked on one after another
   static constexpr int GB = 16 * RB;                         // bytes of a group: [RB / AW][16 keys][AW]
-  static constexpr int KB = NG * GB;                         // bytes of a block's keys (or values)
-  static constexpr int W = 8;                                // warps
+  static constexpr int KB = NG * GB;                         // bytes of a block's keys (or values): 4 KB, 8 for 512-byte rows
   static constexpr int SC = E4M3 ? 2 * BK * 4 : 0;           // bytes of a block's scales
+  static constexpr int MAX_STAGES = kStageBytes / (TEAMS * 2 * KB);
   static constexpr int MP = D + 4;                           // floats between rows of the merge area (no bank twice)
+  static constexpr int MERGE = W * 8 * NQ * MP;              // floats of it; a join's thread groups take W * 32 * 4
 };
 
 struct AttendParams {
@@ -64,7 +68,6 @@ struct AttendParams {
   int stages;
   int box_shift;    // log2 of the keys that one TMA load brings: min(BK, page size); rows of one span when over 16
   int nr;           // rows of an item that can be real: min(rows, R)
-  int merge;        // floats of the merge area
   unsigned* sync;   // arrivals of each item, zero between calls
   float* part;      // [2 * CTAs][partial_floats(nr, D)]: partial outputs, (maximum, sum) pairs
   float* logits;    // weights wanted: [batch * heads][rows][cap], base-2 logits
@@ -187,9 +190,9 @@ __device__ __forceinline__ uint32_t chunk_from(uint32_t at_odd, int even) {
   return C::AW == 128 ? (at_odd ^ ((even & 7) << 4)) + (even >> 3) * 2048 : at_odd ^ (even << 4);
 }
 
-// Where a warp's next block lies: t in the order of all blocks, the item it belongs to, block of that item.
+// Where a team's next block lies: t in the order of all blocks, the item it belongs to, block of that item.
 struct Cursor {
-  int t, b, h, blk, blocks, j0, len;  // j0: its first key; len: cached tokens, 0 past the end of the warp's blocks
+  int t, b, h, blk, blocks, j0, len;  // j0: its first key; len: cached tokens, 0 past the end of the team's blocks
   int page;                           // this lane's page of the block, loaded ahead
 };
 
@@ -203,9 +206,9 @@ struct Loader {
     u.page = j < min(u.len, u.j0 + C::BK) ? p.c.table[u.b * p.c.table_ld + (j >> p.c.page_shift)] : 0;
   }
 
-  // Moves the cursor to the warp's first block at or after position t with anything to load.
+  // Moves the cursor to the team's first block at or after position t with anything to load.
   static __device__ __forceinline__ void seek(Cursor& u, int t, int end, const SeqInfo* info, const AttendParams& p, int lane) {
-    for (;; t += C::W) {
+    for (;; t += C::TEAMS) {
       u.t = t;
       u.len = 0;
       if (t >= end) return;
@@ -223,13 +226,13 @@ struct Loader {
     fetch_pages(u, p, lane);
   }
   static __device__ __forceinline__ void next(Cursor& u, int end, const SeqInfo* info, const AttendParams& p, int lane) {
-    if (u.blk + C::W < u.blocks && u.t + C::W < end) {
-      u.t += C::W;
-      u.blk += C::W;
-      u.j0 += C::W * C::BK;
+    if (u.blk + C::TEAMS < u.blocks && u.t + C::TEAMS < end) {
+      u.t += C::TEAMS;
+      u.blk += C::TEAMS;
+      u.j0 += C::TEAMS * C::BK;
       fetch_pages(u, p, lane);
     } else {
-      seek(u, u.t + C::W, end, info, p, lane);
+      seek(u, u.t + C::TEAMS, end, info, p, lane);
     }
   }
 
@@ -268,20 +271,20 @@ constexpr int kWeightShift = 7;
 template <class C>
 __global__ void __launch_bounds__(C::W * 32, 1)
     attend_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm, const AttendParams p) {
-  constexpr int D = C::D, W = C::W, NQ = C::NQ, R = C::R, NG = C::NG, KS = D / 16, NTHREADS = W * 32, MP = C::MP;
-  constexpr int V = kPartLoads;
+  constexpr int D = C::D, W = C::W, NQ = C::NQ, S = C::S, TEAMS = C::TEAMS, R = C::R, NG = C::NG, KS = D / 16;
+  constexpr int NTHREADS = W * 32, MP = C::MP, V = kPartLoads;
   constexpr bool E4M3 = C::E4M3;
   using L = Loader<C>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem;
-  float* scale_ring = reinterpret_cast<float*>(ring + (size_t)W * p.stages * 2 * C::KB);
-  float* merge = scale_ring + (size_t)W * p.stages * (C::SC / 4);
-  SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + p.merge);
-  __shared__ uint64_t bars[W * kMaxStages];
-  __shared__ float2 s_ms[W * R];       // each warp's (maximum, sum) of a row
-  __shared__ float2 s_team[NTHREADS];  // that of a row in each thread group of a join
+  float* scale_ring = reinterpret_cast<float*>(ring + (size_t)TEAMS * p.stages * 2 * C::KB);
+  float* merge = scale_ring + (size_t)TEAMS * p.stages * (C::SC / 4);
+  SeqInfo* info = reinterpret_cast<SeqInfo*>(merge + C::MERGE);
+  __shared__ uint64_t full[TEAMS * C::MAX_STAGES], empty[TEAMS * C::MAX_STAGES];
+  __shared__ float2 s_ms[TEAMS * R];   // each warp's (maximum, sum) of a row
+  __shared__ float2 s_group[NTHREADS]; // that of a row in each thread group of a join
   __shared__ int s_scan[W], s_work[W], s_long[W], s_abort, s_todo;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / S, tile = warp % S;
   if ((smem_u32(smem) & 1023u) != 0) {
     if (tid == 0) atomicOr(p.c.err, kErrSmemAlign);
     return;
@@ -289,14 +292,17 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   if (tid == 0) {
     tma_prefetch_desc(&km);
     tma_prefetch_desc(&vm);
+    s_abort = 0;
   }
-  if (lane < p.stages) mbar_init(&bars[warp * p.stages + lane], 1);
-  if (tid == 0) s_abort = 0;
+  if (tid < TEAMS * p.stages) {
+    mbar_init(&full[tid], 1);
+    mbar_init(&empty[tid], S > 1 ? S - 1 : 1);
+  }
   fence_barrier_init();
   pdl_launch_dependents();
   pdl_wait();
 
-  // Every sequence's blocks and rounds (a round: a block for each warp) and their running totals.
+  // Every sequence's places and rounds (a round: a block for each team) and their running totals.
   int total = 0, work = 0, longest = 0;
   for (int b0 = 0; b0 < p.c.batch; b0 += NTHREADS) {
     const int b = b0 + tid;
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       s.count = paged_count(p.c, p.counts, b, p.T, s.len);
       blocks = item_blocks<C>(p, s.len, s.count);
       x = blocks ? (blocks + kPad) * p.c.heads * p.chunks : 0;
-      y = (blocks + W - 1) / W * p.c.heads * p.chunks;
+      y = (blocks + TEAMS - 1) / TEAMS * p.c.heads * p.chunks;
     }
     const int my_x = x, my_y = y;
 #pragma unroll
@@ -337,8 +343,8 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     if (b == p.c.batch - 1) info[b + 1] = SeqInfo{x + my_x, y + my_y, 0, 0};
     __syncthreads();
   }
-  // Few rounds: a CTA takes one, so no item waits for another. Else CTA i takes blocks [share(i), share(i + 1)):
-  // `each` of them, the first `more` CTAs one more.
+  // Few rounds: a CTA takes one, so no item waits for another. Else CTA i takes places [share(i), share(i + 1)): `each`
+  // of them, the first `more` CTAs one more.
   // Sequences of one length with few items: as many CTAs for each item, as long as that leaves out no more than one in
   // twenty; a CTA with the end of one item and the start of the next would have two partials to add up at the end.
   const bool by_round = work <= (int)gridDim.x;
@@ -349,20 +355,23 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x) {
     if (info[b].count) continue;
     const int heads = p.c.heads * p.group;
-    for (int i = tid; i < heads * p.T * (D / 8); i += NTHREADS) {
-      const int row = i / (D / 8), t = row / heads;
+    for (int64_t i = tid; i < (int64_t)heads * p.T * (D / 8); i += NTHREADS) {
+      const int row = (int)(i / (D / 8)), t = row / heads;
       *reinterpret_cast<uint4*>(p.out + b * p.o_sb + (int64_t)(row - t * heads) * p.o_sh + t * p.o_st + i % (D / 8) * 8) =
           make_uint4(0, 0, 0, 0);
     }
   }
   if ((int)blockIdx.x >= ctas) return;
-  const int each = total / ctas, more = total - each * ctas;
+  const int each = (even ? longest : total) / (even ? per_item : ctas), more = (even ? longest : total) - each * (even ? per_item : ctas);
   auto share = [&](int i) { return each * i + min(i, more); };
-  int c0 = share(blockIdx.x), c1 = share(blockIdx.x + 1), first_b = 0;
+  int c0, c1, first_b = 0;
   if (even) {
     const int item = blockIdx.x / per_item, r = blockIdx.x - item * per_item;
-    c0 = item * (longest + kPad) + (int)((unsigned)(r * longest) / (unsigned)per_item);
-    c1 = item * (longest + kPad) + (int)((unsigned)((r + 1) * longest) / (unsigned)per_item);
+    c0 = item * (longest + kPad) + share(r);
+    c1 = item * (longest + kPad) + share(r + 1);
+  } else {
+    c0 = share(blockIdx.x);
+    c1 = share(blockIdx.x + 1);
   }
   for (int hi = p.c.batch; hi - first_b > 1;) {
     const int mid = (first_b + hi) >> 1;
@@ -371,27 +380,32 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   }
   if (by_round) {
     const SeqInfo s = info[first_b];
-    const int blocks = item_blocks<C>(p, s.len, s.count), rounds = (blocks + W - 1) / W, x = blockIdx.x - s.rounds;
+    const int blocks = item_blocks<C>(p, s.len, s.count), rounds = (blocks + TEAMS - 1) / TEAMS, x = blockIdx.x - s.rounds;
     const int item = x / rounds, r = x - item * rounds;
-    c0 = s.cum + item * (blocks + kPad) + r * W;
-    c1 = s.cum + item * (blocks + kPad) + min(blocks, (r + 1) * W);
+    c0 = s.cum + item * (blocks + kPad) + r * TEAMS;
+    c1 = s.cum + item * (blocks + kPad) + min(blocks, (r + 1) * TEAMS);
   }
 
-  uint8_t* my_ring = ring + (size_t)warp * p.stages * 2 * C::KB;
-  float* my_scales = scale_ring + (size_t)warp * p.stages * (C::SC / 4);
-  uint64_t* my_bars = bars + warp * p.stages;
+  // The team's ring. Its first warp loads; every warp of it waits for a block and reads it.
+  uint8_t* my_ring = ring + (size_t)team * p.stages * 2 * C::KB;
+  float* my_scales = scale_ring + (size_t)team * p.stages * (C::SC / 4);
+  uint64_t* my_full = full + team * p.stages;
+  uint64_t* my_empty = empty + team * p.stages;
   Cursor u;
   u.b = first_b;
-  int issued = 0, waiting = 0;  // stage of the next load; blocks issued and not consumed yet
+  u.len = 0;
+  int issued = 0, waiting = 0;  // stage of the next load; blocks loaded and not used yet
   auto issue = [&]() {
-    L::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_bars[issued], &km, &vm, p);
+    L::load(u, my_ring + (size_t)issued * 2 * C::KB, my_scales + issued * (C::SC / 4), &my_full[issued], &km, &vm, p);
     issued = issued + 1 == p.stages ? 0 : issued + 1;
     ++waiting;
     L::next(u, c1, info, p, lane);
   };
-  L::seek(u, c0 + warp, c1, info, p, lane);
+  if (tile == 0) {
+    L::seek(u, c0 + team, c1, info, p, lane);
 #pragma unroll 1
-  while (waiting < p.stages && u.len) issue();
+    while (waiting < p.stages && u.len) issue();
+  }
   int stage = 0, phase = 0;
   bool dead = false;  // a wait gave up: nothing more is loaded or computed, every barrier is still reached
 
@@ -400,7 +414,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   const uint32_t k_lane = chunk_at<C>(lane & 15, lane >> 4);
   const uint32_t v_lane = E4M3 ? k_lane : chunk_at<C>(((lane >> 4) & 1) * 8 + (lane & 7), (lane >> 3) & 1);
 
-  // The item that holds block t.
+  // The item that holds place t.
   struct Item {
     SeqInfo s;
     int start, blocks, b, h, row0, nrow;
@@ -419,7 +433,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     return it;
   };
   const size_t part_ld = partial_floats(p.nr, D);
-  auto owner = [&](int x) {  // the CTA that has block x
+  auto owner = [&](int x) {  // the CTA that has place x
     const int big = more * (each + 1);
     return x < big ? x / (each + 1) : more + (x - big) / each;
   };
@@ -454,7 +468,7 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     const Item it = item_at(!join ? t : todo & 1 ? open0 : open1, first_b);
     const SeqInfo s = it.s;
     const int start = it.start, h = it.h, row0 = it.row0, nrow = it.nrow, b = it.b;
-    const int end = min(c1, start + it.blocks);
+    const int end = min(c1, start + it.blocks), n4 = nrow * (D / 4);
     if (!join && t >= end) {  // places without blocks
       t = min(c1, start + it.blocks + kPad);
       continue;
@@ -462,12 +476,10 @@ __global__ void __launch_bounds__(C::W * 32, 1)
     // the partials to add up: part k's outputs from src + k src_ld, its (maximum, sum) pairs from ms + k ms_ld
     const float* src = merge;
     const float2* ms = s_ms;
-    size_t src_ld = 8 * MP, ms_ld = R, skip0 = 0;  // skip0: part 0 lies that much further on
-    int pitch = MP;                                   // floats between a part's rows
-    int parts = W, teams = 1;
+    size_t src_ld = R * MP, ms_ld = R, skip0 = 0;  // skip0: part 0 lies that much further on
+    int pitch = MP;                                // floats between a part's rows
+    int parts = TEAMS, groups = 1;
     bool split = false;
-    float o[NQ][KS][4];  // O^T: 16 columns of the values x 8 query rows a tile
-    float vtop = 0.f;    // e4m3: bound of the value scales met so far
     if (join) {
       const bool first = todo & 1;
       const int i0 = first ? at0 : at1;
@@ -480,354 +492,354 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       pitch = D;
       if (!by_round && !even && share(i0) < start) skip0 = part_ld;  // that CTA had another item before this one
       // groups of threads share the parts out
-      teams = max(1, min((parts + V - 1) / V, NTHREADS / (nrow * (D / 4))));
+      groups = max(1, min((parts + V - 1) / V, NTHREADS / n4));
     } else {
-    split = end - t != it.blocks;
-    if (split) {
-      int i0, n;
-      if (by_round) {
-        n = (it.blocks + W - 1) / W;
-        i0 = s.rounds + (h * p.chunks + row0 / R) * n;
-      } else if (even) {
-        n = per_item;
-        i0 = blockIdx.x / per_item * per_item;
-      } else {
-        i0 = owner(start);
-        n = owner(start + it.blocks - 1) - i0 + 1;
-      }
-      const int word = (b * p.c.heads + h) * p.chunks + row0 / R;
-      if (t == c0) open0 = t, at0 = i0, parts0 = n, word0 = word;
-      else open1 = t, at1 = i0, parts1 = n, word1 = word;
-    }
-    const int lo = first_block<C>(p, s.len, s.count);
-    // B fragments of the item's query rows (a lane loads row g4 of each tile), and what this lane has to know of
-    // the rows in its accumulator columns, 2 c4 and 2 c4 + 1 of each tile
-    uint32_t qf[NQ][KS][2];
-    float mul[NQ][2];
-    int at[NQ][2];  // position of the row's token; -1: the row is not there
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int r = row0 + q * 8 + g4, tok = token_of(p, r);
-      const bool there = r < p.rows && tok < s.count;
-      const __nv_bfloat16* x = p.q + b * p.q_sb + (int64_t)(h * p.group + r - tok * p.group) * p.q_sh + tok * p.q_st;
-      if (E4M3) {
-        // fp16 rows: the largest magnitude to [2^14, 2^15) by a power of two, undone in the logits' factor. In
-        // column 16 k + 4 c of a k16 step sit the two pairs the byte order of a cached row puts there.
-        uint2 y[KS];
-        unsigned m = 0;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) y[k] = there ? *reinterpret_cast<const uint2*>(x + k * 16 + c4 * 4) : make_uint2(0, 0);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          m = max(m, max(max((y[k].x << 16) & 0x7fffffffu, y[k].x & 0x7fff0000u),
-                         max((y[k].y << 16) & 0x7fffffffu, y[k].y & 0x7fff0000u)));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const int e = m == 0 || m >= 0x7f800000u ? 15 : max(frexp_exp(__uint_as_float(m)), -110);
-        const float f = exp2i(15 - e), undo = p.scale_log2 * exp2i(e - 15);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          qf[q][k][0] = pack_f16(bf16lo(y[k].x) * f, bf16hi(y[k].x) * f);
-          qf[q][k][1] = pack_f16(bf16lo(y[k].y) * f, bf16hi(y[k].y) * f);
+      split = end - t != it.blocks;
+      if (split) {
+        int i0, n;
+        if (by_round) {
+          n = (it.blocks + TEAMS - 1) / TEAMS;
+          i0 = s.rounds + (h * p.chunks + row0 / R) * n;
+        } else if (even) {
+          n = per_item;
+          i0 = blockIdx.x / per_item * per_item;
+        } else {
+          i0 = owner(start);
+          n = owner(start + it.blocks - 1) - i0 + 1;
         }
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) mul[q][e2] = __shfl_sync(0xffffffffu, undo, (2 * c4 + e2) * 4);
-      } else {
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          qf[q][k][0] = there ? *reinterpret_cast<const uint32_t*>(x + k * 16 + c4 * 2) : 0u;
-          qf[q][k][1] = there ? *reinterpret_cast<const uint32_t*>(x + k * 16 + 8 + c4 * 2) : 0u;
-        }
-        mul[q][0] = mul[q][1] = p.scale_log2;
+        const int word = (b * p.c.heads + h) * p.chunks + row0 / R;
+        if (t == c0) open0 = t, at0 = i0, parts0 = n, word0 = word;
+        else open1 = t, at1 = i0, parts1 = n, word1 = word;
       }
+      const int lo = first_block<C>(p, s.len, s.count);
+      const int tile0 = tile * NQ * 8;        // the warp's first row of the item
+      const bool rows_here = tile0 < nrow;    // else this warp only frees the team's stages
+      // B fragments of the warp's query rows (a lane loads row g4 of each tile), and what this lane has to know of the
+      // rows in its accumulator columns, 2 c4 and 2 c4 + 1 of each tile
+      uint32_t qf[NQ][KS][2];
+      float mul[NQ][2];
+      int at[NQ][2];  // position of the row's token; -1: the row is not there
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r2 = row0 + q * 8 + 2 * c4 + e, tok2 = token_of(p, r2);
-        at[q][e] = r2 < p.rows && tok2 < s.count ? s.len - s.count + tok2 : -1;
-      }
-    }
-    float m[NQ][2], l[NQ][2];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) m[q][0] = m[q][1] = kNoMax, l[q][0] = l[q][1] = 0.f;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-      for (int k = 0; k < KS; ++k) o[q][k][0] = o[q][k][1] = o[q][k][2] = o[q][k][3] = 0.f;
-    float vmul = 0.f;  // e4m3: 2^kWeightShift over vtop
-    const int pos_min = s.len - s.count, pos_max = s.len - 1;
-
-    const int first = t + (warp - (t - c0) % W + W) % W;
-#pragma unroll 1
-    for (int x = first; x < end && s.count; x += W) {
-      // every lane looks once; only a wait in earnest is left to one lane and its limit
-      if (!__all_sync(0xffffffffu, !dead && mbar_try_wait(&my_bars[stage], phase)) &&
-          (dead || !mbar_wait_warp(&my_bars[stage], phase, &s_abort, p.c.err))) {
-        dead = true;
-        break;
-      }
-      const uint32_t kb = smem_u32(my_ring) + stage * (2 * C::KB);
-      const float* ksc = my_scales + stage * (C::SC / 4) + g4;
-      const int j0 = (lo + x - start) * C::BK;
-      const int groups = min(NG, (s.len - j0 + 15) >> 4);
-#pragma unroll 1
-      for (int g = 0; g < groups; ++g) {
-        // S^T of 16 keys (rows g4, g4 + 8) x the query rows; for a single tile two accumulators shorten the chain of
-        // dependent products. Fragments come in batches of four loads, so that a load's latency is met per batch.
-        const uint32_t ka = kb + g * C::GB + k_lane;
-        constexpr int CH = NQ == 1 ? 2 : 1;
-        float acc[NQ * CH][4];
-        constexpr int KI = E4M3 ? KS / 2 : KS, KB4 = KI < 4 ? KI : 4;
-#pragma unroll
-        for (int k0 = 0; k0 < KI; k0 += KB4) {
-          uint32_t r[KB4][4];
-#pragma unroll
-          for (int k = 0; k < KB4; ++k) ldsm4(r[k], chunk_from<C>(ka, 2 * (k0 + k)));
-#pragma unroll
-          for (int kk = 0; kk < KB4; ++kk)
-#pragma unroll
-            for (int half = 0; half < (E4M3 ? 2 : 1); ++half) {
-              // bf16: a register is eight keys' chunk half; e4m3: eight keys' chunk, two k16 steps in the four
-              const int k = E4M3 ? 2 * (k0 + kk) + half : k0 + kk;
-              uint32_t a[4];
-              if (E4M3) {
-                e4m3_f16(r[kk][2 * half], a[0], a[2]);
-                e4m3_f16(r[kk][2 * half + 1], a[1], a[3]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = r[kk][i];
-              }
-#pragma unroll
-              for (int q = 0; q < NQ; ++q) {
-                float(&d)[4] = acc[q * CH + k % CH];
-                if (k < CH) mma16_first<E4M3>(d, a, qf[q][k][0], qf[q][k][1]);
-                else mma16<E4M3>(d, a, qf[q][k][0], qf[q][k][1]);
-              }
-            }
-        }
-        const int jg = j0 + g * 16;
-        const bool whole = jg + 15 <= pos_min && (!p.window || jg > pos_max - p.window);
-        float ks[2] = {1.f, 1.f}, vs[2];  // e4m3: scales of this lane's two keys
+      for (int q = 0; q < NQ; ++q) {
+        const int r = row0 + tile0 + q * 8 + g4, tok = token_of(p, r);
+        const bool there = r < p.rows && tok < s.count;
+        const __nv_bfloat16* x = p.q + b * p.q_sb + (int64_t)(h * p.group + r - tok * p.group) * p.q_sh + tok * p.q_st;
         if (E4M3) {
+          // fp16 rows: the largest magnitude to [2^14, 2^15) by a power of two, undone in the logits' factor. In
+          // column 16 k + 4 c of a k16 step sit the two pairs the byte order of a cached row puts there.
+          uint2 y[KS];
+          unsigned m = 0;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ks[i] = ksc[g * 16 + i * 8];
-            vs[i] = ksc[C::BK + g * 16 + i * 8];
+          for (int k = 0; k < KS; ++k) y[k] = there ? *reinterpret_cast<const uint2*>(x + k * 16 + c4 * 4) : make_uint2(0, 0);
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            m = max(m, max(max((y[k].x << 16) & 0x7fffffffu, y[k].x & 0x7fff0000u),
+                           max((y[k].y << 16) & 0x7fffffffu, y[k].y & 0x7fff0000u)));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const int e = m == 0 || m >= 0x7f800000u ? 15 : max(frexp_exp(__uint_as_float(m)), -110);
+          const float f = exp2i(15 - e), undo = p.scale_log2 * exp2i(e - 15);
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            qf[q][k][0] = pack_f16(bf16lo(y[k].x) * f, bf16hi(y[k].x) * f);
+            qf[q][k][1] = pack_f16(bf16lo(y[k].y) * f, bf16hi(y[k].y) * f);
           }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) mul[q][i] = __shfl_sync(0xffffffffu, undo, (2 * c4 + i) * 4);
+        } else {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            qf[q][k][0] = there ? *reinterpret_cast<const uint32_t*>(x + k * 16 + c4 * 2) : 0u;
+            qf[q][k][1] = there ? *reinterpret_cast<const uint32_t*>(x + k * 16 + 8 + c4 * 2) : 0u;
+          }
+          mul[q][0] = mul[q][1] = p.scale_log2;
         }
-        // logits in units of log 2
-        float sc[NQ][4];
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
+        for (int e = 0; e < 2; ++e) {
+          const int r2 = row0 + tile0 + q * 8 + 2 * c4 + e, tok2 = token_of(p, r2);
+          at[q][e] = r2 < p.rows && tok2 < s.count ? s.len - s.count + tok2 : -1;
+        }
+      }
+      float o[NQ][KS][4] = {};  // O^T: 16 columns of the values x 8 query rows a tile
+      float m[NQ][2], l[NQ][2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = CH == 2 ? acc[q * CH][e] + acc[q * CH + CH - 1][e] : acc[q][e];
-            sc[q][e] = y * (E4M3 ? mul[q][e & 1] * ks[e >> 1] : mul[q][e & 1]);
-          }
-        if (!whole) {
+      for (int q = 0; q < NQ; ++q) m[q][0] = m[q][1] = kNoMax, l[q][0] = l[q][1] = 0.f;
+      float vtop = 0.f, vmul = 0.f;  // e4m3: bound of the value scales met so far, and 2^kWeightShift over it
+      const int pos_min = s.len - s.count, pos_max = s.len - 1;
+
+      const int first = t + (team - (t - c0) % TEAMS + TEAMS) % TEAMS;
+#pragma unroll 1
+      for (int x = first; x < end; x += TEAMS) {
+        // every lane looks once; only a wait in earnest is left to one lane and its limit
+        if (!__all_sync(0xffffffffu, !dead && mbar_try_wait(&my_full[stage], phase)) &&
+            (dead || !mbar_wait_warp(&my_full[stage], phase, &s_abort, p.c.err))) {
+          dead = true;
+          break;
+        }
+        const uint32_t kb = smem_u32(my_ring) + stage * (2 * C::KB);
+        const float* ksc = my_scales + stage * (C::SC / 4) + g4;
+        const int j0 = (lo + x - start) * C::BK;
+        const int groups16 = rows_here ? min(NG, (s.len - j0 + 15) >> 4) : 0;
+#pragma unroll 1
+        for (int g = 0; g < groups16; ++g) {
+          // S^T of 16 keys (rows g4, g4 + 8) x the query rows; for a single tile two accumulators shorten the chain of
+          // dependent products. Fragments come in batches of four loads, so that a load's latency is met once a batch.
+          const uint32_t ka = kb + g * C::GB + k_lane;
+          constexpr int CH = NQ == 1 ? 2 : 1;
+          float acc[NQ * CH][4];
+          constexpr int KI = E4M3 ? KS / 2 : KS, KB4 = KI < 4 ? KI : 4;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int j = jg + g4 + i * 8;
-            // the scale of a row that nobody sees may be anything
-            if (E4M3 && (j > pos_max || (p.window && j <= pos_min - p.window))) vs[i] = 0.f;
+          for (int k0 = 0; k0 < KI; k0 += KB4) {
+            uint32_t r[KB4][4];
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
+            for (int k = 0; k < KB4; ++k) ldsm4(r[k], chunk_from<C>(ka, 2 * (k0 + k)));
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const bool see = j <= at[q][e] && (!p.window || j > at[q][e] - p.window);
-                if (!see) sc[q][2 * i + e] = -INFINITY;
+            for (int kk = 0; kk < KB4; ++kk)
+#pragma unroll
+              for (int half = 0; half < (E4M3 ? 2 : 1); ++half) {
+                // bf16: a register is eight keys' chunk half; e4m3: eight keys' chunk, two k16 steps in the four
+                const int k = E4M3 ? 2 * (k0 + kk) + half : k0 + kk;
+                uint32_t a[4];
+                if (E4M3) {
+                  e4m3_f16(r[kk][2 * half], a[0], a[2]);
+                  e4m3_f16(r[kk][2 * half + 1], a[1], a[3]);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) a[i] = r[kk][i];
+                }
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                  float(&d)[4] = acc[q * CH + k % CH];
+                  if (k < CH) mma16_first<E4M3>(d, a, qf[q][k][0], qf[q][k][1]);
+                  else mma16<E4M3>(d, a, qf[q][k][0], qf[q][k][1]);
+                }
               }
           }
-        }
-        if (p.logits) {
+          const int jg = j0 + g * 16;
+          const bool whole = jg + 15 <= pos_min && (!p.window || jg > pos_max - p.window);
+          float ks[2] = {1.f, 1.f}, vs[2];  // e4m3: scales of this lane's two keys
+          if (E4M3) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              ks[i] = ksc[g * 16 + i * 8];
+              vs[i] = ksc[C::BK + g * 16 + i * 8];
+            }
+          }
+          // logits in units of log 2
+          float sc[NQ][4];
 #pragma unroll
           for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (at[q][e & 1] >= 0)
-                p.logits[((int64_t)(b * p.c.heads + h) * p.rows + row0 + q * 8 + 2 * c4 + (e & 1)) * p.c.cap + jg + g4 +
-                         (e >> 1) * 8] = sc[q][e];
-        }
-        bool grew = false;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) grew |= fmaxf(sc[q][e], sc[q][2 + e]) - m[q][e] > kSlack;
-        if (E4M3) grew |= fmaxf(vs[0], vs[1]) > vtop && fmaxf(vs[0], vs[1]) < INFINITY;
-        if (__any_sync(0xffffffffu, grew)) {
-          float more_room = 1.f;
-          if (E4M3) {
-            const float y = column_max(fmaxf(vs[0] < INFINITY ? vs[0] : 0.f, vs[1] < INFINITY ? vs[1] : 0.f));
-            if (y > vtop) {  // two bits of room, so that the next ones rarely come here
-              const float now = fmaxf(y * 4.f, 0x1p-110f);
-              more_room = vtop / now;
-              vtop = now;
-              vmul = (float)(1 << kWeightShift) / now;
+            for (int e = 0; e < 4; ++e) {
+              const float y = CH == 2 ? acc[q * CH][e] + acc[q * CH + CH - 1][e] : acc[q][e];
+              sc[q][e] = y * (E4M3 ? mul[q][e & 1] * ks[e >> 1] : mul[q][e & 1]);
             }
-          }
+          if (!whole) {
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            float fac[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float was = m[q][e];
-              m[q][e] = fmaxf(was, column_max(fmaxf(sc[q][e], sc[q][2 + e])));
-              fac[e] = ex2(was - m[q][e]);
-              l[q][e] *= fac[e];
-              fac[e] *= more_room;
-            }
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[q][k][e] *= fac[e & 1];
-          }
-        }
-        float pw[NQ][4];  // weights for the output
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float w = ex2(sc[q][e] - m[q][e & 1]);
-            l[q][e & 1] += w;
-            pw[q][e] = E4M3 ? w * (vs[e >> 1] * vmul) : w;
-          }
-        const uint32_t vg = kb + C::KB + g * C::GB, va = vg + v_lane;
-        bool odd = false;
-        if (!whole) {
-          // A masked weight is 0, but 0 x NaN is not: if the values of a partly masked group hold infinities or
-          // NaNs (stale slots, a later token's), those are added here, to the rows that see them, and are zeros in
-          // the products below; all other bits of the result stay what they are without them.
-#pragma unroll 1
-          for (int i = lane; i < C::GB / 16; i += 32) {
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vg + i * 16));
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              odd |= (E4M3 ? __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpeq2(w[k] & 0x7f807f80u, 0x7f807f80u)) != 0;
-          }
-          odd = __any_sync(0xffffffffu, odd);
-          if (E4M3) {  // a scale may be NaN too
-#pragma unroll
-            for (int q = 0; q < NQ; ++q)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (sc[q][e] == -INFINITY) pw[q][e] = 0.f;
-          }
-          if (odd) {
-#pragma unroll 1
-            for (int k = 0; k < 16; ++k) {
-              const int j = jg + k;
-              float w[NQ][2];
-              bool see[NQ][2];
+            for (int i = 0; i < 2; ++i) {
+              const int j = jg + g4 + i * 8;
+              // the scale of a row that nobody sees may be anything
+              if (E4M3 && (j > pos_max || (p.window && j <= pos_min - p.window))) vs[i] = 0.f;
 #pragma unroll
               for (int q = 0; q < NQ; ++q)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const float w0 = __shfl_sync(0xffffffffu, pw[q][e], (k & 7) * 4 + c4);
-                  const float w1 = __shfl_sync(0xffffffffu, pw[q][2 + e], (k & 7) * 4 + c4);
-                  w[q][e] = k < 8 ? w0 : w1;
-                  see[q][e] = j <= at[q][e] && (!p.window || j > at[q][e] - p.window);
+                  const bool see = j <= at[q][e] && (!p.window || j > at[q][e] - p.window);
+                  if (!see) sc[q][2 * i + e] = -INFINITY;
                 }
+            }
+          }
+          if (p.logits) {
 #pragma unroll
-              for (int n = 0; n < KS; ++n) {
-                // this lane's two output rows of tile n: bf16 columns g4 and g4 + 8, e4m3 columns 2 g4 and 2 g4 + 1
-                float y[2];
-                if (E4M3) {
-                  unsigned short v;
-                  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(vg + chunk_at<C>(k, n) + g4 * 2));
-                  uint32_t lo2, hi2;
-                  e4m3_f16(v, lo2, hi2);
-                  y[0] = f16lo(lo2);
-                  y[1] = f16hi(lo2);
-                } else {
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                  for (int i = 0; i < 2; ++i) {
-                    unsigned short v;
-                    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(vg + chunk_at<C>(k, 2 * n + i) + g4 * 2));
-                    y[i] = bf16lo(v);
-                  }
-                }
+              for (int e = 0; e < 4; ++e)
+                if (at[q][e & 1] >= 0)
+                  p.logits[((int64_t)(b * p.c.heads + h) * p.rows + row0 + tile0 + q * 8 + 2 * c4 + (e & 1)) * p.c.cap + jg +
+                           g4 + (e >> 1) * 8] = sc[q][e];
+          }
+          bool grew = false;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) grew |= fmaxf(sc[q][e], sc[q][2 + e]) - m[q][e] > kSlack;
+          if (E4M3) grew |= fmaxf(vs[0], vs[1]) > vtop && fmaxf(vs[0], vs[1]) < INFINITY;
+          if (__any_sync(0xffffffffu, grew)) {
+            float more_room = 1.f;
+            if (E4M3) {
+              const float y = column_max(fmaxf(vs[0] < INFINITY ? vs[0] : 0.f, vs[1] < INFINITY ? vs[1] : 0.f));
+              if (y > vtop) {  // two bits of room, so that the next ones rarely come here
+                const float now = fmaxf(y * 4.f, 0x1p-110f);
+                more_room = vtop / now;
+                vtop = now;
+                vmul = (float)(1 << kWeightShift) / now;
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+              float fac[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float was = m[q][e];
+                m[q][e] = fmaxf(was, column_max(fmaxf(sc[q][e], sc[q][2 + e])));
+                fac[e] = ex2(was - m[q][e]);
+                l[q][e] *= fac[e];
+                fac[e] *= more_room;
+              }
+#pragma unroll
+              for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[q][k][e] *= fac[e & 1];
+            }
+          }
+          float pw[NQ][4];  // weights for the output
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w = ex2(sc[q][e] - m[q][e & 1]);
+              l[q][e & 1] += w;
+              pw[q][e] = E4M3 ? w * (vs[e >> 1] * vmul) : w;
+            }
+          const uint32_t vg = kb + C::KB + g * C::GB, va = vg + v_lane;
+          bool odd = false;
+          if (!whole) {
+            // A masked weight is 0, but 0 x NaN is not: if the values of a partly masked group hold infinities or
+            // NaNs (stale slots, a later token's), those are added here, to the rows that see them, and are zeros in
+            // the products below; all other bits of the result stay what they are without them.
+#pragma unroll 1
+            for (int i = lane; i < C::GB / 16; i += 32) {
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vg + i * 16));
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                odd |= (E4M3 ? __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpeq2(w[k] & 0x7f807f80u, 0x7f807f80u)) != 0;
+            }
+            odd = __any_sync(0xffffffffu, odd);
+            if (E4M3) {  // a scale may be NaN too
+#pragma unroll
+              for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (sc[q][e] == -INFINITY) pw[q][e] = 0.f;
+            }
+            if (odd) {
+#pragma unroll 1
+              for (int k = 0; k < 16; ++k) {
+                const int j = jg + k;
+                float w[NQ][2];
+                bool see[NQ][2];
 #pragma unroll
                 for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    if (see[q][e & 1] && !isfinite(y[e >> 1])) o[q][n][e] += w[q][e & 1] * y[e >> 1];
+                  for (int e = 0; e < 2; ++e) {
+                    const float w0 = __shfl_sync(0xffffffffu, pw[q][e], (k & 7) * 4 + c4);
+                    const float w1 = __shfl_sync(0xffffffffu, pw[q][2 + e], (k & 7) * 4 + c4);
+                    w[q][e] = k < 8 ? w0 : w1;
+                    see[q][e] = j <= at[q][e] && (!p.window || j > at[q][e] - p.window);
+                  }
+#pragma unroll
+                for (int n = 0; n < KS; ++n) {
+                  // this lane's two output rows of tile n: bf16 columns g4 and g4 + 8, e4m3 columns 2 g4 and 2 g4 + 1
+                  float y[2];
+                  if (E4M3) {
+                    unsigned short v;
+                    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(vg + chunk_at<C>(k, n) + g4 * 2));
+                    uint32_t lo2, hi2;
+                    e4m3_f16(v, lo2, hi2);
+                    y[0] = f16lo(lo2);
+                    y[1] = f16hi(lo2);
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                      unsigned short v;
+                      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(vg + chunk_at<C>(k, 2 * n + i) + g4 * 2));
+                      y[i] = bf16lo(v);
+                    }
+                  }
+#pragma unroll
+                  for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                      if (see[q][e & 1] && !isfinite(y[e >> 1])) o[q][n][e] += w[q][e & 1] * y[e >> 1];
+                }
+              }
+            }
+          }
+          // P^T as the products' B operand. e4m3: fp16, 11 bits, on values that are exact in fp16. bf16: in two parts
+          // (16 bits of them): one part would add its 2^-9 to the output's own rounding
+          uint32_t hi[NQ][2], lw[NQ][2];
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float y = pw[q][2 * i], z = pw[q][2 * i + 1];
+              const uint32_t w = E4M3 ? pack_f16(y, z) : pack_bf16(y, z);
+              hi[q][i] = transpose8(w);
+              if (!E4M3) lw[q][i] = transpose8(pack_bf16(y - bf16lo(w), z - bf16hi(w)));
+            }
+          constexpr int VI = E4M3 ? KS / 2 : KS, VB4 = VI < 4 ? VI : 4;
+#pragma unroll
+          for (int k0 = 0; k0 < VI; k0 += VB4) {
+            uint32_t r[VB4][4];
+#pragma unroll
+            for (int k = 0; k < VB4; ++k) {
+              ldsm4t(r[k], chunk_from<C>(va, 2 * (k0 + k)));
+              if (odd) finite_only<E4M3>(r[k]);
+            }
+#pragma unroll
+            for (int kk = 0; kk < VB4; ++kk) {
+              if (E4M3) {
+                // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: paired by keys, the even columns of a
+                // chunk are the tile's rows 0-7 and the odd ones its rows 8-15
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  uint32_t a[4];
+                  e4m3_f16(__byte_perm(r[kk][2 * i], 0, 0x3120), a[0], a[1]);
+                  e4m3_f16(__byte_perm(r[kk][2 * i + 1], 0, 0x3120), a[2], a[3]);
+#pragma unroll
+                  for (int q = 0; q < NQ; ++q) mma16<true>(o[q][2 * (k0 + kk) + i], a, hi[q][0], hi[q][1]);
+                }
+              } else {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                  mma16<false>(o[q][k0 + kk], r[kk], hi[q][0], hi[q][1]);
+                  mma16<false>(o[q][k0 + kk], r[kk], lw[q][0], lw[q][1]);
+                }
               }
             }
           }
         }
-        // P^T as the products' B operand. e4m3: fp16, 11 bits, on values that are exact in fp16. bf16: in two parts
-        // (16 bits of them): one part would add its 2^-9 to the output's own rounding
-        uint32_t hi[NQ][2], lw[NQ][2];
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float y = pw[q][2 * i], z = pw[q][2 * i + 1];
-            const uint32_t w = E4M3 ? pack_f16(y, z) : pack_bf16(y, z);
-            hi[q][i] = transpose8(w);
-            if (!E4M3) lw[q][i] = transpose8(pack_bf16(y - bf16lo(w), z - bf16hi(w)));
-          }
-        constexpr int VI = E4M3 ? KS / 2 : KS, VB4 = VI < 4 ? VI : 4;
-#pragma unroll
-        for (int k0 = 0; k0 < VI; k0 += VB4) {
-          uint32_t r[VB4][4];
-#pragma unroll
-          for (int k = 0; k < VB4; ++k) {
-            ldsm4t(r[k], chunk_from<C>(va, 2 * (k0 + k)));
-            if (odd) finite_only<E4M3>(r[k]);
-          }
-#pragma unroll
-          for (int kk = 0; kk < VB4; ++kk) {
-            if (E4M3) {
-              // a register holds columns 2 n, 2 n + 1 of keys 2 c, 2 c + 1: paired by keys, the even columns of a
-              // chunk are the tile's rows 0-7 and the odd ones its rows 8-15
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                uint32_t a[4];
-                e4m3_f16(__byte_perm(r[kk][2 * i], 0, 0x3120), a[0], a[1]);
-                e4m3_f16(__byte_perm(r[kk][2 * i + 1], 0, 0x3120), a[2], a[3]);
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) mma16<true>(o[q][2 * (k0 + kk) + i], a, hi[q][0], hi[q][1]);
-              }
-            } else {
-#pragma unroll
-              for (int q = 0; q < NQ; ++q) {
-                mma16<false>(o[q][k0 + kk], r[kk], hi[q][0], hi[q][1]);
-                mma16<false>(o[q][k0 + kk], r[kk], lw[q][0], lw[q][1]);
-              }
-            }
-          }
+        __syncwarp();  // this warp has read the stage
+        bool freed = true;
+        if (S > 1 && tile > 0) {
+          if (lane == 0) mbar_arrive(&my_empty[stage]);
+        } else if (u.len) {
+          // the team's other warps run on the same block, so they are about done with it too
+          if (S > 1) freed = mbar_wait_warp(&my_empty[stage], phase, &s_abort, p.c.err);
         }
+        --waiting;
+        stage = stage + 1 == p.stages ? 0 : stage + 1;
+        phase ^= stage == 0;
+        if (!freed) {
+          dead = true;
+          break;
+        }
+        if (tile == 0 && u.len) issue();
       }
-      __syncwarp();  // the stage is free
-      --waiting;
-      if (u.len) issue();
-      stage = stage + 1 == p.stages ? 0 : stage + 1;
-      phase ^= stage == 0;
-    }
 
-    // the warps' parts of the item: their maxima and sums here, their outputs below, a tile of eight rows at a time
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        l[q][e] = column_sum(l[q][e]);
-        if (g4 == 0) s_ms[warp * R + q * 8 + 2 * c4 + e] = make_float2(m[q][e], l[q][e]);
-      }
-    }
-    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * part_ld;
-    const int tiles = join ? 1 : (nrow + 7) / 8;
-#pragma unroll 1
-    for (int tile = 0; tile < tiles; ++tile) {
-    if (!join) {
+      // the warps' parts of the item
       const float f = E4M3 ? vtop * (1.f / (1 << kWeightShift)) : 1.f;
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (q != tile || q * 8 + 2 * c4 + e >= p.nr) continue;
-          float* dst = merge + ((size_t)warp * 8 + 2 * c4 + e) * MP;
+          const int r = tile0 + q * 8 + 2 * c4 + e;  // row of the item
+          l[q][e] = column_sum(l[q][e]);
+          if (g4 == 0) s_ms[team * R + r] = make_float2(m[q][e], l[q][e]);
+          if (r >= nrow) continue;
+          float* dst = merge + (size_t)(team * R + r) * MP;
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             if (E4M3) {
@@ -840,25 +852,25 @@ __global__ void __launch_bounds__(C::W * 32, 1)
         }
       __syncthreads();
     }
-    const int r0 = tile * 8, n4 = (join ? nrow : min(8, nrow - r0)) * (D / 4);
+    float* part = p.part + (2 * (size_t)blockIdx.x + (t == c0 ? 0 : 1)) * part_ld;
 #pragma unroll 1
     for (bool again = false;; again = true) {  // again: the thread groups' sums of a join
-      const int team = teams == 1 ? 0 : tid / n4;
+      const int group = groups == 1 ? 0 : tid / n4;
 #pragma unroll 1
-      for (int i = tid - team * n4; i < n4 && team < teams; i += NTHREADS) {
+      for (int i = tid - group * n4; i < n4 && group < groups; i += NTHREADS) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         const float* x = src + (again ? i * 4 : r * pitch + d);
-        const float2* y = ms + (again ? i : r0 + r);
+        const float2* y = ms + (again ? i : r);
         float a = kNoMax, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-        for (int k0 = team; k0 < parts; k0 += V * teams) {
+        for (int k0 = group; k0 < parts; k0 += V * groups) {
           float2 z[V];
           float4 w[V];
           float top = a;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const int k = k0 + j * teams;
+            const int k = k0 + j * groups;
             const size_t off = k ? 0 : skip0;
             z[j] = make_float2(kNoMax, 0.f);
             w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -880,15 +892,15 @@ __global__ void __launch_bounds__(C::W * 32, 1)
             v.x += w[j].x * f; v.y += w[j].y * f; v.z += w[j].z * f; v.w += w[j].w * f;
           }
         }
-        if (teams > 1) {
+        if (groups > 1) {
           *reinterpret_cast<float4*>(merge + tid * 4) = v;
-          s_team[tid] = make_float2(a, sum);
+          s_group[tid] = make_float2(a, sum);
         } else if (split) {
-          *reinterpret_cast<float4*>(part + (r0 + r) * D + d) = v;
-          if (d == 0) *reinterpret_cast<float2*>(part + p.nr * D + 2 * (r0 + r)) = make_float2(a, sum);
+          *reinterpret_cast<float4*>(part + r * D + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(part + p.nr * D + 2 * r) = make_float2(a, sum);
         } else {
           // v / sum as bf16; zeros for rows that see nothing
-          const int row = row0 + r0 + r, tok = token_of(p, row);
+          const int row = row0 + r, tok = token_of(p, row);
           const float g = sum == 0.f || tok >= s.count ? 0.f : __fdividef(1.f, sum);
           if (g == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
           *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * p.group + row - tok * p.group) * p.o_sh +
@@ -896,24 +908,23 @@ __global__ void __launch_bounds__(C::W * 32, 1)
           if (p.lse && d == 0) p.lse[(int64_t)(b * p.c.heads + h) * p.rows + row] = a + log2f(sum);
         }
       }
-      if (teams == 1) break;
+      if (groups == 1) break;
       __syncthreads();
       src = merge;
       src_ld = n4 * 4;
-      ms = s_team;
+      ms = s_group;
       ms_ld = n4;
       skip0 = 0;
-      parts = teams;
-      teams = 1;
+      parts = groups;
+      groups = 1;
     }
     __syncthreads();  // the merge area is free
-    }
     if (!join) t = min(c1, start + it.blocks + kPad);
   }
-  if (dead) {  // see this warp's copies in flight through, again with a limit, before leaving
+  if (dead && tile == 0) {  // see the team's copies in flight through, again with a limit, before leaving
     for (int i = 0; lane == 0 && i < waiting; ++i) {
       volatile int never = 0;
-      mbar_wait(&my_bars[stage], phase, &never, p.c.err);
+      mbar_wait(&my_full[stage], phase, &never, p.c.err);
       stage = stage + 1 == p.stages ? 0 : stage + 1;
       phase ^= stage == 0;
     }
@@ -974,11 +985,11 @@ int tile_map(CUtensorMap* map, void* base, const tbf16_paged_cache* c, int64_t s
 constexpr int kSmemMax = 227 * 1024;
 
 template <class C>
-int attend_smem(const AttendParams& p, int stages) {
-  return C::W * stages * (2 * C::KB + C::SC) + p.merge * 4 + (p.c.batch + 1) * (int)sizeof(SeqInfo);
+int attend_smem(const AttendParams& p) {
+  return C::TEAMS * p.stages * (2 * C::KB + C::SC) + C::MERGE * 4 + (p.c.batch + 1) * (int)sizeof(SeqInfo);
 }
 // Static shared memory of the kernel, rounded up.
-constexpr int kSmemStatic = 5 * 1024;
+constexpr int kSmemStatic = 4 * 1024;
 
 template <class C>
 int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
@@ -988,10 +999,9 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   while ((1 << p.box_shift) < box) ++p.box_shift;
   if (int s = tile_map(&km, cache->k, cache, cache->k_sp, cache->k_sh, cache->k_ss, box)) return s;
   if (int s = tile_map(&vm, cache->v, cache, cache->v_sp, cache->v_sh, cache->v_ss, box)) return s;
-  p.merge = std::max(C::W * 8 * C::MP, C::W * 32 * 4);  // the warps' outputs, or a join's thread groups' sums
-  p.stages = kMaxStages;
-  while (p.stages > 1 && attend_smem<C>(p, p.stages) + kSmemStatic > kSmemMax) --p.stages;
-  const int smem = attend_smem<C>(p, p.stages);
+  static_assert(C::MERGE >= C::W * 32 * 4, "room for a join's thread groups");
+  p.stages = C::MAX_STAGES;
+  const int smem = attend_smem<C>(p);  // a batch of 1024 with 256-wide bf16 rows takes 216 KB
   if (smem + kSmemStatic > kSmemMax) return TBF16_ERR_UNSUPPORTED;
   static const cudaError_t attr =
       cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic);
@@ -999,10 +1009,9 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   return tbf16_host::launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, 1, st, km, vm, p);
 }
 
-// Query rows of an item. Heads with more rows make several items of the same keys, which run at the same time and find
-// them in L2: 32 rows in one item (four tiles; registers spill, and the merge area leaves a single stage) took 100 us
-// where two items take 62 (8 sequences of 32768 tokens, 32 query heads on one key/value head of 128).
-int item_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
+// Query rows of an item. Heads with more than 32 make several items of the same keys,
+// which run at the same time and find most of them in L2.
+int item_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
 struct Workspace {
   int64_t rows, chunks, nr, part, lse, logits;  // sizes in floats, in this order
@@ -1020,8 +1029,14 @@ struct Workspace {
 
 template <int D, bool E4M3>
 int launch_rows(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
-  return item_rows(p.rows) == 8 ? launch_attend<Tile<D, E4M3, 1>>(cache, p, sms, st)
-                                : launch_attend<Tile<D, E4M3, 2>>(cache, p, sms, st);
+  // Up to 16 rows in one warp: a cached fragment is read from shared memory and converted once for both tiles. 256-wide
+  // outputs of two tiles would not fit a warp's registers; there, and for 32 rows, two or four warps share a block
+  // (16 query heads on one of 128, 8 sequences of 32768 tokens: two tiles 39 us, two warps 51; on one of 256: 80 and 68).
+  constexpr bool WIDE = D == 256;
+  const int R = item_rows(p.rows);
+  if (R == 8) return launch_attend<Tile<D, E4M3, 1, 1>>(cache, p, sms, st);
+  if (R == 16) return launch_attend<Tile<D, E4M3, WIDE ? 1 : 2, WIDE ? 2 : 1>>(cache, p, sms, st);
+  return launch_attend<Tile<D, E4M3, WIDE ? 1 : 2, WIDE ? 4 : 2>>(cache, p, sms, st);
 }
 
 bool attend_sizes_ok(const tbf16_paged_cache* c, int64_t Hq, int64_t T) {
