@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   auto key_at = [&](int i) { return p.in_smem ? keys[i - lo] : rank_key(w[i], pos[i], protect_from); };
   uint32_t prefix = 0;
   int need = p.keep;
-  int equal = 0;  // positions whose key is the need-th largest
+  int equal = 0;  // positions whose key, as far as its digits are known, is the need-th largest
+  int low = 32;   // bits of the keys that are not known
   const ClusterScan scan{scan_sums, &cta_sum, ctas, rank};
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
@@ -350,17 +351,18 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
     for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
     if (pass == 0) {
-      for (int i = lo + tid; i < hi; i += 4 * kSelThreads) {
-        float x[4];
-        int y[4];
+      constexpr int V = 8;  // positions that a thread has in flight
+      for (int i = lo + tid; i < hi; i += V * kSelThreads) {
+        float x[V];
+        int y[V];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; ++k) {
           const int j = i + k * kSelThreads;
           x[k] = j < hi ? w[j] : 0.f;
           y[k] = j < hi ? pos[j] : 0;
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; ++k) {
           const int j = i + k * kSelThreads;
           if (j >= hi) break;
           const uint32_t key = rank_key(x[k], y[k], protect_from);
@@ -424,9 +426,12 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
     prefix |= (uint32_t)s_digit << shift;
     need = s_need;
     equal = s_equal;
+    low = shift;
+    if (equal == need) break;  // all of them are kept, whatever their further digits: usual after two passes
   }
-  // `need` of the positions whose key equals `prefix` are kept, the lowest first: where that is not all of them, each
-  // warp has to know how many come before its own
+  prefix >>= low;
+  // `need` of the positions whose key (without its unknown bits) equals `prefix` are kept, the lowest first: where that
+  // is not all of them, each warp has to know how many come before its own
   int2 total;
   int ties_before = 0;
   if (equal == need) {
@@ -434,7 +439,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   } else {
     int ties = 0;
     for (int i = first + lane; i - lane < last; i += 32)
-      ties += __popc(__ballot_sync(0xffffffffu, i < last && key_at(i) == prefix));
+      ties += __popc(__ballot_sync(0xffffffffu, i < last && key_at(i) >> low == prefix));
     ties_before = scan(make_int2(ties, 0), total).x;
   }
   int2* moves = p.moves + (int64_t)bh * p.max_moves;
@@ -449,7 +454,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int i = i0 + k * 32 + lane;
-        key[k] = i < last ? key_at(i) : 0u;
+        key[k] = i < last ? key_at(i) >> low : 0u;
         if (write && i < min(last, p.keep)) {
           x[k] = w[i];
           y[k] = pos[i];
@@ -587,6 +592,6 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
     return rc;
   if (p.inline_moves) return TBF16_OK;
   const int64_t blocks = (p.max_moves + kMoveRows - 1) / kMoveRows;
-  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(blocks, 8 * sms / items));
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(blocks, 16 * sms / items));
   return tbf16_host::launch_pdl(move_kernel, dim3((unsigned)items, (unsigned)splits), 256, 0, 1, st, p);
 }
