@@ -211,7 +211,7 @@ __device__ __forceinline__ uint32_t rank_key(float w, int pos, int protect_from)
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kDigitBits = 11;  // keys are ranked by digits of 11, 11 and 10 bits: the first is sign, exponent and two
 constexpr int kBins = 1 << kDigitBits;  // bits of the weight, so that like weights still spread over several counters
@@ -378,12 +378,14 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
     }
     if (ctas > 1) cluster_sync();
     else __syncthreads();
-    // counts of four bins a thread over the cluster, the highest bins first; the bin in which the need-th key lies.
+    // counts of two bins a thread over the cluster, the highest bins first; the bin in which the need-th key lies.
     // All CTAs' counts are asked for before the first is used.
     constexpr int PB = kBins / kSelThreads;
-    static_assert(PB == 4, "four bins a thread");
+    static_assert(PB == 2, "two bins a thread");
     const int low_bin = kBins - PB - tid * PB;
-    int bin[PB] = {0, 0, 0, 0};
+    int bin[PB], mine = 0;
+#pragma unroll
+    for (int k = 0; k < PB; ++k) bin[k] = 0;
     if (ctas == 1) {
 #pragma unroll
       for (int k = 0; k < PB; ++k) bin[k] = hist[low_bin + PB - 1 - k];
@@ -392,17 +394,17 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
       int y[8][PB];
 #pragma unroll
       for (int c = 0; c < 8; ++c)
-        if (c < ctas)
-          asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(y[c][0]), "=r"(y[c][1]), "=r"(y[c][2]), "=r"(y[c][3])
-                       : "r"(mapa_u32(at, c)));
+        if (c < ctas) {
+          asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(y[c][0]), "=r"(y[c][1]) : "r"(mapa_u32(at, c)));
+        }
 #pragma unroll
       for (int c = 0; c < 8; ++c)
         if (c < ctas)
 #pragma unroll
           for (int k = 0; k < PB; ++k) bin[k] += y[c][PB - 1 - k];
     }
-    const int mine = bin[0] + bin[1] + bin[2] + bin[3];
+#pragma unroll
+    for (int k = 0; k < PB; ++k) mine += bin[k];
     int x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -434,9 +436,10 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   // is not all of them, each warp has to know how many come before its own
   int2 total;
   int ties_before = 0;
-  if (equal == need) {
-    need = INT_MAX;
-  } else {
+  const bool cut = equal != need;
+  const unsigned lane_below = (1u << lane) - 1;
+  auto low_bits = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; };
+  if (cut) {
     int ties = 0;
     for (int i = first + lane; i - lane < last; i += 32)
       ties += __popc(__ballot_sync(0xffffffffu, i < last && key_at(i) >> low == prefix));
@@ -446,13 +449,14 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   int2 before = make_int2(0, 0);  // holes, and kept positions at or beyond `keep`, in the warps before this one
 #pragma unroll 1
   for (int write = 0; write < 2; ++write) {
+    constexpr int V = 4;  // groups of 32 positions in flight
     int tie = ties_before, holes = before.x, loose = before.y;
-    for (int i0 = first; i0 < last; i0 += 128) {
-      float x[4];
-      int y[4];
-      uint32_t key[4];
+    for (int i0 = first; i0 < last; i0 += 32 * V) {
+      float x[V];
+      int y[V];
+      uint32_t key[V];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < V; ++k) {
         const int i = i0 + k * 32 + lane;
         key[k] = i < last ? key_at(i) >> low : 0u;
         if (write && i < min(last, p.keep)) {
@@ -461,24 +465,28 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = i0 + k * 32 + lane;
-        const bool in = i < last;
-        const unsigned below = (1u << lane) - 1, eq = __ballot_sync(0xffffffffu, in && key[k] == prefix);
-        const bool kept = in && (key[k] > prefix || (key[k] == prefix && tie + __popc(eq & below) < need));
-        tie += __popc(eq);
-        const unsigned hb = __ballot_sync(0xffffffffu, in && !kept && i < p.keep);
-        const unsigned lb = __ballot_sync(0xffffffffu, kept && i >= p.keep);
+      for (int k = 0; k < V; ++k) {
+        // the group as bits: positions that exist, lie below `keep`, are kept, are holes, are kept beyond `keep`
+        const int g = i0 + k * 32, i = g + lane;
+        const unsigned in = low_bits(last - g), under = low_bits(p.keep - g);
+        unsigned kept = __ballot_sync(0xffffffffu, key[k] >= prefix) & in;
+        if (cut) {
+          const unsigned eq = __ballot_sync(0xffffffffu, key[k] == prefix) & in;
+          const bool over = ((eq >> lane) & 1) && tie + __popc(eq & lane_below) >= need;
+          kept &= ~__ballot_sync(0xffffffffu, over);
+          tie += __popc(eq);
+        }
+        const unsigned hole = in & under & ~kept, beyond = kept & ~under;
         if (write) {
-          if ((hb >> lane) & 1) moves[holes + __popc(hb & below)].y = i;
-          if ((lb >> lane) & 1) moves[loose + __popc(lb & below)].x = i;
-          if (kept && i < p.keep) {
+          if ((hole >> lane) & 1) moves[holes + __popc(hole & lane_below)].y = i;
+          if ((beyond >> lane) & 1) moves[loose + __popc(beyond & lane_below)].x = i;
+          if (((kept & under) >> lane) & 1) {
             w_out[i] = x[k];
             pos_out[i] = y[k];
           }
         }
-        holes += __popc(hb);
-        loose += __popc(lb);
+        holes += __popc(hole);
+        loose += __popc(beyond);
       }
     }
     if (!write) before = scan(make_int2(holes, loose), total);
@@ -573,12 +581,13 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   p.counts = static_cast<int*>(ws);
   p.moves = reinterpret_cast<int2*>(p.counts + (items + 3) / 4 * 4);
   p.max_moves = (int)compact_max_moves(cols, keep);
-  // CTAs for an item: more while its slices are long and the SMs not full. A cluster's barriers and remote reads cost
-  // about 9 us, which slices of 4096 positions and more win back (128 items of 2112: 17 us with one CTA, 26 with two;
-  // 64 of 16000: 65 / 52 / 50 with 1 / 2 / 4; 8 of 36156: 79 / 52 / 36 / 32 with 1 / 2 / 4 / 8).
+  // CTAs for an item: more while its slices are long and there are SMs for them. A cluster's barriers and remote reads
+  // cost about 9 us, which slices of 4096 positions and more win back (whole calls: 128 items of 2112 positions 17 us
+  // with one CTA, 26 with two; 8 of 36156: 79 / 52 / 36 / 32 with 1 / 2 / 4 / 8); more CTAs than SMs do not pay (64 items of
+  // 16000: 43 us with two, 51 with four).
   const int sms = tbf16_host::device_info()->sms;
   int ctas = 1;
-  while (ctas < 8 && (cols + ctas - 1) / ctas > 4096 && items * ctas * 2 <= 2 * sms) ctas *= 2;
+  while (ctas < 8 && (cols + ctas - 1) / ctas > 4096 && items * ctas * 2 <= sms) ctas *= 2;
   constexpr int kMaxKeys = 48 * 1024;
   while (ctas < 8 && (cols + ctas - 1) / ctas > kMaxKeys) ctas *= 2;
   const int64_t slice = (cols + ctas - 1) / ctas;
