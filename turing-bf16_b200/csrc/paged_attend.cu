@@ -345,11 +345,15 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   }
   // Few rounds: a CTA takes one, so no item waits for another. Else CTA i takes places [share(i), share(i + 1)): `each`
   // of them, the first `more` CTAs one more.
-  // Sequences of one length with few items: as many CTAs for each item, as long as that leaves out no more than one in
-  // twenty; a CTA with the end of one item and the start of the next would have two partials to add up at the end.
+  // Sequences of one length with fewer items than SMs: as many CTAs for each item, so that none has the end of one and
+  // the start of the next to add up and join (128 items of 8000 tokens: 92 us with all SMs, 84 with 128). Leaving SMs
+  // out pays while the others' loads fill the memory's queues: down to four fifths of them, or three where a CTA's bf16
+  // part is up to 2 MB, start and end a large part of its time (96 items of 1 MB: 29 us with all, 26.6 with 96; of
+  // 8000 tokens 72 and 71; of 8000 e4m3 tokens, bound by instructions, 53 and 62).
   const bool by_round = work <= (int)gridDim.x;
   const int items = p.c.batch * p.c.heads * p.chunks, per_item = items <= (int)gridDim.x ? gridDim.x / items : 0;
-  const bool even = !by_round && per_item * items * 20 >= (int)gridDim.x * 19 && (longest + kPad) * items == total;
+  const bool small = !E4M3 && longest <= per_item * ((2 << 20) / (2 * C::KB));
+  const bool even = !by_round && per_item * items * 5 >= (int)gridDim.x * (small ? 3 : 4) && (longest + kPad) * items == total;
   const int ctas = by_round ? work : even ? per_item * items : (int)gridDim.x;
   // sequences without new tokens: zeros
   for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x) {
