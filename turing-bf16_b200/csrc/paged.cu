@@ -91,7 +91,7 @@ __device__ __forceinline__ uint2 e4m3x8(uint4 x, float scale) {
 // D / 8 lanes hold a row, 8 elements each; the 256 D / 8 rows of a pass are 2^tp_log2 tokens (one when decoding) x
 // heads, and a thread goes through the heads with the same kAppendVectors tokens, so that page numbers and offsets
 // are worked out once and a row costs two pointer steps (with both strides multiplied out for each row, the 8-bit
-// form was bound by instructions: 163 a row, 37 us where this takes AAA). Bound by HBM: each row is read once and
+// form was bound by instructions: 163 a row, 37 us where this takes 33). Bound by HBM: each row is read once and
 // written once.
 // An e4m3 row is scaled by 2^(8 - e), e the exponent (frexp) of its largest magnitude, which lands in
 // [128, 256): half the format's range stays unused, none of its precision does, and nothing can saturate.
@@ -198,7 +198,7 @@ struct CompactParams {
   float* w_out;
   int* pos_out;
   int* counts;     // moves of each (sequence, head)
-  int2* moves;     // (from, to): max_moves for each
+  int* moves;      // where they come from, then where they go: max_moves each, for each
   int max_moves;
 };
 
@@ -216,43 +216,64 @@ constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kDigitBits = 11;  // keys are ranked by digits of 11, 11 and 10 bits: the first is sign, exponent and two
 constexpr int kBins = 1 << kDigitBits;  // bits of the weight, so that like weights still spread over several counters
 
-// Exclusive prefix of a pair of counts (the same in all lanes of a warp) over the warps of the cluster, in order of
-// CTA and warp, and the totals.
-struct ClusterScan {
-  int2* warp_sums;  // [kSelWarps]
-  int2* cta_sum;    // one pair that the other CTAs read
-  int ctas, rank;
-  __device__ int2 operator()(int2 v, int2& total) const {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) warp_sums[warp] = v;
-    __syncthreads();
-    const int2 x = lane < kSelWarps ? warp_sums[lane] : make_int2(0, 0);
-    int2 before = sum(lane < warp ? x : make_int2(0, 0));
-    total = sum(x);
-    if (ctas > 1) {
-      if (threadIdx.x == 0) *cta_sum = total;
-      cluster_sync();
-      int2 y = make_int2(0, 0);
-      if (lane < ctas)
-        asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(y.x), "=r"(y.y) : "r"(mapa_u32(smem_u32(cta_sum), lane)));
-      const int2 others = sum(lane < rank ? y : make_int2(0, 0));
-      before.x += others.x;
-      before.y += others.y;
-      total = sum(y);
-      cluster_sync();  // the pair may be written again, or its CTA end
-    } else {
-      __syncthreads();
-    }
-    return before;
-  }
-  static __device__ int2 sum(int2 v) {
-    return make_int2(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y));
-  }
-};
+static_assert(kSelWarps == 32 && kBins == 64 * kSelWarps, "a warp for each group of 64 bins, a lane for each group");
 
-// Makes moves m0, m0 + kMoveRows * stride, ... of an item: looks up the pages of kMoveRows moves (and does their
-// scales, weights and numbers), then streams the rows, 16 bytes a thread, V loads in flight.
-constexpr int kMoveRows = 64;
+// Another CTA's copy of a shared variable.
+__device__ __forceinline__ int ld_cluster(const int* x, int cta) {
+  int y;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(y) : "r"(mapa_u32(smem_u32(x), cta)) : "memory");
+  return y;
+}
+__device__ __forceinline__ int2 ld_cluster2(const int* x, int cta) {
+  int2 y;
+  asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(y.x), "=r"(y.y) : "r"(mapa_u32(smem_u32(x), cta)) : "memory");
+  return y;
+}
+// Inclusive sums over the lanes.
+__device__ __forceinline__ int scan_lanes(int x) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if ((int)(threadIdx.x & 31) >= o) x += y;
+  }
+  return x;
+}
+
+// Exclusive prefix of four counts (the same in all lanes of a warp) over the warps of the cluster, in order of CTA and
+// warp, and the totals.
+__device__ __forceinline__ int4 add4(int4 a, int4 b) { return make_int4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+__device__ __forceinline__ int4 warp_sum(int4 v) {
+  return make_int4(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y),
+                   __reduce_add_sync(0xffffffffu, v.z), __reduce_add_sync(0xffffffffu, v.w));
+}
+__device__ __forceinline__ int4 cluster_scan(int4 v, int ctas, int rank, int4* warp_sums, int4* cta_sum, int4& total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 zero = make_int4(0, 0, 0, 0);
+  if (lane == 0) warp_sums[warp] = v;
+  __syncthreads();
+  const int4 x = lane < kSelWarps ? warp_sums[lane] : zero;
+  int4 before = warp_sum(lane < warp ? x : zero);
+  total = warp_sum(x);
+  if (ctas > 1) {
+    if (threadIdx.x == 0) *cta_sum = total;
+    cluster_sync();
+    int4 y = zero;
+    if (lane < ctas)
+      asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                   : "r"(mapa_u32(smem_u32(cta_sum), lane)));
+    before = add4(before, warp_sum(lane < rank ? y : zero));
+    total = warp_sum(y);
+    cluster_sync();  // no CTA ends while its counts are read
+  }
+  return before;
+}
+
+// Makes moves m0, m0 + kMoveRows * stride, ... of an item: looks up the pages of kMoveRows moves, then streams the
+// rows, 16 bytes a thread, V loads in flight, and last stores the moves' scales, weights and numbers, which come in
+// meanwhile. 84000 moves of 512 bytes with 256 threads: 15 us with 128 rows and four loads; 16.4 with 64 and four, 17.6
+// with 128 and eight, 19.7 with 64 and eight or 32 and four; copying them takes 13 at the HBM rate.
+constexpr int kMoveRows = 128;
 struct MoveScratch {
   int64_t from[2][kMoveRows], to[2][kMoveRows];  // byte offsets of keys, values; -1: not to be copied
 };
@@ -264,23 +285,28 @@ __device__ __forceinline__ void move_rows(const CompactParams& p, int bh, int co
   const int row0 = tid >> (p.row16_log2 + 1), step = THREADS >> (p.row16_log2 + 1);  // rows of a pass
   for (m0 *= kMoveRows; m0 < count; m0 += stride * kMoveRows) {
     const int rows = min(kMoveRows, count - m0);
+    // the move of this thread: its scales, weight and number are on their way while the rows move
+    int2 mv = make_int2(0, 0);
+    float weight = 0.f, ks = 0.f, vs = 0.f;
+    int number = 0;
+    int64_t ks_to = -1, vs_to = 0;
     if (tid < rows) {
-      const int2 mv = p.moves[(int64_t)bh * p.max_moves + m0 + tid];
+      const int* moves = p.moves + (int64_t)bh * 2 * p.max_moves + m0 + tid;
+      mv = make_int2(moves[0], moves[p.max_moves]);
+      weight = p.w[b * p.w_sb + h * p.w_sh + mv.x];
+      number = p.pos[b * p.p_sb + h * p.p_sh + mv.x];
       const int from = paged_page(p.c, b, mv.x), to = paged_page(p.c, b, mv.y);
       const int sf = paged_slot(p.c, mv.x), st = paged_slot(p.c, mv.y);
-      const int64_t out = (int64_t)bh * p.cols + mv.y;
-      p.w_out[out] = p.w[b * p.w_sb + h * p.w_sh + mv.x];
-      p.pos_out[out] = p.pos[b * p.p_sb + h * p.p_sh + mv.x];
       const bool ok = from >= 0 && to >= 0;
       s.from[0][tid] = ok ? from * p.c.k_sp + sf * p.c.k_ss : -1;
       s.from[1][tid] = ok ? from * p.c.v_sp + sf * p.c.v_ss : -1;
       s.to[0][tid] = to * p.c.k_sp + st * p.c.k_ss;
       s.to[1][tid] = to * p.c.v_sp + st * p.c.v_ss;
       if (ok && p.scaled) {
-        float* ks = p.c.k_scale + h * p.c.ks_sh;
-        float* vs = p.c.v_scale + h * p.c.vs_sh;
-        ks[to * p.c.ks_sp + st] = ks[from * p.c.ks_sp + sf];
-        vs[to * p.c.vs_sp + st] = vs[from * p.c.vs_sp + sf];
+        ks = p.c.k_scale[h * p.c.ks_sh + from * p.c.ks_sp + sf];
+        vs = p.c.v_scale[h * p.c.vs_sh + from * p.c.vs_sp + sf];
+        ks_to = h * p.c.ks_sh + to * p.c.ks_sp + st;
+        vs_to = h * p.c.vs_sh + to * p.c.vs_sp + st;
       }
     }
     __syncthreads();
@@ -298,18 +324,29 @@ __device__ __forceinline__ void move_rows(const CompactParams& p, int bh, int co
         if (r < rows && s.from[value][r] >= 0) *reinterpret_cast<uint4*>(pool + s.to[value][r]) = x[k];
       }
     }
+    if (tid < rows) {
+      const int64_t out = (int64_t)bh * p.cols + mv.y;
+      p.w_out[out] = weight;
+      p.pos_out[out] = number;
+      if (ks_to >= 0) {
+        p.c.k_scale[ks_to] = ks;
+        p.c.v_scale[vs_to] = vs;
+      }
+    }
     __syncthreads();
   }
 }
 
 // A cluster of 1 to 8 CTAs per (sequence, head), each with an equal slice of the positions, whose rank keys it keeps
 // in shared memory. The keep-th largest key comes from a radix select over the slices' histograms (read through
-// distributed shared memory); then every warp numbers its holes and the rows that fill them.
+// distributed shared memory); then every warp numbers its holes and the rows that fill them. Bound by the chain of its
+// steps: with four items of 100001 positions on 32 CTAs it takes 20 us, 6 of them to read and rank, 7 for the three
+// digits, 6 to count and list the moves.
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams p) {
   extern __shared__ uint32_t keys[];
-  __shared__ __align__(16) int hist[kBins];
-  __shared__ int warp_sums[kSelWarps];
-  __shared__ int2 scan_sums[kSelWarps], cta_sum;
+  __shared__ __align__(16) int hists[3][kBins];  // one for each digit: no pass waits until all have read the last one's
+  __shared__ int groups[3][kSelWarps];
+  __shared__ int4 scan_sums[kSelWarps], cta_sum;
   __shared__ int s_digit, s_need, s_equal;
   __shared__ MoveScratch scratch;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -344,13 +381,13 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
   int need = p.keep;
   int equal = 0;  // positions whose key, as far as its digits are known, is the need-th largest
   int low = 32;   // bits of the keys that are not known
-  const ClusterScan scan{scan_sums, &cta_sum, ctas, rank};
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
+    int* hist = hists[pass];
     if (pass == 0) {
+      for (int i = tid; i < 3 * kBins; i += kSelThreads) hists[0][i] = 0;
+      __syncthreads();
       constexpr int V = 8;  // positions that a thread has in flight
       for (int i = lo + tid; i < hi; i += V * kSelThreads) {
         float x[V];
@@ -367,64 +404,56 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
           if (j >= hi) break;
           const uint32_t key = rank_key(x[k], y[k], protect_from);
           if (p.in_smem) keys[j - lo] = key;
+          if (j < p.keep) {  // holes among them get another weight and number with their row
+            w_out[j] = x[k];
+            pos_out[j] = y[k];
+          }
           atomicAdd(&hist[key >> 21], 1);
         }
       }
     } else {
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t key = key_at(i);
-        if ((key >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], 1);
+      constexpr int V = 4;
+      for (int i = lo + tid; i < hi; i += V * kSelThreads) {
+        uint32_t key[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) key[k] = i + k * kSelThreads < hi ? key_at(i + k * kSelThreads) : ~prefix;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (((key[k] ^ prefix) >> (shift + bits)) == 0) atomicAdd(&hist[(key[k] >> shift) & ((1 << bits) - 1)], 1);
       }
     }
+    // The bin in which the need-th key lies, the highest first. Every warp adds up one of 32 groups of 64 bins, then
+    // warp 0 finds the group in the sums of all CTAs, and the bin in the group's counts: 320 bytes from each CTA (8 KB
+    // from each, all bins at once, took 2.5 us of a pass where this takes 1.5).
+    __syncthreads();
+    const int2 pair = reinterpret_cast<const int2*>(hist)[tid];
+    const int group_sum = __reduce_add_sync(0xffffffffu, pair.x + pair.y);
+    if (lane == 0) groups[pass][warp] = group_sum;
     if (ctas > 1) cluster_sync();
     else __syncthreads();
-    // counts of two bins a thread over the cluster, the highest bins first; the bin in which the need-th key lies.
-    // All CTAs' counts are asked for before the first is used.
-    constexpr int PB = kBins / kSelThreads;
-    static_assert(PB == 2, "two bins a thread");
-    const int low_bin = kBins - PB - tid * PB;
-    int bin[PB], mine = 0;
-#pragma unroll
-    for (int k = 0; k < PB; ++k) bin[k] = 0;
-    if (ctas == 1) {
-#pragma unroll
-      for (int k = 0; k < PB; ++k) bin[k] = hist[low_bin + PB - 1 - k];
-    } else {
-      const uint32_t at = smem_u32(hist + low_bin);
-      int y[8][PB];
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c < ctas) {
-          asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(y[c][0]), "=r"(y[c][1]) : "r"(mapa_u32(at, c)));
-        }
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c < ctas)
-#pragma unroll
-          for (int k = 0; k < PB; ++k) bin[k] += y[c][PB - 1 - k];
-    }
-#pragma unroll
-    for (int k = 0; k < PB; ++k) mine += bin[k];
-    int x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    int above = x - mine + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane & (kSelWarps - 1)] : 0);
-#pragma unroll
-    for (int k = 0; k < PB; ++k) {
-      if (above < need && need <= above + bin[k]) {
-        s_digit = kBins - 1 - (tid * PB + k);
-        s_need = need - above;
-        s_equal = bin[k];
+    if (warp == 0) {
+      int x = 0, a = 0, b = 0;  // lane 0: the highest group, then the highest two bins
+#pragma unroll 8
+      for (int c = 0; c < ctas; ++c) x += ld_cluster(&groups[pass][31 - lane], c);
+      int above = scan_lanes(x) - x;
+      const int at = 31 - (__ffs(__ballot_sync(0xffffffffu, above + x >= need)) - 1);  // the first that reaches `need`
+      above = __shfl_sync(0xffffffffu, above, 31 - at);
+#pragma unroll 8
+      for (int c = 0; c < ctas; ++c) {
+        const int2 y = ld_cluster2(&hist[64 * at + 62 - 2 * lane], c);
+        a += y.y;
+        b += y.x;
       }
-      above += bin[k];
+      above += scan_lanes(a + b) - a - b;
+      const int bin = 64 * at + 63 - 2 * lane;
+      if (above < need && need <= above + a + b) {
+        const bool second = need > above + a;
+        s_digit = bin - second;
+        s_need = need - above - (second ? a : 0);
+        s_equal = second ? b : a;
+      }
     }
-    if (ctas > 1) cluster_sync();  // every CTA has read the histograms
-    else __syncthreads();
+    __syncthreads();
     prefix |= (uint32_t)s_digit << shift;
     need = s_need;
     equal = s_equal;
@@ -432,70 +461,69 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const CompactParams
     if (equal == need) break;  // all of them are kept, whatever their further digits: usual after two passes
   }
   prefix >>= low;
-  // `need` of the positions whose key (without its unknown bits) equals `prefix` are kept, the lowest first: where that
-  // is not all of them, each warp has to know how many come before its own
-  int2 total;
-  int ties_before = 0;
+  // Positions with a larger key than `prefix` (without the unknown bits) are kept, and `need` of those with an equal one,
+  // the lowest first. Four counts of what comes before a warp tell it the rest: those above and those at the cut, below
+  // `keep` and from there on.
   const bool cut = equal != need;
-  const unsigned lane_below = (1u << lane) - 1;
-  auto low_bits = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; };
-  if (cut) {
-    int ties = 0;
-    for (int i = first + lane; i - lane < last; i += 32)
-      ties += __popc(__ballot_sync(0xffffffffu, i < last && key_at(i) >> low == prefix));
-    ties_before = scan(make_int2(ties, 0), total).x;
-  }
-  int2* moves = p.moves + (int64_t)bh * p.max_moves;
-  int2 before = make_int2(0, 0);  // holes, and kept positions at or beyond `keep`, in the warps before this one
-#pragma unroll 1
-  for (int write = 0; write < 2; ++write) {
-    constexpr int V = 4;  // groups of 32 positions in flight
-    int tie = ties_before, holes = before.x, loose = before.y;
-    for (int i0 = first; i0 < last; i0 += 32 * V) {
-      float x[V];
-      int y[V];
-      uint32_t key[V];
+  auto count = [&](int from, int to, int& above, int& at) {
+    constexpr int V = 4;  // keys in flight
+    for (int i = from + lane; i < to; i += 32 * V) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const int i = i0 + k * 32 + lane;
-        key[k] = i < last ? key_at(i) >> low : 0u;
-        if (write && i < min(last, p.keep)) {
-          x[k] = w[i];
-          y[k] = pos[i];
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        // the group as bits: positions that exist, lie below `keep`, are kept, are holes, are kept beyond `keep`
-        const int g = i0 + k * 32, i = g + lane;
-        const unsigned in = low_bits(last - g), under = low_bits(p.keep - g);
-        unsigned kept = __ballot_sync(0xffffffffu, key[k] >= prefix) & in;
-        if (cut) {
-          const unsigned eq = __ballot_sync(0xffffffffu, key[k] == prefix) & in;
-          const bool over = ((eq >> lane) & 1) && tie + __popc(eq & lane_below) >= need;
-          kept &= ~__ballot_sync(0xffffffffu, over);
-          tie += __popc(eq);
-        }
-        const unsigned hole = in & under & ~kept, beyond = kept & ~under;
-        if (write) {
-          if ((hole >> lane) & 1) moves[holes + __popc(hole & lane_below)].y = i;
-          if ((beyond >> lane) & 1) moves[loose + __popc(beyond & lane_below)].x = i;
-          if (((kept & under) >> lane) & 1) {
-            w_out[i] = x[k];
-            pos_out[i] = y[k];
-          }
-        }
-        holes += __popc(hole);
-        loose += __popc(beyond);
+        const int j = i + k * 32;
+        const uint32_t key = j < to ? key_at(j) >> low : 0;
+        above += key > prefix;
+        at += j < to && key == prefix;
       }
     }
-    if (!write) before = scan(make_int2(holes, loose), total);
+  };
+  int4 mine4 = make_int4(0, 0, 0, 0), total;
+  count(first, min(last, p.keep), mine4.x, mine4.y);
+  count(max(first, p.keep), last, mine4.z, mine4.w);
+  const int4 before = cluster_scan(warp_sum(mine4), ctas, rank, scan_sums, &cta_sum, total);
+  const int moved = p.keep - total.x - min(need, total.y);
+  int tie = before.y + before.w;
+  int holes = min(first, p.keep) - before.x - min(need, before.y);
+  int loose = before.z + min(need, tie) - min(need, before.y);
+  int* from = p.moves + (int64_t)bh * 2 * p.max_moves;
+  int* to = from + p.max_moves;
+  const unsigned lane_below = (1u << lane) - 1;
+  auto low_bits = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; };
+  constexpr int V = 4;  // groups of 32 positions in flight
+  for (int i0 = first; i0 < last; i0 += 32 * V) {
+    uint32_t key[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int i = i0 + k * 32 + lane;
+      key[k] = i < last ? key_at(i) >> low : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      // the group as bits: positions that exist, are kept, lie below `keep`
+      const int g = i0 + k * 32, i = g + lane;
+      const unsigned in = low_bits(last - g), under = low_bits(p.keep - g);
+      unsigned kept = __ballot_sync(0xffffffffu, key[k] >= prefix) & in;
+      if (cut) {
+        const unsigned eq = __ballot_sync(0xffffffffu, key[k] == prefix) & in;
+        const bool over = ((eq >> lane) & 1) && tie + __popc(eq & lane_below) >= need;
+        kept &= ~__ballot_sync(0xffffffffu, over);
+        tie += __popc(eq);
+      }
+      if (under) {
+        const unsigned hole = in & under & ~kept;
+        if ((hole >> lane) & 1) to[holes + __popc(hole & lane_below)] = i;
+        holes += __popc(hole);
+      }
+      const unsigned beyond = kept & ~under;
+      if ((beyond >> lane) & 1) from[loose + __popc(beyond & lane_below)] = i;
+      loose += __popc(beyond);
+    }
   }
   if (p.inline_moves) {  // one CTA, few moves: made here
     __syncthreads();
-    move_rows<kSelThreads, 4>(p, bh, total.x, 0, 1, scratch);
+    move_rows<kSelThreads, 4>(p, bh, moved, 0, 1, scratch);
   } else if (rank == 0 && tid == 0) {
-    p.counts[bh] = total.x;
+    p.counts[bh] = moved;
   }
 }
 
@@ -504,7 +532,7 @@ __global__ void __launch_bounds__(256) move_kernel(const CompactParams p) {
   __shared__ MoveScratch scratch;
   pdl_launch_dependents();
   pdl_wait();
-  move_rows<256, 8>(p, blockIdx.x, p.counts[blockIdx.x], blockIdx.y, gridDim.y, scratch);
+  move_rows<256, 4>(p, blockIdx.x, p.counts[blockIdx.x], blockIdx.y, gridDim.y, scratch);
 }
 
 }  // namespace
@@ -549,7 +577,7 @@ int64_t compact_max_moves(int64_t cols, int64_t keep) { return std::max<int64_t>
 extern "C" int64_t tbf16_paged_compact_ws_size(const tbf16_paged_cache* cache, int64_t cols, int64_t keep) {
   if (!cache || cache->batch < 0 || cache->heads < 1 || cols < 0 || keep < 0) return 0;
   const int64_t items = cache->batch * cache->heads;
-  return items * compact_max_moves(cols, keep) * (int64_t)sizeof(int2) + (items + 3) / 4 * 4 * (int64_t)sizeof(int);
+  return items * compact_max_moves(cols, keep) * 2 * (int64_t)sizeof(int) + (items + 3) / 4 * 4 * (int64_t)sizeof(int);
 }
 
 extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* weights, int64_t w_sb, int64_t w_sh,
@@ -579,12 +607,11 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   p.w_out = weights_out;
   p.pos_out = pos_out;
   p.counts = static_cast<int*>(ws);
-  p.moves = reinterpret_cast<int2*>(p.counts + (items + 3) / 4 * 4);
+  p.moves = p.counts + (items + 3) / 4 * 4;
   p.max_moves = (int)compact_max_moves(cols, keep);
-  // CTAs for an item: more while its slices are long and there are SMs for them. A cluster's barriers and remote reads
-  // cost about 9 us, which slices of 4096 positions and more win back (whole calls: 128 items of 2112 positions 17 us
-  // with one CTA, 26 with two; 8 of 36156: 79 / 52 / 36 / 32 with 1 / 2 / 4 / 8); more CTAs than SMs do not pay (64 items of
-  // 16000: 43 us with two, 51 with four).
+  // CTAs for an item: more while its slices are long and there are SMs for them. Whole calls with 1 / 2 / 4 / 8 CTAs:
+  // 8 items of 36156 positions 46 / 36 / 32 / 26 us, of 9000 17.8 / 17.3 / 16.8 / 18.6, of 4200 13.9 / 14.1 / 14.3 / 14.4.
+  // More CTAs than SMs do not pay: 64 items of 16000 57 / 54 / 63 / 87, 128 of 2112 9 / 22 / 41 / 73.
   const int sms = tbf16_host::device_info()->sms;
   int ctas = 1;
   while (ctas < 8 && (cols + ctas - 1) / ctas > 4096 && items * ctas * 2 <= sms) ctas *= 2;
@@ -592,8 +619,9 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   while (ctas < 8 && (cols + ctas - 1) / ctas > kMaxKeys) ctas *= 2;
   const int64_t slice = (cols + ctas - 1) / ctas;
   p.in_smem = slice <= kMaxKeys;
-  p.inline_moves = ctas == 1 && p.max_moves <= 2 * kMoveRows;
-  static const cudaError_t attr = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
+  p.inline_moves = ctas == 1 && p.max_moves <= kMoveRows;
+  static const cudaError_t attr = cudaFuncSetAttribute(
+      select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
   if (attr != cudaSuccess || items * ctas > INT32_MAX) return TBF16_ERR_LAUNCH;
   auto st = static_cast<cudaStream_t>(stream);
   if (int rc = tbf16_host::launch_pdl(select_kernel, dim3((unsigned)(items * ctas)), kSelThreads,
