@@ -72,32 +72,42 @@ struct AppendParams {
   int64_t pos_sb, pos_sh;
   int T, d8;       // d8: source row length in 8-element vectors
   int tp_log2;     // log2 of the tokens of a pass
-  int tiles;       // blocks of a sequence, kAppendVectors passes of tokens each
+  int tiles;       // blocks of a sequence, V passes of tokens each
   int block_heads; // heads of a block
 };
-constexpr int kAppendVectors = 4;  // rows that a thread has in flight
+// What a thread has in flight: N vectors of each of V rows. (Four rows of bf16 take as long for prompts, and 3.5 us in place
+// of 2.6 for one token of 64 sequences.)
+template <int D_, bool E4M3_>
+struct AppendTile {
+  static constexpr int D = D_;
+  static constexpr bool E4M3 = E4M3_;
+  static constexpr int N = E4M3 ? 2 : 1, V = 2;
+  static constexpr int LR = D / 8 / N, ROWS = 256 / LR;  // lanes of a row, rows of a pass
+};
 
-// Eight bf16 values times `scale` (a power of two: exact short of e4m3's range) rounded to nearest-even e4m3.
-__device__ __forceinline__ uint2 e4m3x8(uint4 x, float scale) {
+// Eight bf16 values times `scale` (a power of two: exact in bf16 as far as e4m3 tells the products from zero) rounded
+// to nearest-even e4m3.
+__device__ __forceinline__ uint2 e4m3x8(uint4 x, __nv_bfloat162 scale) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   uint32_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(bf16lo(w[i]) * scale, bf16hi(w[i]) * scale), __NV_SATFINITE, __NV_E4M3);
+    h[i] = __nv_cvt_float2_to_fp8x2(__bfloat1622float2(__hmul2(reinterpret_cast<const __nv_bfloat162&>(w[i]), scale)),
+                                    __NV_SATFINITE, __NV_E4M3);
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
 // A block copies the rows of some tokens and heads of one sequence to their slots; blockIdx.y picks keys or values.
-// D / 8 lanes hold a row, 8 elements each; the 256 D / 8 rows of a pass are 2^tp_log2 tokens (one when decoding) x
-// heads, and a thread goes through the heads with the same kAppendVectors tokens, so that page numbers and offsets
-// are worked out once and a row costs two pointer steps (with both strides multiplied out for each row, the 8-bit
-// form was bound by instructions: 163 a row, 37 us where this takes 33). Bound by HBM: each row is read once and
-// written once.
+// LR lanes hold a row, N vectors of 8 elements each; the ROWS rows of a pass are 2^tp_log2 tokens (one when decoding) x
+// heads, and a thread goes through the heads with the same V tokens, so that page numbers and offsets are worked out
+// once and a row costs two pointer steps. Bound by HBM, the 8-bit form by its instructions as well (8 x 8 heads of 128
+// elements, up to 4096 tokens: 23 us; 33 with one vector of each of four rows, whose maxima and scales take twice as
+// many, 37 with both strides multiplied out for each row). Each row is read once and written once.
 // An e4m3 row is scaled by 2^(8 - e), e the exponent (frexp) of its largest magnitude, which lands in
 // [128, 256): half the format's range stays unused, none of its precision does, and nothing can saturate.
-template <int D, bool E4M3>
+template <class A>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  constexpr int LR = D / 8, V = kAppendVectors, ROWS = 256 / LR;
+  constexpr int LR = A::LR, V = A::V, N = A::N, ROWS = A::ROWS;
   const int kv = blockIdx.y, chunk = threadIdx.x % LR, row = threadIdx.x / LR;
   const int b = (int)(blockIdx.x / (unsigned)p.tiles), tp = 1 << p.tp_log2;
   const int t0 = (int)(blockIdx.x % (unsigned)p.tiles) * (V * tp) + (row & (tp - 1));
@@ -118,8 +128,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
     live |= (page >= 0) << i;
     src[i] = p.src[kv] + b * p.sb[kv] + h0 * p.sh[kv] + t * p.st[kv] + chunk * 8;
     dst[i] = (kv ? p.c.v + page * p.c.v_sp + slot * p.c.v_ss : p.c.k + page * p.c.k_sp + slot * p.c.k_ss) + h0 * sh +
-             chunk * (E4M3 ? 8 : 16);
-    if (E4M3) scale[i] = (kv ? p.c.v_scale + page * p.c.vs_sp : p.c.k_scale + page * p.c.ks_sp) + h0 * ssh + slot;
+             chunk * (A::E4M3 ? 8 : 16);
+    if (A::E4M3) scale[i] = (kv ? p.c.v_scale + page * p.c.vs_sp : p.c.k_scale + page * p.c.ks_sp) + h0 * ssh + slot;
     if (p.pos && page >= 0 && kv == 0 && chunk == 0)
       for (int h = h0; h < h1; h += hp) p.pos[b * p.pos_sb + h * p.pos_sh + j] = p.seen[b] - n + t;
   }
@@ -127,19 +137,24 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 #pragma unroll 1
   for (int k = 0, h = h0; k < passes; ++k, h += hp) {
     if (h >= h1) live = 0;
-    uint4 x[V];
+    uint4 x[V][N];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (((live >> i) & 1) && chunk < p.d8) x[i] = __ldcs(reinterpret_cast<const uint4*>(src[i]));
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        x[i][c] = make_uint4(0, 0, 0, 0);
+        if (((live >> i) & 1) && chunk + c * LR < p.d8) x[i][c] = __ldcs(reinterpret_cast<const uint4*>(src[i]) + c * LR);
+      }
       src[i] += hp * p.sh[kv];
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (E4M3) {
+      if (A::E4M3) {
         // the largest magnitude as bits, ordered like the values with infinity and NaN on top; two in a register
         unsigned m = 0;
-        for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) m = __vmaxu2(m, w & 0x7fff7fffu);
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+          for (uint32_t w : {x[i][c].x, x[i][c].y, x[i][c].z, x[i][c].w}) m = __vmaxu2(m, w & 0x7fff7fffu);
 #pragma unroll
         for (int o = LR / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
         m = max(m << 16, m & 0xffff0000u);
@@ -147,26 +162,26 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
         // its frexp exponent; at least -118 (2^-119), so that 2^(8 - e) and 2^(e - 8) are normal: smaller rows round
         // to e4m3's subnormals
         const int e = m == 0 || !finite ? 8 : (int)(max(m, 8u << 23) >> 23) - 126;
-        const uint2 y = e4m3x8(x[i], __uint_as_float((unsigned)(135 - e) << 23));
+        const __nv_bfloat162 up = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)((135 - e) << 7)));
         if ((live >> i) & 1) {
-          *reinterpret_cast<uint2*>(dst[i]) = y;
+#pragma unroll
+          for (int c = 0; c < N; ++c) *(reinterpret_cast<uint2*>(dst[i]) + c * LR) = e4m3x8(x[i][c], up);
           if (chunk == 0) *scale[i] = __uint_as_float(finite ? (unsigned)(119 + e) << 23 : 0x7fc00000u);
         }
         scale[i] += hp * ssh;
       } else if ((live >> i) & 1) {
-        *reinterpret_cast<uint4*>(dst[i]) = x[i];
+        *reinterpret_cast<uint4*>(dst[i]) = x[i][0];
       }
       dst[i] += hp * sh;
     }
   }
 }
 
-template <int D>
-int launch_append(AppendParams& p, bool e4m3, cudaStream_t st) {
-  constexpr int ROWS = 256 / (D / 8);
+template <class A>
+int launch_append(AppendParams& p, cudaStream_t st) {
   p.tp_log2 = 0;
-  while ((2 << p.tp_log2) <= std::min(p.T, ROWS)) ++p.tp_log2;
-  const int tokens = kAppendVectors << p.tp_log2, hp = ROWS >> p.tp_log2, passes = (p.c.heads + hp - 1) / hp;
+  while ((2 << p.tp_log2) <= std::min(p.T, A::ROWS)) ++p.tp_log2;
+  const int tokens = A::V << p.tp_log2, hp = A::ROWS >> p.tp_log2, passes = (p.c.heads + hp - 1) / hp;
   p.tiles = (p.T + tokens - 1) / tokens;
   const int64_t blocks = (int64_t)p.c.batch * p.tiles;
   if (blocks > INT32_MAX) return TBF16_ERR_INVALID;
@@ -174,9 +189,13 @@ int launch_append(AppendParams& p, bool e4m3, cudaStream_t st) {
   const int sms = tbf16_host::device_info()->sms;
   const int64_t k = std::max<int64_t>(1, std::min<int64_t>(passes, 2 * blocks * passes / (4 * sms)));
   p.block_heads = (int)k * hp;
-  return tbf16_host::launch_pdl(e4m3 ? append_kernel<D, true> : append_kernel<D, false>,
+  return tbf16_host::launch_pdl(append_kernel<A>,
                                 dim3((unsigned)blocks, 2, (unsigned)((p.c.heads + p.block_heads - 1) / p.block_heads)), 256, 0,
                                 1, st, p);
+}
+template <int D>
+int launch_append(AppendParams& p, bool e4m3, cudaStream_t st) {
+  return e4m3 ? launch_append<AppendTile<D, true>>(p, st) : launch_append<AppendTile<D, false>>(p, st);
 }
 
 // ------------------------------------------------------------------ compact
