@@ -17,11 +17,13 @@ using namespace tbf16;
 // Work split. The keys of a (sequence, head, query rows) item are cut into blocks of BK keys; the blocks of all
 // items, laid end to end, are shared out evenly over the CTAs (one per SM), from the lengths on the device:
 // ragged batches and one long sequence keep all SMs equally busy, and a captured graph follows the lengths. A
-// CTA's blocks go round-robin to its warps. Each warp is a pipeline of its own: it issues the TMA loads of its
-// blocks into its own ring of stages, waits for them, and keeps its own running maximum, sum and output in
-// registers, so the warps never wait for one another inside an item. At its end they are added up through shared
-// memory. An item that spans CTAs leaves one partial (output, maximum, sum) per CTA in the workspace; the CTA
-// that arrives last adds them in a fixed order, so results do not depend on which one that is.
+// CTA's blocks go round-robin to its teams, of one warp each unless an item has more query rows than a warp's
+// registers hold outputs for: then the warps of a team read the same blocks, each for its own rows. A team is a
+// pipeline of its own: it issues the TMA loads of its blocks into its own ring of stages, waits for them, and its
+// warps keep their running maximum, sum and output in registers, so teams never wait for one another inside an
+// item. At its end they are added up through shared memory. An item that spans CTAs leaves one partial (output,
+// maximum, sum) per CTA in the workspace; the CTA that arrives last adds them in a fixed order, so results do not
+// depend on which one that is.
 //
 // Tiles. mma.sync m16n8k16 with the cache as the 16-row operand and eight query rows as columns: S^T = K Q^T,
 // O^T = V^T P^T. With the usual group of up to eight query rows no product is wasted on empty rows (a 16-row
