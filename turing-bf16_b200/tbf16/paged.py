@@ -332,8 +332,7 @@ class PagedCache:
         if size is None:
             size = self._sizes[keep] = int(self._lib.tbf16_paged_compact_ws_size(c.ref, cols, keep))
         shape = c.weights.shape
-        weights = torch.empty(shape, device=self.device)
-        pos = torch.empty(shape, device=self.device, dtype=torch.int32)
+        weights, pos = c.weights.new_empty(shape), c.pos.new_empty(shape)
         stream = torch._C._cuda_getCurrentRawStream(self.device.index)
         buf = self._scratch(stream, 0, size)
         self._run(self._lib.tbf16_paged_compact, "compact", c.ref, *c.weight_args, *c.pos_args[:3], cols, c.pos_args[3], keep,
