@@ -408,6 +408,45 @@ def test_compact(lens, keep, recent, kind, D, bits, page, layout):
     assert _ext.device_status() == 0
 
 
+@pytest.mark.parametrize("cols", [49152, 49153])
+def test_compact_of_many_items_with_long_slices(cols):
+    """More items than half the SMs have no clusters: one CTA ranks all positions, as many as its shared memory
+    holds, or (one more) a pair does. Every kept row is found by its number."""
+    import tbf16
+    from tbf16 import _ext
+    B, page, keep, recent = 75, 64, 9000, 100
+    lens = [cols, cols - 5] + [90] * (B - 2)
+    need, cap = [-(-n // page) for n in lens], -(-cols // page)
+    order = torch.randperm(sum(need), generator=torch.Generator().manual_seed(1)).to(torch.int32).split(need)
+    table = torch.zeros(B, cap, dtype=torch.int32)
+    for b, pages in enumerate(order):
+        table[b, :need[b]] = pages
+    g = torch.Generator(device=DEV).manual_seed(2)
+    k, v = (torch.randn(sum(need), 1, page, 64, generator=g, device=DEV).bfloat16() for _ in range(2))
+    w = torch.exp(torch.randn(B, 1, cap * page, generator=g, device=DEV))
+    pos = torch.arange(cap * page, dtype=torch.int32, device=DEV).expand(B, 1, -1).contiguous()
+    ints = dict(dtype=torch.int32, device=DEV)
+    cache = tbf16.PagedCache.over(k, v, table.to(DEV), torch.tensor(lens, **ints), weights=w, pos=pos,
+                                  seen=torch.tensor(lens, **ints))
+    rows = lambda x, b, n: x[table[b].long().to(DEV), 0].reshape(-1, 64)[:n]  # noqa: E731
+    old = [[rows(x, b, lens[b]).clone() for x in (k, v)] for b in range(3)]
+    new_w, new_pos = cache.compact(keep, recent)
+    for b in range(B):
+        n, m = lens[b], min(lens[b], keep)
+        rank = w[b, 0, :n].double()
+        rank[n - recent if n > recent else 0:] = math.inf
+        kept = torch.zeros(n, dtype=torch.bool, device=DEV)
+        kept[torch.sort(rank, descending=True, stable=True).indices[:m]] = True
+        number = new_pos[b, 0, :m].long()
+        stay = torch.arange(m, device=DEV)
+        assert torch.equal(number.sort().values, kept.nonzero()[:, 0])
+        assert torch.equal(number[kept[:m]], stay[kept[:m]]) and bool((number[~kept[:m]].diff() > 0).all())
+        assert torch.equal(new_w[b, 0, :m], w[b, 0, number]) and not new_w[b, 0, m:].any() and bool((new_pos[b, 0, m:] == -1).all())
+        if b < len(old):
+            assert all(torch.equal(rows(x, b, m), y[number]) for x, y in zip((k, v), old[b]))
+    assert _ext.device_status() == 0
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
 @pytest.mark.parametrize("head_dim", [64, 80, 256])
 def test_cache_decodes_like_attention_over_everything(dtype, head_dim):
