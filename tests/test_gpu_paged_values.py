@@ -1,0 +1,95 @@
+"""What attend makes of values and scales at the ends of their range, against 64-bit arithmetic: rows of zeros, rows
+whose scales lie far apart, infinities and NaNs that are seen. Tolerances are those of test_gpu_paged (Case.exact): one
+bf16 ulp, the logits' and weights' relative errors, and for an 8-bit cache fp16's floor, taken of the largest
+*weighted* value row."""
+import math
+
+import pytest
+import torch
+
+from helpers import bf16_ulp
+from test_gpu_paged import DEV, Case
+
+pytestmark = pytest.mark.gpu
+
+
+def _set_values(case, b, j, factor=None, zero=False):
+    """Position j of sequence b, all heads: its value row times `factor` (by its scale, exactly), or zeros as append
+    writes them (scale 1)."""
+    page, slot = int(case.table[b, j // case.page]), j % case.page
+    if zero:
+        case.v.view(torch.uint8)[page, :, slot] = 0
+        case.v_scale[page, :, slot] = 1.0
+        case.v64[b, :, j] = 0.0
+    else:
+        case.v_scale[page, :, slot] *= factor
+        case.v64[b, :, j] *= factor
+
+
+def _set_keys(case, b, j, rows):
+    """Position j of sequence b: its key rows (heads, D), of at most 448, as e4m3 with scale 1."""
+    page, slot = int(case.table[b, j // case.page]), j % case.page
+    x = rows.to(torch.float8_e4m3fn)
+    case.k.view(torch.uint8)[page, :, slot] = x.view(torch.uint8).to(DEV)
+    case.k_scale[page, :, slot] = 1.0
+    case.k64[b, :, j] = x.double()
+
+
+def _check(case, q, window=0, counts=None):
+    from tbf16 import _ext
+    dc = None if counts is None else torch.tensor(counts, dtype=torch.int32, device=DEV)
+    out = case.cache().attend(q, window=window, counts=dc).cpu().double()
+    ref, tol, _, _ = case.exact(q, counts, window)
+    err = (out - ref).abs()
+    assert bool((err <= tol).all()), f"max excess {(err - tol).max().item():.3e}, {((err > tol).double().mean()):.3f} of all"
+    assert _ext.device_status() == 0
+
+
+@pytest.mark.parametrize("magnitude", [2.0 ** -8, 2.0 ** -16, 2.0 ** -24, 2.0 ** -60])
+@pytest.mark.parametrize("D,Hq,T", [(64, 4, 1), (128, 16, 1), (256, 4, 4), (256, 64, 1)])
+def test_zero_value_rows_leave_the_others_their_bits(magnitude, D, Hq, T):
+    """A zero row has scale 1, however small the rows beside it are."""
+    lens = [50, 400, 33]
+    for zeros in ([0], [17, 18], [49, 300, 399]):
+        case = Case(lens, 2, D, 16, 8, seed=D)
+        for b, n in enumerate(lens):
+            for j in range(n):
+                _set_values(case, b, j, factor=magnitude)
+            for j in zeros:
+                if j < n:
+                    _set_values(case, b, j, zero=True)
+        _check(case, case.queries(Hq, T))
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 20, 2.0 ** 30])
+@pytest.mark.parametrize("light", ["first", "front", "middle", "last", "all but one", "every third"])
+@pytest.mark.parametrize("D", [64, 256])
+def test_large_rows_of_little_weight_leave_the_others_their_bits(ratio, light, D):
+    """Keys that the first query row of a head hardly sees (their logits lie about 45 below) and whose value rows are
+    `ratio` times as large; the second row, the negated query, sees little else."""
+    lens = [300, 41]
+    case = Case(lens, 2, D, 16, 8, seed=3, gain=0.25)
+    q = case.queries(4, 1)
+    q[:, 1::2] = -q[:, ::2]
+    for b, n in enumerate(lens):
+        at = {"first": [0], "front": range(40), "middle": [n // 2], "last": [n - 1], "all but one": range(n - 1),
+              "every third": range(0, n, 3)}[light]
+        for j in at:
+            x = q[b, ::2, 0].cpu().double()
+            _set_keys(case, b, j, (-45 * math.sqrt(D) * x / x.square().sum(-1, keepdim=True)).float())
+            _set_values(case, b, j, factor=ratio)
+    _check(case, q)
+    if light != "all but one":
+        _check(case, q, window=35)
+
+
+def test_scales_of_either_sign():
+    """A caller's scales need not be positive."""
+    lens = [100, 17]
+    case = Case(lens, 2, 128, 16, 8)
+    for b, n in enumerate(lens):
+        for j in range(n):
+            if j % 3 != 1 or j < 16:
+                _set_values(case, b, j, factor=-1.0)
+    _check(case, case.queries(4, 1))
+    _check(case, case.queries(4, 3))

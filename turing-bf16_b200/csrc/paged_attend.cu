@@ -265,9 +265,14 @@ struct Loader {
 // output is rescaled, a few times per item and not with every block, and no lane has to ask the others for it.
 constexpr float kSlack = 8.f;
 constexpr float kNoMax = -3.4028234e38f;  // of a row that has seen nothing: every logit is far above it
-// e4m3: the weights that multiply the values carry the value row's scale over a power of two that is at least
-// the largest scale met so far, times 2^7: at most 2^15 in fp16 (2^kSlack 2^7), with 29 bits below that.
+// e4m3: the weights that multiply the values carry the value row's scale over the query row's `vtop`, times 2^7: at most
+// 2^15 in fp16 (2^kSlack 2^7) while scales stay within vtop, and rounded to 11 bits down to 2^-14. vtop follows the
+// scales, four times the largest so far, but not further than 2^kRange times the largest weighted scale that the row
+// has met at a change of its maximum: else one key with a large value row, of no weight, would push the weights that
+// count into fp16's subnormals. So the largest weighted scale stays at 2^(7 - kRange) or more, and what fp16's smallest
+// step loses below 2^-20 of it. Groups with scales beyond vtop are looked at key by key.
 constexpr int kWeightShift = 7;
+constexpr float kRange = 2048.f;
 
 // Shared memory: [rings][scales][merge][info].
 template <class C>
@@ -570,7 +575,12 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       float m[NQ][2], l[NQ][2];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) m[q][0] = m[q][1] = kNoMax, l[q][0] = l[q][1] = 0.f;
-      float vtop = 0.f, vmul = 0.f;  // e4m3: bound of the value scales met so far, and 2^kWeightShift over it
+      // e4m3, of each row: vtop, 2^kWeightShift over it, the largest weighted scale that is known; the lane's smallest vtop
+      float vtop[NQ][2], vmul[NQ][2], heavy[NQ][2], vlow = 0.f;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) vtop[q][e] = heavy[q][e] = 0.f, vmul[q][e] = 1.f;
       const int pos_min = s.len - s.count, pos_max = s.len - 1;
 
       const int first = t + (team - (t - c0) % TEAMS + TEAMS) % TEAMS;
@@ -669,18 +679,32 @@ __global__ void __launch_bounds__(C::W * 32, 1)
           for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int e = 0; e < 2; ++e) grew |= fmaxf(sc[q][e], sc[q][2 + e]) - m[q][e] > kSlack;
-          if (E4M3) grew |= fmaxf(vs[0], vs[1]) > vtop && fmaxf(vs[0], vs[1]) < INFINITY;
+          if (E4M3) grew |= fmaxf(fabsf(vs[0]), fabsf(vs[1])) > vlow;
           if (__any_sync(0xffffffffu, grew)) {
-            float more_room = 1.f;
+            float top = 0.f;  // e4m3: the largest scale, infinities aside
             if (E4M3) {
-              const float y = column_max(fmaxf(vs[0] < INFINITY ? vs[0] : 0.f, vs[1] < INFINITY ? vs[1] : 0.f));
-              if (y > vtop) {  // two bits of room, so that the next ones rarely come here
-                const float now = fmaxf(y * 4.f, 0x1p-110f);
-                more_room = vtop / now;
-                vtop = now;
-                vmul = (float)(1 << kWeightShift) / now;
+              // rows of zeros have a scale too (append gives them 1): they count for nothing
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint32_t any = 0;
+#pragma unroll 1
+                for (int k = c4; k < C::RB / 16; k += 4) {
+                  uint32_t w[4];
+                  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                               : "r"(kb + C::KB + g * C::GB + chunk_at<C>(g4 + i * 8, k)));
+                  any |= (w[0] | w[1] | w[2] | w[3]) & 0x7f7f7f7fu;
+                }
+                any |= __shfl_xor_sync(0xffffffffu, any, 1);
+                any |= __shfl_xor_sync(0xffffffffu, any, 2);
+                if (fabsf(vs[i]) < INFINITY) {
+                  if (any == 0) vs[i] = 0.f;
+                  top = fmaxf(top, fabsf(vs[i]));
+                }
               }
+              top = column_max(top);
             }
+            vlow = INFINITY;
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
               float fac[2];
@@ -690,7 +714,22 @@ __global__ void __launch_bounds__(C::W * 32, 1)
                 m[q][e] = fmaxf(was, column_max(fmaxf(sc[q][e], sc[q][2 + e])));
                 fac[e] = ex2(was - m[q][e]);
                 l[q][e] *= fac[e];
-                fac[e] *= more_room;
+                if (E4M3) {
+                  float y = 0.f;
+#pragma unroll
+                  for (int i = 0; i < 2; ++i)
+                    if (fabsf(vs[i]) < INFINITY) y = fmaxf(y, ex2(sc[q][2 * i + e] - m[q][e]) * fabsf(vs[i]));
+                  heavy[q][e] = fmaxf(heavy[q][e] * fac[e], column_max(y));
+                  const float v = vtop[q][e];
+                  float now = top > v ? top * 4.f : v;  // two bits of room, so that the next ones rarely come here
+                  if (heavy[q][e] > 0.f) now = fminf(now, heavy[q][e] * kRange);
+                  now = fminf(fmaxf(now, 0x1p-110f), 0x1p126f);
+                  now = fmaxf(now, fac[e] * v * 0x1p-40f);  // what the row has summed up stays in fp32's range
+                  fac[e] = fac[e] * v / now;
+                  vtop[q][e] = now;
+                  vmul[q][e] = (float)(1 << kWeightShift) / now;
+                  vlow = fminf(vlow, now);
+                }
               }
 #pragma unroll
               for (int k = 0; k < KS; ++k)
@@ -705,7 +744,8 @@ __global__ void __launch_bounds__(C::W * 32, 1)
             for (int e = 0; e < 4; ++e) {
               const float w = ex2(sc[q][e] - m[q][e & 1]);
               l[q][e & 1] += w;
-              pw[q][e] = E4M3 ? w * (vs[e >> 1] * vmul) : w;
+              // the scale first: over a vtop that is far below, it could pass fp32's range where the product does not
+              pw[q][e] = E4M3 ? w * vs[e >> 1] * vmul[q][e & 1] : w;
             }
           const uint32_t vg = kb + C::KB + g * C::GB, va = vg + v_lane;
           bool odd = false;
@@ -836,12 +876,12 @@ __global__ void __launch_bounds__(C::W * 32, 1)
       }
 
       // the warps' parts of the item
-      const float f = E4M3 ? vtop * (1.f / (1 << kWeightShift)) : 1.f;
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = tile0 + q * 8 + 2 * c4 + e;  // row of the item
+          const float f = E4M3 ? vtop[q][e] * (1.f / (1 << kWeightShift)) : 1.f;
           l[q][e] = column_sum(l[q][e]);
           if (g4 == 0) s_ms[team * R + r] = make_float2(m[q][e], l[q][e]);
           if (r >= nrow) continue;
