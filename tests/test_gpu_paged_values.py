@@ -93,3 +93,27 @@ def test_scales_of_either_sign():
                 _set_values(case, b, j, factor=-1.0)
     _check(case, case.queries(4, 1))
     _check(case, case.queries(4, 3))
+
+
+@pytest.mark.parametrize("T,Hq", [(1, 2), (3, 8), (1, 16)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_visible_infinities_follow_the_formula(T, Hq, D):
+    """A value of +-infinity that a row sees, wherever it lies, makes that output column +-infinity: every weight is
+    positive. Both signs make it NaN, as a NaN does; the other columns keep their values."""
+    lens = [50, 300]
+    case = Case(lens, 1, D, 16)
+    q = case.queries(Hq, T)
+    bad = {5: [(3, math.inf)], 6: [(20, -math.inf)], 7: [(3, math.inf), (21, -math.inf)], 8: [(30, math.nan)],
+           9: [(n - 1 - T, math.inf) for n in (50,)], 40: [(40, -math.inf), (41, -math.inf)]}
+    for b in range(len(lens)):
+        for col, rows in bad.items():
+            for j, x in rows:
+                case.v[case.table[b, j // 16], :, j % 16, col] = x
+    got = case.cache().attend(q).cpu().double()
+    ref, tol, _, _ = case.exact(q)  # of the finite values that were there
+    fine = [c for c in range(D) if c not in bad]
+    assert bool(((got - ref).abs() <= tol)[..., fine].all())
+    for col, rows in bad.items():
+        want = sum(x for _, x in rows)
+        x = got[..., col]
+        assert bool(x.isnan().all() if math.isnan(want) else (x == want).all()), (col, x)

@@ -814,16 +814,20 @@ __global__ void __launch_bounds__(C::W * 32, 1)
             }
           }
           // P^T as the products' B operand. e4m3: fp16, 11 bits, on values that are exact in fp16. bf16: in two parts
-          // (16 bits of them): one part would add its 2^-9 to the output's own rounding
+          // (16 bits of them): one part would add its 2^-9 to the output's own rounding. The first is cut
+          // off, not rounded, and the second more than 0, so that an infinite value makes both products infinite, of
+          // one sign; a weight of 0 has two zeros
           uint32_t hi[NQ][2], lw[NQ][2];
 #pragma unroll
           for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float y = pw[q][2 * i], z = pw[q][2 * i + 1];
-              const uint32_t w = E4M3 ? pack_f16(y, z) : pack_bf16(y, z);
+              const uint32_t w = E4M3 ? pack_f16(y, z) : __byte_perm(__float_as_uint(y), __float_as_uint(z), 0x7632);
               hi[q][i] = transpose8(w);
-              if (!E4M3) lw[q][i] = transpose8(pack_bf16(y - bf16lo(w), z - bf16hi(w)));
+              if (!E4M3)
+                lw[q][i] = transpose8(pack_bf16(fmaxf(y - bf16hi(__float_as_uint(y)), fminf(y, 0x1p-126f)),
+                                                fmaxf(z - bf16hi(__float_as_uint(z)), fminf(z, 0x1p-126f))));
             }
           constexpr int VI = E4M3 ? KS / 2 : KS, VB4 = VI < 4 ? VI : 4;
 #pragma unroll
