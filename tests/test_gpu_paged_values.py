@@ -117,3 +117,24 @@ def test_visible_infinities_follow_the_formula(T, Hq, D):
         want = sum(x for _, x in rows)
         x = got[..., col]
         assert bool(x.isnan().all() if math.isnan(want) else (x == want).all()), (col, x)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_nan_weights_stay_among_the_positions_a_row_sees(bits):
+    """Totals: a row whose softmax is NaN makes the totals of what it sees NaN, and no other's."""
+    case = Case([50, 70], 2, 64, 16, bits)
+
+    def totals(q, window):
+        w = torch.zeros(2, 2, case.cap, device=DEV)
+        case.cache(weights=w).attend(q, window=window)
+        return w.cpu()
+    q = case.queries(4, 1)
+    q[:, :, 0, 0] = float("nan")
+    w = totals(q, 21)  # the window begins inside a block
+    for b, n in enumerate(case.lens):
+        assert w[b, :, n - 21:n].isnan().all() and not w[b, :, :n - 21].any() and not w[b, :, n:].any()
+    q = case.queries(4, 2)
+    q[:, :, 0, 0] = float("nan")  # the first of two new tokens, which does not see the second
+    w = totals(q, 0)
+    for b, n in enumerate(case.lens):
+        assert w[b, :, :n - 1].isnan().all() and torch.isfinite(w[b, :, n - 1:]).all() and (w[b, :, n - 1] > 0).all()

@@ -1016,6 +1016,12 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const AttendPar
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         if (z[k] == -INFINITY) continue;  // past the rows, or a row that sees nothing
+        if (z[k] != z[k]) {  // a row of NaN weights: only what it sees
+          const int at = len - n + token_of(p, r0 + k), from = p.window ? at - p.window + 1 : 0;
+          if (j >= from && j <= at) a[0] = z[k];
+          if (j + 1 >= from && j + 1 <= at) a[1] = z[k];
+          continue;
+        }
         a[0] += ex2(v[k].x - z[k]);
         a[1] += ex2(v[k].y - z[k]);
       }
