@@ -407,13 +407,13 @@ int tbf16_attn_bwd_sharded(const void* q16, const void* k16, const void* v16, co
  * row of D values per key/value head, bf16 or e4m3. An e4m3 row is its bf16 row times a power of two that
  * takes the row's largest magnitude to [128, 256), and its inverse scale stands in k_scale / v_scale
  * (a zero row has 1, a row that holds an infinity or NaN has NaN). Sequence b's token j sits in slot
- * j % page_size of page table[b * table_ld + j / page_size]; lens[b] tokens are cached. table, lens and
- * counts are read on the device, so a captured graph follows their contents.
+ * j % page_size of page table[b * table_ld + j / page_size]; lens[b] tokens are cached. table, lens,
+ * counts and fresh are read on the device, so a captured graph follows their contents.
  *
  * Limits: D 64, 128 or 256 (zero-pad others); page_size a power of two from 16 to 1024; batch up to 1024;
  * pointers and strides multiples of 16 bytes (scales: 16-byte pointers, strides multiples of 4 floats,
  * the page_size scales of a (page, head) contiguous). Page numbers outside [0, pages), lengths outside
- * [0, max_pages * page_size] and counts outside [0, min(T, lens)] set bit 8 of the device status word. */
+ * [0, max_pages * page_size], counts outside [0, min(T, lens)] and negative fresh set bit 8 of the device status word. */
 typedef struct tbf16_paged_cache {
   void* k;              /* [pages, heads, page_size, D], last dimension contiguous */
   void* v;
@@ -426,12 +426,13 @@ typedef struct tbf16_paged_cache {
   int64_t table_ld;
   int64_t batch, heads, D, page_size, pages, max_pages;
   int64_t dtype; /* TBF16_BF16 or TBF16_E4M3 */
+  const int32_t* fresh; /* [batch] or NULL: tokens that the last step added to each sequence */
 } tbf16_paged_cache;
 
 /* Writes the newest rows of every sequence into its pages: k, v bf16 (batch, heads, T, d) with element
  * strides of batch, head, token and contiguous last dimension, d <= D a multiple of 8 (the cache row's
  * remaining columns are zeroed). lens counts the new tokens already: token t < counts[b] goes to position
- * lens[b] - counts[b] + t (counts NULL: min(T, lens[b]) each). pos (nullable): int32 (batch, heads, capacity) with
+ * lens[b] - counts[b] + t (counts NULL: min(T, lens[b], fresh[b]) each, without fresh the first two). pos (nullable): int32 (batch, heads, capacity) with
  * strides pos_sb, pos_sh; position j of every head receives seen[b] - counts[b] + t, the token's number
  * in the whole sequence, where seen[b] counts all tokens ever appended. */
 int tbf16_paged_append(const tbf16_paged_cache* cache, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st,
@@ -442,7 +443,7 @@ int tbf16_paged_append(const tbf16_paged_cache* cache, const void* k, int64_t k_
 /* Attention of the newest T tokens of every sequence over its cache. q bf16 (batch, Hq, T, D), out bf16
  * of the same shape, element strides of batch, head, token, contiguous last dimension, 16-byte rows;
  * Hq a multiple of heads (query head h reads key/value head h / (Hq / heads)). Token t < counts[b]
- * (NULL: min(T, lens[b])) sits at position i = lens[b] - counts[b] + t and sees the cached positions j
+ * (NULL: as for append) sits at position i = lens[b] - counts[b] + t and sees the cached positions j
  * with i - window < j <= i (window 0: all j <= i). Rows that see nothing, and tokens t >= counts[b], give zeros.
  * weights (nullable): fp32 (batch, heads, capacity) with strides w_sb, w_sh; the softmax weight of every
  * visible position, summed over the head's query heads and the new tokens, is added to it.

@@ -1,0 +1,85 @@
+"""tbf16.PagedCache as a serving loop uses it: what the calls after `advance` take for granted, refused drafts,
+steps that were captured, more than one GPU."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _rows(B, H, T, D, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [torch.randn(B, h, T, D, device=DEV, generator=g).bfloat16() for h in (H, H, 2 * H)]
+
+
+def _counts(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _same(a, b):
+    for name in ("k", "v", "pos", "weights", "lens", "seen"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+
+
+@pytest.mark.parametrize("T", [3, 5])
+def test_calls_take_the_counts_of_the_last_advance(T):
+    """A sequence whose count is below T gets its first rows, into the places that advance made, and keeps the tokens
+    it had; one without new tokens is left alone. With counts given, the calls do the same as before."""
+    import tbf16
+    from tbf16 import _ext
+    a, b = (tbf16.PagedCache(3, 2, 64, 100, page_size=16, track=True) for _ in range(2))
+    k, v, q = _rows(3, 2, 20, 64)
+    for c in (a, b):
+        c.advance([20, 15, 7])
+        c.append(k, v, counts=_counts([20, 15, 7]))
+        c.attend(q[:, :, :1], counts=_counts([1, 1, 1]))
+    for step, new in enumerate(([3, 1, 0], [0, 2, 3], [1, 1, 1])):
+        k, v, q = _rows(3, 2, T, 64, seed=step + 1)
+        for c in (a, b):
+            c.advance(new)
+        a.append(k, v)
+        b.append(k, v, counts=_counts(new))
+        assert torch.equal(a.attend(q), b.attend(q, counts=_counts(new)))
+        _same(a, b)
+    assert _ext.device_status() == 0
+
+
+def test_fewer_query_rows_than_new_tokens():
+    """After a prompt, attention of its last tokens alone: the newest T of each."""
+    import tbf16
+    from tbf16 import _ext
+    c = tbf16.PagedCache(2, 2, 64, 100, page_size=16)
+    k, v, q = _rows(2, 2, 30, 64)
+    c.advance([30, 9])
+    c.append(k, v)
+    every = c.attend(q, counts=_counts([30, 9]))
+    for T in (1, 2):
+        last = torch.stack([q[b, :, n - T:n] for b, n in enumerate((30, 9))])
+        got = c.attend(last)
+        for b, n in enumerate((30, 9)):
+            assert torch.equal(got[b], every[b, :, n - T:n])
+    c.release(0)
+    assert not c.attend(q[:, :, :1])[0].any()
+    assert _ext.device_status() == 0
+
+
+def test_a_captured_step_follows_the_counts_of_advance():
+    import tbf16
+    a, b = (tbf16.PagedCache(2, 2, 64, 100, page_size=16, track=True) for _ in range(2))
+    k, v, q = _rows(2, 2, 4, 64)
+    for c in (a, b):
+        c.advance(4)
+        c.append(k, v)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.append(k, v)
+        out = a.attend(q)
+    for i, new in enumerate(([4, 1], [0, 3], [2, 2], [1, 0])):
+        for x, y in zip((k, v, q), _rows(2, 2, 4, 64, seed=i + 5)):
+            x.copy_(y)
+        a.advance(new)
+        graph.replay()
+        b.advance(new)
+        b.append(k, v, counts=_counts(new))
+        assert torch.equal(out, b.attend(q, counts=_counts(new)))
+        _same(a, b)

@@ -40,6 +40,7 @@ int paged_view(const tbf16_paged_cache* c, tbf16::PagedView* v) {
   v->v_scale = c->v_scale;
   v->table = c->table;
   v->lens = c->lens;
+  v->fresh = c->fresh;
   v->k_sp = c->k_sp * item; v->k_sh = c->k_sh * item; v->k_ss = c->k_ss * item;
   v->v_sp = c->v_sp * item; v->v_sh = c->v_sh * item; v->v_ss = c->v_ss * item;
   v->ks_sp = c->ks_sp; v->ks_sh = c->ks_sh; v->vs_sp = c->vs_sp; v->vs_sh = c->vs_sh;

@@ -12,6 +12,7 @@ struct PagedView {
   float* v_scale;
   const int* table;
   const int* lens;
+  const int* fresh;
   int64_t k_sp, k_sh, k_ss, v_sp, v_sh, v_ss, ks_sp, ks_sh, vs_sp, vs_sh, table_ld;
   int64_t pages;
   int batch, heads, page_shift, max_pages, cap;  // cap = max_pages << page_shift, below 2^31
@@ -24,9 +25,9 @@ __device__ __forceinline__ int paged_len(const PagedView& c, int b) {
   if (n < 0 || n > c.cap) atomicOr(c.err, kErrPage);
   return min(max(n, 0), c.cap);
 }
-// New tokens of sequence b, held inside [0, min(T, len)] (counts null: that many).
+// New tokens of sequence b, held inside [0, min(T, len)] (counts null: that many, or the cache's own count if less).
 __device__ __forceinline__ int paged_count(const PagedView& c, const int* counts, int b, int T, int len) {
-  const int n = counts ? counts[b] : min(T, len);
+  const int n = counts ? counts[b] : c.fresh ? min(c.fresh[b], min(T, len)) : min(T, len);
   if (n < 0 || n > T || n > len) atomicOr(c.err, kErrPage);
   return min(max(n, 0), min(T, len));
 }

@@ -188,7 +188,7 @@ __global__ void bounded_wait_selftest_kernel(unsigned int* err, uint64_t timeout
 
 extern "C" {
 
-int tbf16_abi_version(void) { return 100; }
+int tbf16_abi_version(void) { return 101; }
 
 const char* tbf16_status_string(int status) {
   switch (status) {

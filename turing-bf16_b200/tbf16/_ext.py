@@ -101,7 +101,8 @@ class PagedCacheStruct(ctypes.Structure):
     """tbf16_paged_cache of include/tbf16_sm100.h."""
     _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale", "table", "lens")]
                 + [(n, _i64) for n in ("k_sp", "k_sh", "k_ss", "v_sp", "v_sh", "v_ss", "ks_sp", "ks_sh", "vs_sp", "vs_sh",
-                                       "table_ld", "batch", "heads", "D", "page_size", "pages", "max_pages", "dtype")])
+                                       "table_ld", "batch", "heads", "D", "page_size", "pages", "max_pages", "dtype")]
+                + [("fresh", _vp)])
 
 
 def _build_module():

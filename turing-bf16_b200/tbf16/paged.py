@@ -2,7 +2,7 @@
 
     cache = tbf16.PagedCache(batch, kv_heads, head_dim, max_len, layers=L)     # bf16; dtype=torch.float8_e4m3fn
     cache.advance(T)                        # room for T new tokens of every sequence (or a count for each)
-    cache.append(k, v, layer)               # k, v (B, kv_heads, T, head_dim): into the pages
+    cache.append(k, v, layer)               # k, v (B, kv_heads, T, head_dim): into the pages, by those counts
     out = cache.attend(q, layer)            # q (B, heads, T, head_dim): attention over everything cached
     cache.evict(keep, recent)               # with track=True: cut every head to its heaviest positions
 
@@ -54,7 +54,7 @@ def _rows(x, name, B, H, d, device):
 class _Layer:
     """One layer's buffers and their description for the library."""
 
-    def __init__(self, k, v, k_scale, v_scale, table, lens, weights, pos, seen):
+    def __init__(self, k, v, k_scale, v_scale, table, lens, weights, pos, seen, fresh):
         self.k, self.v, self.k_scale, self.v_scale, self.weights, self.pos = k, v, k_scale, v_scale, weights, pos
         pages, heads, page_size, D = k.shape
         c = self.struct = PagedCacheStruct()
@@ -67,6 +67,7 @@ class _Layer:
             c.vs_sp, c.vs_sh = v_scale.stride()[:2]
         c.table_ld, c.batch, c.max_pages = table.stride(0), table.shape[0], table.shape[1]
         c.heads, c.D, c.page_size, c.pages, c.dtype = heads, D, page_size, pages, _DTYPES[k.dtype]
+        c.fresh = None if fresh is None else fresh.data_ptr()
         self.ref, self.D = ctypes.addressof(c), D
         self.weight_args = (None, 0, 0) if weights is None else (weights.data_ptr(), *weights.stride()[:2])
         self.pos_args = (None, 0, 0, None) if pos is None else (pos.data_ptr(), *pos.stride()[:2], seen.data_ptr())
@@ -77,7 +78,7 @@ class PagePool:
 
     def __init__(self, batch, pages, page_size, max_len):
         self.page_size, self.max_len = page_size, max_len
-        self.lengths, self.seen = [0] * batch, [0] * batch
+        self.lengths, self.seen, self.fresh = [0] * batch, [0] * batch, [0] * batch  # fresh: of the last advance
         self.owned = [[] for _ in range(batch)]
         self.free = list(range(pages - 1, -1, -1))
 
@@ -96,7 +97,7 @@ class PagePool:
             raise RuntimeError(f"tbf16.PagedCache.advance: out of pages ({sum(want)} wanted, {len(self.free)} free)")
         for own, w in zip(self.owned, want):
             own.extend(self.free.pop() for _ in range(w))
-        self.lengths = new
+        self.lengths, self.fresh = new, counts
         self.seen = [s + c for s, c in zip(self.seen, counts)]
         return any(want)
 
@@ -107,6 +108,7 @@ class PagePool:
         self.free.extend(reversed(own[used:]))
         del own[used:]
         self.lengths[sequence] = n
+        self.fresh[sequence] = min(self.fresh[sequence], n)
 
     def rows(self, width):
         """The page table: one row of `width` page numbers for each sequence, 0 past its pages."""
@@ -142,8 +144,9 @@ class PagedCache:
         shape = (layers, batch, kv_heads, per * page_size)
         weights = torch.zeros(shape, device=dev) if track else None
         pos = torch.full(shape, -1, **ints) if track else None
-        self._state = torch.zeros((2, batch), **ints)  # lens, seen
-        self._init(k, v, ks, vs, torch.zeros((batch, per), **ints), *self._state.unbind(0), weights, pos, head_dim)
+        self._state = torch.zeros((3, batch), **ints)  # lens, seen, fresh
+        lens, seen, fresh = self._state.unbind(0)
+        self._init(k, v, ks, vs, torch.zeros((batch, per), **ints), lens, seen, weights, pos, head_dim, fresh)
         self.pool = PagePool(batch, pages, page_size, max_len)
 
     @classmethod
@@ -158,7 +161,7 @@ class PagedCache:
         self.pool = None
         return self
 
-    def _init(self, k, v, k_scale, v_scale, table, lens, seen, weights, pos, head_dim):
+    def _init(self, k, v, k_scale, v_scale, table, lens, seen, weights, pos, head_dim, fresh=None):
         require_cuda(k, v, table, lens, k_scale, v_scale, seen, weights, pos)
         if k.dtype not in _DTYPES or v.dtype != k.dtype:
             raise RuntimeError(f"tbf16.PagedCache: bf16 or e4m3 pools expected, got {k.dtype} and {v.dtype}")
@@ -197,8 +200,8 @@ class PagedCache:
         self.head_dim, self.dtype, self.table, self.lens, self.seen = head_dim, k.dtype, table, lens, seen
         self.k, self.v, self.k_scale, self.v_scale, self.weights, self.pos = k, v, k_scale, v_scale, weights, pos
         pick = lambda x, i: None if x is None else x[i]  # noqa: E731
-        self._layers = [_Layer(k[i], v[i], pick(k_scale, i), pick(v_scale, i), table, lens, pick(weights, i), pick(pos, i), seen)
-                        for i in range(L)]
+        self._layers = [_Layer(k[i], v[i], pick(k_scale, i), pick(v_scale, i), table, lens, pick(weights, i), pick(pos, i),
+                               seen, fresh) for i in range(L)]
         self._sizes, self._buffers, self._lib = {}, {}, lib()
 
     # ------------------------------------------------------------------------------------------- host side
@@ -215,7 +218,8 @@ class PagedCache:
 
     def advance(self, counts):
         """Makes room for counts new tokens (an int for every sequence, or one int each): takes pages from the
-        pool and raises lens and seen. Call it once a step, before `append` and `attend` of every layer."""
+        pool and raises lens and seen. Call it once a step, before `append` and `attend` of every layer, which take
+        these counts unless they are given others."""
         self._upload(table=self._owned("advance").advance(counts))
 
     def release(self, sequence):
@@ -229,10 +233,10 @@ class PagedCache:
         self._upload(table=False)
 
     def _upload(self, table):
-        """lens, seen and, where it changed, the table to the GPU, in stream order and without waiting for it: from
+        """lens, seen, the new counts and, where it changed, the table to the GPU, in stream order and without waiting for it: from
         pinned memory that torch's allocator does not hand out again before the copy is done."""
         pinned = dict(dtype=torch.int32, pin_memory=True)
-        self._state.copy_(torch.tensor([self.pool.lengths, self.pool.seen], **pinned), non_blocking=True)
+        self._state.copy_(torch.tensor([self.pool.lengths, self.pool.seen, self.pool.fresh], **pinned), non_blocking=True)
         if table:
             self.table.copy_(torch.tensor(self.pool.rows(self.table.shape[1]), **pinned), non_blocking=True)
 
@@ -272,7 +276,8 @@ class PagedCache:
     def append(self, k, v, layer=0, counts=None):
         """Writes the newest rows of every sequence into the pages: k, v bf16 (B, kv_heads, T, head_dim), any
         strides. lens counts them already (`advance`). counts: int32 (B,) on the GPU, the tokens that are real
-        in each sequence (the first ones of its T; default: all, or lens where that is less)."""
+        in each sequence (the first ones of its T; default: those of the last `advance`, at most T; over a caller's
+        buffers T, or lens where that is less)."""
         c = self._layers[layer]
         k = _rows(k, "k", self.batch, self.kv_heads, self.head_dim, self.device)
         v = _rows(v, "v", self.batch, self.kv_heads, self.head_dim, self.device)
@@ -286,8 +291,8 @@ class PagedCache:
 
     def attend(self, q, layer=0, counts=None, scale=None, window=0):
         """Attention of the newest T tokens over the cache: q bf16 (B, heads, T, head_dim), heads a multiple of
-        kv_heads -> bf16 of the same shape, over (B, T, heads, head_dim) memory as tbf16.sdpa returns it. Token
-        t of a sequence sits at position lens - counts + t and sees the positions up to its own; window > 0: only
+        kv_heads -> bf16 of the same shape, over (B, T, heads, head_dim) memory as tbf16.sdpa returns it. counts as in
+        `append`. Token t of a sequence sits at position lens - counts + t and sees the positions up to its own; window > 0: only
         the last `window` of them. Rows past counts, and rows that see nothing, are zeros. A tracking cache adds
         the attention weights to `weights`."""
         c, d = self._layers[layer], self.head_dim
