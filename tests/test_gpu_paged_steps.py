@@ -83,3 +83,19 @@ def test_a_captured_step_follows_the_counts_of_advance():
         b.append(k, v, counts=_counts(new))
         assert torch.equal(out, b.attend(q, counts=_counts(new)))
         _same(a, b)
+
+
+def _attend_and_cut(dev):
+    import tbf16
+    c = tbf16.PagedCache(1, 80, 64, 18000, track=True, device=dev)
+    g = torch.Generator().manual_seed(1)
+    k, v, q = (torch.randn(1, h, 17000, 64, generator=g).bfloat16().to(dev) for h in (80, 80, 80))
+    c.advance(17000)
+    c.append(k, v)
+    return c.attend(q[:, :, -1:]).cpu(), *(x.cpu() for x in c.compact(16000))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="two GPUs")
+def test_every_gpu_of_a_process():
+    """Kernels that need more shared memory than a launch may have by default ask for it on each GPU."""
+    assert all(torch.equal(x, y) for x, y in zip(_attend_and_cut("cuda:0"), _attend_and_cut("cuda:1")))

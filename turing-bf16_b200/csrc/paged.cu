@@ -632,7 +632,8 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   // CTAs for an item: more while its slices are long and there are SMs for them. Whole calls with 1 / 2 / 4 / 8 CTAs:
   // 8 items of 36156 positions 46 / 36 / 32 / 26 us, of 9000 17.8 / 17.3 / 16.8 / 18.6, of 4200 13.9 / 14.1 / 14.3 / 14.4.
   // More CTAs than SMs do not pay: 64 items of 16000 57 / 54 / 63 / 87, 128 of 2112 9 / 22 / 41 / 73.
-  const int sms = tbf16_host::device_info()->sms;
+  const tbf16_host::DeviceInfo* dev = tbf16_host::device_info();
+  const int sms = dev->sms;
   int ctas = 1;
   while (ctas < 8 && (cols + ctas - 1) / ctas > 4096 && items * ctas * 2 <= sms) ctas *= 2;
   constexpr int kMaxKeys = 48 * 1024;
@@ -640,9 +641,15 @@ extern "C" int tbf16_paged_compact(const tbf16_paged_cache* cache, const float* 
   const int64_t slice = (cols + ctas - 1) / ctas;
   p.in_smem = slice <= kMaxKeys;
   p.inline_moves = ctas == 1 && p.max_moves <= kMoveRows;
-  static const cudaError_t attr = cudaFuncSetAttribute(
-      select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
-  if (attr != cudaSuccess || items * ctas > INT32_MAX) return TBF16_ERR_LAUNCH;
+  if (items * ctas > INT32_MAX) return TBF16_ERR_LAUNCH;
+  static bool attr_done[64] = {false};
+  if (!attr_done[dev->device & 63]) {
+    if (cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4) != cudaSuccess) {
+      cudaGetLastError();
+      return TBF16_ERR_LAUNCH;
+    }
+    attr_done[dev->device & 63] = true;
+  }
   auto st = static_cast<cudaStream_t>(stream);
   if (int rc = tbf16_host::launch_pdl(select_kernel, dim3((unsigned)(items * ctas)), kSelThreads,
                                       p.in_smem ? (size_t)slice * 4 : 0, (unsigned)ctas, st, p))

@@ -1048,7 +1048,7 @@ int attend_smem(const AttendParams& p) {
 constexpr int kSmemStatic = 4 * 1024;
 
 template <class C>
-int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
+int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, const tbf16_host::DeviceInfo* dev, cudaStream_t st) {
   CUtensorMap km, vm;
   const int box = (int)std::min<int64_t>(C::BK, cache->page_size);
   p.box_shift = 0;
@@ -1059,10 +1059,16 @@ int launch_attend(const tbf16_paged_cache* cache, AttendParams& p, int sms, cuda
   p.stages = C::MAX_STAGES;
   const int smem = attend_smem<C>(p);  // a batch of 1024 with 256-wide bf16 rows takes 216 KB
   if (smem + kSmemStatic > kSmemMax) return TBF16_ERR_UNSUPPORTED;
-  static const cudaError_t attr =
-      cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic);
-  if (attr != cudaSuccess) return TBF16_ERR_LAUNCH;
-  return tbf16_host::launch_pdl(attend_kernel<C>, sms, C::W * 32, smem, 1, st, km, vm, p);
+  static bool attr_done[64] = {false};
+  if (!attr_done[dev->device & 63]) {
+    if (cudaFuncSetAttribute(attend_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kSmemStatic) !=
+        cudaSuccess) {
+      cudaGetLastError();
+      return TBF16_ERR_LAUNCH;
+    }
+    attr_done[dev->device & 63] = true;
+  }
+  return tbf16_host::launch_pdl(attend_kernel<C>, dev->sms, C::W * 32, smem, 1, st, km, vm, p);
 }
 
 // Query rows of an item. Heads with more than 32 make several items of the same keys,
@@ -1084,15 +1090,15 @@ struct Workspace {
 };
 
 template <int D, bool E4M3>
-int launch_rows(const tbf16_paged_cache* cache, AttendParams& p, int sms, cudaStream_t st) {
+int launch_rows(const tbf16_paged_cache* cache, AttendParams& p, const tbf16_host::DeviceInfo* dev, cudaStream_t st) {
   // Up to 16 rows in one warp: a cached fragment is read from shared memory and converted once for both tiles. 256-wide
   // outputs of two tiles would not fit a warp's registers; there, and for 32 rows, two or four warps share a block
   // (16 query heads on one of 128, 8 sequences of 32768 tokens: two tiles 39 us, two warps 51; on one of 256: 80 and 68).
   constexpr bool WIDE = D == 256;
   const int R = item_rows(p.rows);
-  if (R == 8) return launch_attend<Tile<D, E4M3, 1, 1>>(cache, p, sms, st);
-  if (R == 16) return launch_attend<Tile<D, E4M3, WIDE ? 1 : 2, WIDE ? 2 : 1>>(cache, p, sms, st);
-  return launch_attend<Tile<D, E4M3, WIDE ? 1 : 2, WIDE ? 4 : 2>>(cache, p, sms, st);
+  if (R == 8) return launch_attend<Tile<D, E4M3, 1, 1>>(cache, p, dev, st);
+  if (R == 16) return launch_attend<Tile<D, E4M3, WIDE ? 1 : 2, WIDE ? 2 : 1>>(cache, p, dev, st);
+  return launch_attend<Tile<D, E4M3, WIDE ? 1 : 2, WIDE ? 4 : 2>>(cache, p, dev, st);
 }
 
 bool attend_sizes_ok(const tbf16_paged_cache* c, int64_t Hq, int64_t T) {
@@ -1153,9 +1159,9 @@ extern "C" int tbf16_paged_attend(const tbf16_paged_cache* cache, const void* q,
   const bool e4m3 = cache->dtype == TBF16_E4M3;
   auto st = static_cast<cudaStream_t>(stream);
   int rc;
-  if (cache->D == 64) rc = e4m3 ? launch_rows<64, true>(cache, p, dev->sms, st) : launch_rows<64, false>(cache, p, dev->sms, st);
-  else if (cache->D == 128) rc = e4m3 ? launch_rows<128, true>(cache, p, dev->sms, st) : launch_rows<128, false>(cache, p, dev->sms, st);
-  else rc = e4m3 ? launch_rows<256, true>(cache, p, dev->sms, st) : launch_rows<256, false>(cache, p, dev->sms, st);
+  if (cache->D == 64) rc = e4m3 ? launch_rows<64, true>(cache, p, dev, st) : launch_rows<64, false>(cache, p, dev, st);
+  else if (cache->D == 128) rc = e4m3 ? launch_rows<128, true>(cache, p, dev, st) : launch_rows<128, false>(cache, p, dev, st);
+  else rc = e4m3 ? launch_rows<256, true>(cache, p, dev, st) : launch_rows<256, false>(cache, p, dev, st);
   if (rc != TBF16_OK || !weights) return rc;
   const int block_keys = cache->D * (e4m3 ? 1 : 2) <= 64 ? 64 : cache->D * (e4m3 ? 1 : 2) <= 128 ? 32 : 16;
   const int span = kWeightThreads * 2;
