@@ -99,3 +99,41 @@ def _attend_and_cut(dev):
 def test_every_gpu_of_a_process():
     """Kernels that need more shared memory than a launch may have by default ask for it on each GPU."""
     assert all(torch.equal(x, y) for x, y in zip(_attend_and_cut("cuda:0"), _attend_and_cut("cuda:1")))
+
+
+def test_calls_run_with_the_caches_device_current(monkeypatch):
+    """Whatever device is current, all that a call asks and does happens on the cache's. (Played here: another device
+    is current until the call has made the cache's current.)"""
+    import tbf16
+    c = tbf16.PagedCache(2, 2, 64, 100, track=True)
+    k, v, q = _rows(2, 2, 5, 64)
+    c.advance(5)
+    depth, seen = [0], []
+
+    class Current:
+        def __init__(self, device):
+            assert torch.device(device) == c.device
+
+        def __enter__(self):
+            depth[0] += 1
+
+        def __exit__(self, *exc):
+            depth[0] -= 1
+
+    def noting(fn):
+        def call(*args):
+            seen.append(depth[0] > 0)
+            return fn(*args)
+        return call
+
+    class Library:
+        def __getattr__(self, name):
+            return noting(getattr(tbf16.paged.lib(), name))
+    c._lib = Library()
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: c.device.index if depth[0] else c.device.index + 1)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", noting(torch._C._cuda_isCurrentStreamCapturing))
+    c.append(k, v)
+    c.attend(q)
+    c.compact(3)
+    assert len(seen) >= 6 and all(seen)

@@ -18,6 +18,7 @@ decoding step can be captured in a CUDA graph and replayed after `advance`. No h
 The reference has no counterpart: it leaves calls with few query rows to torch (tbf16/convert.py there).
 """
 import ctypes
+import functools
 
 import torch
 
@@ -49,6 +50,18 @@ def _rows(x, name, B, H, d, device):
         # clone: also rewrites odd strides of dimensions of one element, which count as contiguous
         x = torch.nn.functional.pad(x, (0, -d % 8)) if d % 8 else x.clone(memory_format=torch.contiguous_format)
     return x
+
+
+def _on_its_device(fn):
+    """A method of PagedCache that runs with the cache's device as the current one: the library's size queries, the
+    question whether a capture is on, allocations and launches all go by that."""
+    @functools.wraps(fn)
+    def call(self, *args, **kw):
+        if torch._C._cuda_getDevice() == self.device.index:
+            return fn(self, *args, **kw)
+        with torch.cuda.device(self.device):
+            return fn(self, *args, **kw)
+    return call
 
 
 class _Layer:
@@ -249,12 +262,7 @@ class PagedCache:
         return counts.data_ptr()
 
     def _run(self, fn, what, *args):
-        """One library call on the cache's device."""
-        if torch._C._cuda_getDevice() == self.device.index:
-            status = fn(*args)
-        else:
-            with torch.cuda.device(self.device):
-                status = fn(*args)
+        status = fn(*args)
         if status:
             check(status, what)
 
@@ -273,6 +281,7 @@ class PagedCache:
 
     # ------------------------------------------------------------------------------------------- operators
 
+    @_on_its_device
     def append(self, k, v, layer=0, counts=None):
         """Writes the newest rows of every sequence into the pages: k, v bf16 (B, kv_heads, T, head_dim), any
         strides. lens counts them already (`advance`). counts: int32 (B,) on the GPU, the tokens that are real
@@ -289,6 +298,7 @@ class PagedCache:
         self._run(self._lib.tbf16_paged_append, "append", c.ref, k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T, d,
                   self._counts(counts), *c.pos_args, torch._C._cuda_getCurrentRawStream(self.device.index))
 
+    @_on_its_device
     def attend(self, q, layer=0, counts=None, scale=None, window=0):
         """Attention of the newest T tokens over the cache: q bf16 (B, heads, T, head_dim), heads a multiple of
         kv_heads -> bf16 of the same shape, over (B, T, heads, head_dim) memory as tbf16.sdpa returns it. counts as in
@@ -322,6 +332,7 @@ class PagedCache:
                   ptr + buf.sync, size, stream)
         return out[..., :d] if d != D else out
 
+    @_on_its_device
     def compact(self, keep, recent=0, layer=0):
         """Cuts one layer's sequences to their `keep` heaviest positions per head, the newest `recent` tokens
         first of all, and moves the kept rows that lie beyond `keep` into the holes. Returns (weights, pos) in
