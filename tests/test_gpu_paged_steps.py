@@ -137,3 +137,16 @@ def test_calls_run_with_the_caches_device_current(monkeypatch):
     c.attend(q)
     c.compact(3)
     assert len(seen) >= 6 and all(seen)
+
+
+def test_rows_of_any_layout_with_a_padded_head_dim():
+    """A head dim that is no multiple of 8, with heads or tokens innermost in memory."""
+    import tbf16
+    for d in (20, 36, 80):
+        k, v, q = _rows(2, 4, 5, d)
+        a, b = (tbf16.PagedCache(2, 4, d, 50, page_size=16) for _ in range(2))
+        for c, lay in ((a, lambda x: x.contiguous()), (b, lambda x: x.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2))):
+            c.advance(5)
+            c.append(lay(k), lay(v))
+            c.out = c.attend(lay(q)), c.attend(lay(q)[:, :, :1].transpose(2, 3).contiguous().transpose(2, 3))
+        assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v) and all(torch.equal(x, y) for x, y in zip(a.out, b.out))

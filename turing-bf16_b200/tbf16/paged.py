@@ -36,8 +36,9 @@ def _kernel_dim(d):
     raise RuntimeError(f"tbf16.PagedCache: head dims up to {KERNEL_D[-1]}, got {d}")
 
 
-def _rows(x, name, B, H, d, device):
-    """A bf16 (B, H, T, d) tensor as the kernels read it: 16-byte rows, contiguous last dimension."""
+def _rows(x, name, B, H, d, device, width):
+    """A bf16 (B, H, T, d) tensor as the kernels read it: 16-byte rows, contiguous last dimension, widened with zeros
+    to `width` columns."""
     if x.dtype != torch.bfloat16 or x.device != device:
         require_cuda(x)
         raise RuntimeError(f"tbf16.PagedCache: {name} must be bf16 on {device}, got {x.dtype} on {x.device}")
@@ -46,9 +47,13 @@ def _rows(x, name, B, H, d, device):
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"tbf16.PagedCache: {name} requires grad; the cache is for inference (use torch.no_grad)")
     sb, sh, st, se = x.stride()
-    if se != 1 or (sb | sh | st) & 7 or d & 7 or x.data_ptr() & 15:
+    if d != width:
+        wide = x.new_zeros((*x.shape[:3], width))
+        wide[..., :d] = x
+        return wide
+    if se != 1 or (sb | sh | st) & 7 or x.data_ptr() & 15:
         # clone: also rewrites odd strides of dimensions of one element, which count as contiguous
-        x = torch.nn.functional.pad(x, (0, -d % 8)) if d % 8 else x.clone(memory_format=torch.contiguous_format)
+        x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
@@ -287,9 +292,9 @@ class PagedCache:
         strides. lens counts them already (`advance`). counts: int32 (B,) on the GPU, the tokens that are real
         in each sequence (the first ones of its T; default: those of the last `advance`, at most T; over a caller's
         buffers T, or lens where that is less)."""
-        c = self._layers[layer]
-        k = _rows(k, "k", self.batch, self.kv_heads, self.head_dim, self.device)
-        v = _rows(v, "v", self.batch, self.kv_heads, self.head_dim, self.device)
+        c, d = self._layers[layer], self.head_dim
+        k = _rows(k, "k", self.batch, self.kv_heads, d, self.device, d + -d % 8)
+        v = _rows(v, "v", self.batch, self.kv_heads, d, self.device, d + -d % 8)
         if k.shape != v.shape:
             raise RuntimeError(f"tbf16.PagedCache.append: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
         _, _, T, d = k.shape
@@ -306,13 +311,11 @@ class PagedCache:
         the last `window` of them. Rows past counts, and rows that see nothing, are zeros. A tracking cache adds
         the attention weights to `weights`."""
         c, d = self._layers[layer], self.head_dim
-        q = _rows(q, "q", self.batch, 0, d, self.device)
-        B, Hq, T, dq = q.shape
-        D = c.D
+        # zero columns leave the logits unchanged and give zero output columns
+        q = _rows(q, "q", self.batch, 0, d, self.device, c.D)
+        B, Hq, T, D = q.shape
         if window < 0:
             raise RuntimeError("tbf16.PagedCache.attend: window must not be negative")
-        if dq != D:  # zero columns leave the logits unchanged and give zero output columns
-            q = torch.nn.functional.pad(q, (0, D - dq))
         sizes = self._sizes.get((Hq, T))
         if sizes is None:
             if Hq == 0 or Hq % self.kv_heads:
