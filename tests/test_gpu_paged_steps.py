@@ -150,3 +150,19 @@ def test_rows_of_any_layout_with_a_padded_head_dim():
             c.append(lay(k), lay(v))
             c.out = c.attend(lay(q)), c.attend(lay(q)[:, :, :1].transpose(2, 3).contiguous().transpose(2, 3))
         assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v) and all(torch.equal(x, y) for x, y in zip(a.out, b.out))
+
+
+def test_advance_is_refused_inside_a_capture():
+    """The lengths are the host's: a recorded upload would put the same ones back with every replay."""
+    import tbf16
+    c = tbf16.PagedCache(2, 2, 64, 100, page_size=16, track=True)
+    c.advance(5)
+    x, graph = torch.zeros(4, device=DEV), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        for fn in (lambda: c.advance(1), lambda: c.release(0), lambda: c.evict(3)):
+            with pytest.raises(RuntimeError):
+                fn()
+    assert c.lengths == [5, 5] and c.pool.seen == [5, 5]
+    c.advance(1)
+    assert c.lens.tolist() == [6, 6]

@@ -229,6 +229,14 @@ class PagedCache:
             raise RuntimeError(f"tbf16.PagedCache.{what}: this cache is over buffers that the caller manages")
         return self.pool
 
+    def _stepping(self, what) -> PagePool:
+        """The pool, for a call that changes it. Its upload would be recorded by a capture, with these lengths."""
+        pool = self._owned(what)
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"tbf16.PagedCache.{what}: not inside a graph capture; call it before each replay")
+        return pool
+
     @property
     def lengths(self):
         """The host's copy of lens."""
@@ -238,11 +246,11 @@ class PagedCache:
         """Makes room for counts new tokens (an int for every sequence, or one int each): takes pages from the
         pool and raises lens and seen. Call it once a step, before `append` and `attend` of every layer, which take
         these counts unless they are given others."""
-        self._upload(table=self._owned("advance").advance(counts))
+        self._upload(table=self._stepping("advance").advance(counts))
 
     def release(self, sequence):
         """Forgets a sequence: its slot is empty again and its pages go back to the pool."""
-        pool = self._owned("release")
+        pool = self._stepping("release")
         pool.cut(sequence, 0)
         pool.seen[sequence] = 0
         if self.weights is not None:
@@ -362,7 +370,7 @@ class PagedCache:
         """`compact` for every layer, then the lengths: sequences longer than keep are keep long from here on,
         and pages that hold nothing any more go back to the pool. Cached order is no longer token order
         (`pos` has the token numbers), so a `window` no longer means the newest tokens."""
-        pool = self._owned("evict")
+        pool = self._stepping("evict")
         for i, c in enumerate(self._layers):
             weights, pos = self.compact(keep, recent, i)
             c.weights.copy_(weights)
