@@ -166,3 +166,52 @@ def test_advance_is_refused_inside_a_capture():
     assert c.lengths == [5, 5] and c.pool.seen == [5, 5]
     c.advance(1)
     assert c.lens.tolist() == [6, 6]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_drafts_that_were_not_accepted(dtype):
+    """After a rewind the cache goes on as one that never had those tokens: rows, numbers and lengths, outputs, and the
+    weights of the positions that are used again."""
+    import tbf16
+    from tbf16 import _ext
+    kw = dict(layers=2, page_size=16, track=True, dtype=dtype)
+    a, b = (tbf16.PagedCache(3, 2, 64, 100, pages=16, **kw) for _ in range(2))
+    k, v, q = _rows(3, 2, 30, 64)
+    for c in (a, b):
+        c.advance([30, 15, 1])
+        for layer in range(2):
+            c.append(k, v, layer)
+            c.attend(q[:, :, :1], layer)
+    start = a.weights.clone()
+    k, v, q = _rows(3, 2, 4, 64, seed=1)
+    accepted = [1, 2, 0]
+    a.advance(4)
+    for layer in range(2):
+        a.append(k, v, layer)
+        drafts = a.attend(q, layer)
+    a.rewind([4 - c for c in accepted])
+    b.advance(accepted)
+    for layer in range(2):
+        b.append(k, v, layer)
+        got = b.attend(q, layer)
+    for s, c in enumerate(accepted):
+        assert torch.allclose(drafts[s, :, :c].float(), got[s, :, :c].float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+    assert a.lengths == b.lengths == [31, 17, 1] and a.lens.tolist() == a.lengths and torch.equal(a.pos, b.pos)
+    for s, n in enumerate(a.lengths):
+        assert not a.weights[:, s, :, n:].any() and bool((a.weights[:, s, :, :n] >= start[:, s, :, :n]).all())
+    a.weights.copy_(b.weights)
+    for step in range(20):  # over the positions given back, and into pages that another sequence gave back
+        k, v, q = _rows(3, 2, 2 if step == 0 else 1, 64, seed=step + 2)
+        outs = []
+        for c in (a, b):
+            c.advance([1, 1, 2 if step == 0 else 1])
+            outs.append([(c.append(k, v, layer), c.attend(q, layer))[1] for layer in range(2)])
+        assert all(torch.equal(x, y) for x, y in zip(*outs))
+        assert torch.equal(a.weights, b.weights) and torch.equal(a.pos, b.pos) and torch.equal(a.lens, b.lens)
+    assert torch.equal(a.seen, b.seen) and sorted(a.pool.free) == sorted(b.pool.free)
+    a.evict(20)
+    with pytest.raises(RuntimeError):
+        a.rewind([1, 0, 0])
+    a.advance([2, 0, 0])
+    a.rewind([2, 0, 0])
+    assert a.lengths == [20, 20, 20] and _ext.device_status() == 0

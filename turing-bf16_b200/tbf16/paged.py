@@ -4,6 +4,7 @@
     cache.advance(T)                        # room for T new tokens of every sequence (or a count for each)
     cache.append(k, v, layer)               # k, v (B, kv_heads, T, head_dim): into the pages, by those counts
     out = cache.attend(q, layer)            # q (B, heads, T, head_dim): attention over everything cached
+    cache.rewind(counts)                    # drafts that were not accepted: the newest tokens of each sequence go
     cache.evict(keep, recent)               # with track=True: cut every head to its heaviest positions
 
 `append` writes bf16 rows as they are, or as e4m3 rows with an exact power-of-two scale from the row's
@@ -97,16 +98,14 @@ class PagePool:
     def __init__(self, batch, pages, page_size, max_len):
         self.page_size, self.max_len = page_size, max_len
         self.lengths, self.seen, self.fresh = [0] * batch, [0] * batch, [0] * batch  # fresh: of the last advance
+        self.fixed = [0] * batch  # positions that an eviction has reordered: they cannot be rewound into
         self.owned = [[] for _ in range(batch)]
         self.free = list(range(pages - 1, -1, -1))
 
     def advance(self, counts) -> bool:
         """Adds counts tokens; takes the pages they need. Returns whether the table changed. Changes nothing
         when it raises."""
-        batch = len(self.lengths)
-        counts = [counts] * batch if isinstance(counts, int) else [int(c) for c in counts]
-        if len(counts) != batch or min(counts) < 0:
-            raise RuntimeError(f"tbf16.PagedCache.advance: {batch} counts of at least 0 expected, got {counts}")
+        counts = self._counts(counts, "advance")
         new = [n + c for n, c in zip(self.lengths, counts)]
         if max(new) > self.max_len:
             raise RuntimeError(f"tbf16.PagedCache.advance: a sequence would pass max_len = {self.max_len}")
@@ -118,6 +117,24 @@ class PagePool:
         self.lengths, self.fresh = new, counts
         self.seen = [s + c for s, c in zip(self.seen, counts)]
         return any(want)
+
+    def _counts(self, counts, what):
+        batch = len(self.lengths)
+        counts = [counts] * batch if isinstance(counts, int) else [int(c) for c in counts]
+        if len(counts) != batch or min(counts) < 0:
+            raise RuntimeError(f"tbf16.PagedCache.{what}: {batch} counts of at least 0 expected, got {counts}")
+        return counts
+
+    def rewind(self, counts):
+        """Takes the newest counts tokens back, as if they had never come. Changes nothing when it raises."""
+        counts = self._counts(counts, "rewind")
+        for b, (n, c, least) in enumerate(zip(self.lengths, counts, self.fixed)):
+            if c and n - c < least:
+                raise RuntimeError(f"tbf16.PagedCache.rewind: sequence {b} can lose {n - least} tokens, not {c}")
+        for b, c in enumerate(counts):
+            self.cut(b, self.lengths[b] - c)
+            self.seen[b] -= c
+            self.fresh[b] = max(0, self.fresh[b] - c)
 
     def cut(self, sequence, length):
         """Shortens a sequence to at most `length` tokens and frees the pages past them."""
@@ -172,7 +189,7 @@ class PagedCache:
         """A one-layer cache over the caller's buffers: pools (pages, kv_heads, page_size, D) with any
         16-byte strides, table (batch, max_pages) and lens (batch) int32; e4m3 pools take k_scale and v_scale
         (pages, kv_heads, page_size). weights / pos / seen as in the class. The caller manages pages, table and
-        lens; `advance`, `release` and `evict` are for caches that own them."""
+        lens; `advance`, `rewind`, `release` and `evict` are for caches that own them."""
         self = cls.__new__(cls)
         up = lambda x: None if x is None else x.unsqueeze(0)  # noqa: E731
         self._init(up(k), up(v), up(k_scale), up(v_scale), table, lens, seen, up(weights), up(pos), head_dim or k.shape[-1])
@@ -248,11 +265,26 @@ class PagedCache:
         these counts unless they are given others."""
         self._upload(table=self._stepping("advance").advance(counts))
 
+    def rewind(self, counts):
+        """Takes back the newest tokens (an int for every sequence, or one int each), as after drafts that were not
+        accepted: lens and seen fall, pages past them go back to the pool, their weights and token numbers are
+        cleared. What their queries added to the weights of earlier positions stays. Tokens that an `evict` has
+        reordered cannot be taken back."""
+        pool = self._stepping("rewind")
+        old = list(pool.lengths)
+        pool.rewind(counts)
+        if self.weights is not None:
+            for b, (n, new) in enumerate(zip(old, pool.lengths)):
+                if new < n:
+                    self.weights[:, b, :, new:n] = 0
+                    self.pos[:, b, :, new:n] = -1
+        self._upload(table=False)
+
     def release(self, sequence):
         """Forgets a sequence: its slot is empty again and its pages go back to the pool."""
         pool = self._stepping("release")
         pool.cut(sequence, 0)
-        pool.seen[sequence] = 0
+        pool.seen[sequence] = pool.fixed[sequence] = 0
         if self.weights is not None:
             self.weights[:, sequence] = 0
             self.pos[:, sequence] = -1
@@ -375,6 +407,8 @@ class PagedCache:
             weights, pos = self.compact(keep, recent, i)
             c.weights.copy_(weights)
             c.pos.copy_(pos)
-        for b in range(self.batch):
-            pool.cut(b, keep)
+        for b, n in enumerate(pool.lengths):
+            if n > keep:
+                pool.cut(b, keep)
+                pool.fixed[b] = keep
         self._upload(table=False)
