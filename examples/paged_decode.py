@@ -5,7 +5,8 @@
 The prompts go through tbf16.sdpa (F.scaled_dot_product_attention, routed by tbf16.convert) and into the cache; every
 decoding step is one captured CUDA graph: linears on the weight-streaming kernels, QK-norm and rotary embedding in one
 pass, cache.append, cache.attend. With --keep the cache is cut to that many positions per head whenever it has grown
-64 past them, by the attention weight each position has received. Weights are random: the tokens mean nothing.
+64 past them, by the attention weight each position has received from the prompt's last 32 tokens (cache.attend on
+their queries; sdpa leaves no weights) and from the tokens decoded. Weights are random: the tokens mean nothing.
 """
 import argparse
 import pathlib
@@ -18,6 +19,9 @@ import torch.nn.functional as F
 sys.path.insert(0, str(pathlib.Path(__file__).resolve().parents[1] / "turing-bf16_b200"))
 import tbf16  # noqa: E402
 from tbf16 import ops  # noqa: E402
+
+
+LAST = 32  # queries of a prompt whose attention weights a cut goes by
 
 
 class Layer(torch.nn.Module):
@@ -75,6 +79,12 @@ class Decoder(torch.nn.Module):
             q, k, v = (t.view(B, S, -1, self.head_dim).transpose(1, 2) for t in layer.qkv(x, cos, sin))
             cache.append(k, v, i, counts=counts)
             a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
+            if cache.weights is not None:
+                # the newest tokens of each prompt, the first rows of T: attend takes as many as a prompt has
+                T = min(LAST, S)
+                at = (counts - counts.clamp(max=T))[:, None] + torch.arange(T, device=x.device)
+                last = q.transpose(1, 2)[torch.arange(B, device=x.device)[:, None], at.clamp(max=S - 1)]
+                cache.attend(last.transpose(1, 2), i)
             x = layer.rest(x, a.transpose(1, 2).reshape(B * S, -1))
         last = x.view(B, S, -1)[torch.arange(B, device=x.device), (counts - 1).long()]
         return self.head(ops.rmsnorm(last, self.norm))

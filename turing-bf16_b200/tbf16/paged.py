@@ -12,7 +12,8 @@ largest exponent (the same idea as the fp16 rows of the linears, at half the byt
 attention of the newest token or few tokens (decode, draft verification) over the pages; with `track=True`
 it also adds each cached position's attention weight to `cache.weights`. `evict` keeps, per head, the
 positions with the largest weights and closes the holes in place (`compact` does one layer). Prompts take
-tbf16.sdpa on the prompt's own k and v, after `append`.
+tbf16.sdpa on the prompt's own k and v, after `append`; sdpa leaves no weights, so where a cut is to know a
+prompt, `attend` on the queries of its last tokens starts them.
 
 Everything a kernel reads that changes from step to step (page table, lengths) lives on the GPU, so a
 decoding step can be captured in a CUDA graph and replayed after `advance`. No host synchronisation.
