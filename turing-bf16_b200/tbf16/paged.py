@@ -20,7 +20,6 @@ decoding step can be captured in a CUDA graph and replayed after `advance`. No h
 The reference has no counterpart: it leaves calls with few query rows to torch (tbf16/convert.py there).
 """
 import ctypes
-import functools
 
 import torch
 
@@ -57,18 +56,6 @@ def _rows(x, name, B, H, d, device, width):
         # clone: also rewrites odd strides of dimensions of one element, which count as contiguous
         x = x.clone(memory_format=torch.contiguous_format)
     return x
-
-
-def _on_its_device(fn):
-    """A method of PagedCache that runs with the cache's device as the current one: the library's size queries, the
-    question whether a capture is on, allocations and launches all go by that."""
-    @functools.wraps(fn)
-    def call(self, *args, **kw):
-        if torch._C._cuda_getDevice() == self.device.index:
-            return fn(self, *args, **kw)
-        with torch.cuda.device(self.device):
-            return fn(self, *args, **kw)
-    return call
 
 
 class _Layer:
@@ -307,6 +294,12 @@ class PagedCache:
             raise RuntimeError(f"tbf16.PagedCache: counts must be a contiguous int32 ({self.batch},) tensor on {self.device}")
         return counts.data_ptr()
 
+    def _elsewhere(self, call, *args):
+        """A call made while another device is current: again, with the cache's current. The library's size queries, the
+        question whether a capture is on, allocations and launches all go by that."""
+        with torch.cuda.device(self.device):
+            return call(*args)
+
     def _run(self, fn, what, *args):
         status = fn(*args)
         if status:
@@ -327,12 +320,13 @@ class PagedCache:
 
     # ------------------------------------------------------------------------------------------- operators
 
-    @_on_its_device
     def append(self, k, v, layer=0, counts=None):
         """Writes the newest rows of every sequence into the pages: k, v bf16 (B, kv_heads, T, head_dim), any
         strides. lens counts them already (`advance`). counts: int32 (B,) on the GPU, the tokens that are real
         in each sequence (the first ones of its T; default: those of the last `advance`, at most T; over a caller's
         buffers T, or lens where that is less)."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            return self._elsewhere(self.append, k, v, layer, counts)
         c, d = self._layers[layer], self.head_dim
         k = _rows(k, "k", self.batch, self.kv_heads, d, self.device, d + -d % 8)
         v = _rows(v, "v", self.batch, self.kv_heads, d, self.device, d + -d % 8)
@@ -344,13 +338,14 @@ class PagedCache:
         self._run(self._lib.tbf16_paged_append, "append", c.ref, k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T, d,
                   self._counts(counts), *c.pos_args, torch._C._cuda_getCurrentRawStream(self.device.index))
 
-    @_on_its_device
     def attend(self, q, layer=0, counts=None, scale=None, window=0):
         """Attention of the newest T tokens over the cache: q bf16 (B, heads, T, head_dim), heads a multiple of
         kv_heads -> bf16 of the same shape, over (B, T, heads, head_dim) memory as tbf16.sdpa returns it. counts as in
         `append`. Token t of a sequence sits at position lens - counts + t and sees the positions up to its own; window > 0: only
         the last `window` of them. Rows past counts, and rows that see nothing, are zeros. A tracking cache adds
         the attention weights to `weights`."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            return self._elsewhere(self.attend, q, layer, counts, scale, window)
         c, d = self._layers[layer], self.head_dim
         # zero columns leave the logits unchanged and give zero output columns
         q = _rows(q, "q", self.batch, 0, d, self.device, c.D)
@@ -376,12 +371,13 @@ class PagedCache:
                   ptr + buf.sync, size, stream)
         return out[..., :d] if d != D else out
 
-    @_on_its_device
     def compact(self, keep, recent=0, layer=0):
         """Cuts one layer's sequences to their `keep` heaviest positions per head, the newest `recent` tokens
         first of all, and moves the kept rows that lie beyond `keep` into the holes. Returns (weights, pos) in
         the new order, 0 and -1 past the end; weights, pos and lens of the cache are left as they were, so that
         every layer sees the same lengths (`evict` does all layers and then takes over the results)."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            return self._elsewhere(self.compact, keep, recent, layer)
         c = self._layers[layer]
         if c.weights is None or c.pos is None or self.seen is None:
             raise RuntimeError("tbf16.PagedCache.compact: needs a cache with weights, pos and seen (track=True)")
