@@ -410,7 +410,9 @@ int tbf16_attn_bwd_sharded(const void* q16, const void* k16, const void* v16, co
  * j % page_size of page table[b * table_ld + j / page_size]; lens[b] tokens are cached. table, lens,
  * counts and fresh are read on the device, so a captured graph follows their contents.
  *
- * Limits: D 64, 128 or 256 (zero-pad others); page_size a power of two from 16 to 1024; batch up to 1024;
+ * Limits: D 64, 128 or 256 (zero-pad others); page_size a power of two from 16 to 1024; batch up to 1024; attend: T up to
+ * 4096, T * Hq / heads up to 65536, and, as sums stay undivided until their end, visible values below 2^119 over the
+ * number of positions;
  * pointers and strides multiples of 16 bytes (scales: 16-byte pointers, strides multiples of 4 floats,
  * the page_size scales of a (page, head) contiguous). Page numbers outside [0, pages), lengths outside
  * [0, max_pages * page_size], counts outside [0, min(T, lens)] and negative fresh set bit 8 of the device status word. */
@@ -445,6 +447,9 @@ int tbf16_paged_append(const tbf16_paged_cache* cache, const void* k, int64_t k_
  * Hq a multiple of heads (query head h reads key/value head h / (Hq / heads)). Token t < counts[b]
  * (NULL: as for append) sits at position i = lens[b] - counts[b] + t and sees the cached positions j
  * with i - window < j <= i (window 0: all j <= i). Rows that see nothing, and tokens t >= counts[b], give zeros.
+ * Logits, maxima, sums and outputs are fp32. Softmax weights meet bf16 values with 16 bits, and e4m3 values with 11, the
+ * value row's scale among them (fewer below 2^-10 of the row's largest weight times scale); queries meet e4m3 keys as
+ * fp16, after a power of two that takes the row's largest element to [2^14, 2^15).
  * weights (nullable): fp32 (batch, heads, capacity) with strides w_sb, w_sh; the softmax weight of every
  * visible position, summed over the head's query heads and the new tokens, is added to it.
  * sync: tbf16_paged_attend_sync_size() bytes that are zero before the first call; every call leaves them

@@ -81,7 +81,8 @@ __host__ __device__ constexpr int partial_floats(int nr, int D) { return (nr * (
 
 // In the order of all blocks each item is followed by kPad places that hold none: what an item costs a CTA beyond its
 // blocks (loading its queries, waiting for its last warp, adding the warps up), so that CTAs with many short items get
-// fewer keys.
+// fewer keys. One number for all tiles: 64 ragged sequences up to 3000 tokens, 16 query heads on 4, with 8 / 24 / 48 take
+// bf16 35 / 30 / 31 us (D 64), 48 / 43 / 43 (128), 77 / 73 / 75 (256), e4m3 33 / 31 / 34, 46 / 40 / 40, 64 / 59 / 55.
 constexpr int kPad = 24;
 
 // What a CTA knows of a sequence: the first of its blocks, and of its rounds, among all; cached and new tokens.
@@ -355,8 +356,11 @@ __global__ void __launch_bounds__(C::W * 32, 1)
   // Sequences of one length with fewer items than SMs: as many CTAs for each item, so that none has the end of one and
   // the start of the next to add up and join (128 items of 8000 tokens: 92 us with all SMs, 84 with 128). Leaving SMs
   // out pays while the others' loads fill the memory's queues: down to four fifths of them, or three where a CTA's bf16
-  // part is up to 2 MB, start and end a large part of its time (96 items of 1 MB: 29 us with all, 26.6 with 96; of
-  // 8000 tokens 72 and 71; of 8000 e4m3 tokens, bound by instructions, 53 and 62).
+  // part is up to 2 MB, start and end a large part of its time. bf16 items of 0.5 / 1 / 2 / 8 MB, all SMs: 80 of them
+  // 18.1 / 25.3 / 37.1 / 108 us, 96 21.9 / 29.3 / 43.1 / 128, 112 24.4 / 32.2 / 47.9 / 146, 128 25.8 / 35.0 / 52.8 / 165;
+  // whole CTAs: 80 17.5 / 25.5 / 41.1 / 133, 96 18.4 / 26.7 / 42.3 / 134, 112 19.5 / 28.4 / 45.0 / 144, 128 20.4 / 30.4 /
+  // 48.8 / 159. e4m3 items, bound by instructions, of 4 MB: 96 of them 77 and 98, 128 97 and 99 (below 1 MB whole CTAs
+  // would win there too, down to 80 items: 0.25 MB 18.7 and 15.9).
   const bool by_round = work <= (int)gridDim.x;
   const int items = p.c.batch * p.c.heads * p.chunks, per_item = items <= (int)gridDim.x ? gridDim.x / items : 0;
   const bool small = !E4M3 && longest <= per_item * ((2 << 20) / (2 * C::KB));
@@ -1093,7 +1097,7 @@ template <int D, bool E4M3>
 int launch_rows(const tbf16_paged_cache* cache, AttendParams& p, const tbf16_host::DeviceInfo* dev, cudaStream_t st) {
   // Up to 16 rows in one warp: a cached fragment is read from shared memory and converted once for both tiles. 256-wide
   // outputs of two tiles would not fit a warp's registers; there, and for 32 rows, two or four warps share a block
-  // (16 query heads on one of 128, 8 sequences of 32768 tokens: two tiles 39 us, two warps 51; on one of 256: 80 and 68).
+  // (16 query heads on one of 128, 8 sequences of 32768 tokens: two tiles 36 us, two warps 51; on one of 256: 80 and 64).
   constexpr bool WIDE = D == 256;
   const int R = item_rows(p.rows);
   if (R == 8) return launch_attend<Tile<D, E4M3, 1, 1>>(cache, p, dev, st);
